@@ -3,9 +3,9 @@ its cache runs on every layer of every step.
 
 * ``window``  - attention over the paged cache with a sliding window and a few first tokens
   that stay visible: ``PagedBatch(..., window=, sinks=).write_and_attend(layer, q, k, v)``.
-* ``weights`` - the same call, or the unwindowed one, that also adds up per cached token and
-  KV head the attention weight it got: ``write_and_attend(..., weights="add" | "replace")``
-  on a pool made with ``track_weights=True``.
+* ``weights`` - the same step, windowed or not, that also adds up per cached token and KV head
+  the attention weight it got: ``PagedBatch(..., weights="add" | "replace")`` on a pool made
+  with ``track_weights=True``.
 * ``evict``   - per layer, sequence and KV head, the ``budget`` tokens worth keeping (first
   tokens, recent tokens, then the largest accumulated weights, ties to the lowest position)
   moved in order into the sequence's new blocks: ``pool.evict(...)``.
@@ -263,7 +263,9 @@ def prepare(case, seed):
     s.vn = _fill(torch.empty((rows, kvh, D), dtype=dt, device="cuda"), seed, 5)
     s.w0 = s.w.clone() if case["mode"] == "add" else None
     if own:
-        s.batch = PagedBatch(s.pool, tables, starts, new, window=case["window"] or None, sinks=case["sinks"])
+        mode = None if case["mode"] == "none" else case["mode"]
+        s.batch = PagedBatch(s.pool, tables, starts, new, window=case["window"] or None, sinks=case["sinks"],
+                             weights=mode)
     else:
         _plan_attend(s, tables, starts, new)
     return s
@@ -392,12 +394,12 @@ def run(s):
         return {"k": s.k, "v": s.v, "weights": s.w, "kept": kept}
     if not own:
         return _attend_plain(s)
-    if c["mode"] == "none":
-        return {"out": s.batch.write_and_attend(0, s.q, s.kn, s.vn), "k": s.k, "v": s.v}
     if s.w0 is not None:  # every pass starts from the same sums
         s.w.copy_(s.w0)
-    return {"out": s.batch.write_and_attend(0, s.q, s.kn, s.vn, weights=c["mode"]), "k": s.k, "v": s.v,
-            "weights": s.w}
+    res = {"out": s.batch.write_and_attend(0, s.q, s.kn, s.vn), "k": s.k, "v": s.v}
+    if s.w is not None:
+        res["weights"] = s.w
+    return res
 
 
 # ------------------------------------------------------------------ the definition, in 64 bits
