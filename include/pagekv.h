@@ -86,6 +86,30 @@ PK_API int pk_pool_copy_blocks_dev(pk_pool* pool, const int64_t* pairs_dev, int6
 PK_API int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const float* v_dev,
                    const int64_t* slots_dev, int64_t n, void* stream);
 
+/* Accumulated attention weights (no counterpart in pagellm): float32
+ * [layers][num_blocks][n_kv_heads][block_size], zero-filled, one value per layer, token slot
+ * and KV head, owned by the pool from the first call on (later calls return the same
+ * memory). They belong to the block: sequences that share a block share its weights. pk_pool_copy_blocks copies a block's weights with it; pk_batch_set_bounds makes
+ * steps keep them up and pk_pool_evict goes by them. */
+PK_API int pk_pool_track_weights(pk_pool* pool, float** weights_dev);
+/* Shortens cached sequences to the tokens worth keeping (no counterpart in pagellm, whose
+ * caches only grow). For every layer, sequence i and KV head, a sequence of lengths[i] > budget
+ * tokens keeps its first `sinks`, its last `recent` and, of the rest, those with the largest
+ * accumulated weights, `budget` in all; equal weights go to the lowest position, NaN counts as
+ * the largest, -0 as 0. A shorter one keeps all its tokens. The kept tokens' K, V and weights
+ * move in order to positions 0..min(lengths[i], budget)-1 of new table i; slots behind them
+ * are left as they were. Layers and heads keep different tokens, so positions of the shortened
+ * cache are cache indices, no longer the tokens' places in the text. Tables: host CSR as in
+ * pk_batch_plan. A block of a new table must not be read by this call, with one exception: it
+ * may be the old block at its own index of the same sequence, if no other sequence reads that
+ * (eviction in place); and no block may appear twice in the new tables.
+ * kept_dev: NULL, or int32 [layers][nseq][n_kv_heads][budget] that receives the kept positions
+ * in ascending order, -1 behind the last. Uploads its tables from host memory of the call:
+ * a capturing stream gets PK_ERR_UNSUPPORTED. */
+PK_API int pk_pool_evict(pk_pool* pool, int nseq, const int64_t* table_indptr, const int32_t* table_ids,
+                  const int64_t* lengths, const int64_t* new_indptr, const int32_t* new_ids, int64_t budget,
+                  int64_t sinks, int64_t recent, int32_t* kept_dev, void* stream);
+
 /* slot_mapping (cache/paged.py:303-306): slots[i] = table[p / bs] * bs + p % bs for
  * p = positions[i]. Device arrays. A position outside [0, table_len * bs) yields slot
  * -1 and, if err_dev is not NULL, sets *err_dev to 1. */
@@ -97,6 +121,19 @@ PK_API int pk_slot_mapping(const int32_t* table_dev, int64_t table_len, const in
  * Replaces PagedBatch (cache/paged.py:383-464): the per-step view of a set of sequences.
  * A batch object is reusable across steps; its device buffers only grow. */
 PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
+/* Bounds of the batch's next plans (no counterpart in pagellm, whose attention always sees the
+ * whole cache). window > 0: the row at position p sees the keys j <= p with j < sinks or
+ * j > p - window (0 = no window; then sinks must be 0); blocks without a visible key are not
+ * read, so their table entries only have to be valid ids. weights_mode 1 (add) / 2 (replace),
+ * on pools with pk_pool_track_weights: every call also sums, per cached token and KV head, the
+ * softmax weight that the step's rows and the KV head's query heads give the token, and adds
+ * it to the token's accumulated weight or puts it in its place. Tokens of the step itself
+ * always start anew; tokens that no row sees keep their weight. With weights, a block that is
+ * read must appear only once in the step (PK_ERR_INVALID_ARG from pk_batch_plan otherwise).
+ * After a change the batch has to be planned again before it attends. A bounded step's first
+ * call with some n_heads cannot be captured (PK_ERR_UNSUPPORTED); later ones can, and graphs
+ * that were captured from one batch share its scratch: replay them one after another. */
+PK_API int pk_batch_set_bounds(pk_batch* batch, int64_t window, int64_t sinks, int weights_mode);
 PK_API int pk_batch_destroy(pk_batch* batch);
 /* PagedBatch.__init__ (:397-439). Host arrays: block tables in CSR form
  * (table_indptr[nseq+1] int64, table_ids int32), starts[nseq], n_new[nseq] (int64).
@@ -119,6 +156,10 @@ PK_API int pk_batch_write_and_attend(pk_batch* batch, int layer, int n_heads, co
 /* Attention only (no append): the read half of write_and_attend. */
 PK_API int pk_batch_attend(pk_batch* batch, int layer, int n_heads, const float* q_dev, float* out_dev,
                     void* stream);
+/* pk_batch_write_and_attend for a bounded step (pk_batch_set_bounds) of a bf16 pool whose q, k, v
+ * and out rows are bf16; k_dev = v_dev = NULL: attention only. */
+PK_API int pk_batch_write_and_attend_bf16(pk_batch* batch, int layer, int n_heads, const void* q_dev,
+                                   const void* k_dev, const void* v_dev, void* out_dev, void* stream);
 /* write_and_attend from HOST buffers: uploads q/k/v, runs the layer and downloads out,
  * all on `stream`; returns after `out_host` is filled (synchronous). When `out_host` lies
  * wholly inside one page-locked allocation the device can address (cudaMallocHost,
@@ -168,6 +209,16 @@ PK_API int pk_selftest_bounded_wait(int device, int64_t limit_ns, int* timed_out
  * (write_and_attend / attend, any batch) returns PK_ERR_CUDA before launching anything, as
  * a failed launch would; later calls run normally. No GPU fault is involved. */
 PK_API int pk_test_inject_launch_failure(void);
+/* Host-only dry runs of the bounded steps' planners (no device needed). pk_plan_evict makes the
+ * checks of pk_pool_evict for a pool of num_blocks blocks and counts the pieces in which rows
+ * move (one for a sequence that is thinned out in place). pk_plan_visible_blocks: the table
+ * entries that hold a key some row at positions first_position .. context - 1 sees:
+ * blocks3[0] leading ones (sinks), then, blocks3[1] entries later, the rest of blocks3[2]. */
+PK_API int pk_plan_evict(int64_t num_blocks, int block_size, int nseq, const int64_t* table_indptr,
+                  const int32_t* table_ids, const int64_t* lengths, const int64_t* new_indptr,
+                  const int32_t* new_ids, int64_t budget, int64_t sinks, int64_t recent, int64_t* n_items);
+PK_API int pk_plan_visible_blocks(int64_t first_position, int64_t context, int64_t window, int64_t sinks,
+                           int block_size, int64_t* blocks3);
 /* Host-only dry run of the split-KV planner (no device needed). The units' blocks, end to
  * end, are cut into contiguous CTA ranges; a range costs its blocks plus
  * `unit_switch_blocks` per unit boundary inside it (a CTA that crosses into another unit
@@ -305,6 +356,17 @@ PK_API int pk_bm_fork(pk_block_manager* m, int64_t parent, int64_t child);
  * prefix cache and held by this sequence alone is unpublished (its next writes change it).
  * n_tokens outside [0, blocks * block_size] -> PK_ERR_INVALID_ARG. */
 PK_API int pk_bm_truncate(pk_block_manager* m, int64_t seq, int64_t n_tokens);
+/* The table of a sequence that pk_pool_evict shortens to n_tokens (no counterpart in pagellm):
+ * its first blocks_needed(n_tokens) blocks, where a block that other sequences hold too, or
+ * that the prefix cache has published, is exchanged for a fresh one. The old table goes to
+ * old_out (up to cap ids, count in *n_old); blocks that are no longer in the table are released
+ * last block first, so run the eviction before anything else writes to the pool. The
+ * sequence's hash chain ends: its blocks no longer hold a prefix of its tokens, and later
+ * pk_bm_seq_push_hashes calls for it publish nothing. n_tokens outside
+ * [0, blocks * block_size] -> PK_ERR_INVALID_ARG; too few free blocks -> PK_ERR_OUT_OF_BLOCKS;
+ * both change nothing. */
+PK_API int pk_bm_compact(pk_block_manager* m, int64_t seq, int64_t n_tokens, int32_t* old_out, int64_t cap,
+                         int64_t* n_old);
 PK_API int pk_bm_free_seq(pk_block_manager* m, int64_t seq);
 /* BlockManager.block_table (paged.py:273-274); sequence ids with a table. */
 PK_API int pk_bm_table(const pk_block_manager* m, int64_t seq, int32_t* out, int64_t cap,

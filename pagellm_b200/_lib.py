@@ -42,6 +42,8 @@ SIGNATURES: dict[str, tuple] = {
     "pk_pool_tc_info": (_i32, [_p, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32), C.POINTER(C.c_char_p)]),
     "pk_pool_copy_blocks": (_i32, [_p, _pi64, _i64, _p]),
     "pk_pool_copy_blocks_dev": (_i32, [_p, _p, _i64, _p]),
+    "pk_pool_track_weights": (_i32, [_p, C.POINTER(_p)]),
+    "pk_pool_evict": (_i32, [_p, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p]),
     "pk_pool_append": (_i32, [_p, _i32, _p, _p, _p, _i64, _p]),
     "pk_slot_mapping": (_i32, [_p, _i64, _p, _i64, _i32, _p, _p, _p]),
     "pk_batch_create": (_i32, [_p, C.POINTER(_p)]),
@@ -51,6 +53,8 @@ SIGNATURES: dict[str, tuple] = {
     "pk_batch_write_and_attend": (_i32, [_p, _i32, _i32, _p, _p, _p, _p, _p]),
     "pk_batch_attend": (_i32, [_p, _i32, _i32, _p, _p, _p]),
     "pk_batch_write_and_attend_host": (_i32, [_p, _i32, _i32, _p, _p, _p, _p, _p]),
+    "pk_batch_write_and_attend_bf16": (_i32, [_p, _i32, _i32, _p, _p, _p, _p, _p]),
+    "pk_batch_set_bounds": (_i32, [_p, _i64, _i64, _i32]),
     "pk_batch_check": (_i32, [_p, _p]),
     "pk_batch_stats": (_i32, [_p, _pi64]),
     "pk_batch_io_stats": (_i32, [_p, _pi64]),
@@ -58,6 +62,8 @@ SIGNATURES: dict[str, tuple] = {
     "pk_bm_truncate": (_i32, [_p, _i64, _i64]),
     "pk_batch_set_prefix_sharing": (_i32, [_p, _i32]),
     "pk_batch_prefix_stats": (_i32, [_p, _pi64]),
+    "pk_plan_evict": (_i32, [_i64, _i32, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i64, _pi64]),
+    "pk_plan_visible_blocks": (_i32, [_i64, _i64, _i64, _i64, _i32, _pi64]),
     "pk_plan_partition": (_i32, [_pi64, _i64, _i32, _i32, _pi64, C.POINTER(_i32)]),
     "pk_gather_interleave": (_i32, [_p, _p, _i32, _i64, _i64, _p]),
     "pk_peer_gather_create": (_i32, [_i32, _i32, _i32, _i64, C.POINTER(_p)]),
@@ -95,6 +101,7 @@ SIGNATURES.update({
     "pk_bm_seq_hashes": (C.c_int, [_p, _i64, _pi64, C.c_char_p, _i64, _pi64]),
     "pk_bm_seq_hash_at": (C.c_int, [_p, _i64, _i64, C.c_char_p, _i64, _pi64]),
     "pk_bm_seq_push_hashes": (C.c_int, [_p, _i64, C.c_char_p, _i64, _i64]),
+    "pk_bm_compact": (C.c_int, [_p, _i64, _i64, _pi32, _i64, _pi64]),
     "pk_bm_fork": (C.c_int, [_p, _i64, _i64]),
     "pk_bm_free_seq": (C.c_int, [_p, _i64]),
     "pk_bm_table": (C.c_int, [_p, _i64, _pi32, _i64, _pi64]),

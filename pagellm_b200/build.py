@@ -22,7 +22,7 @@ INCLUDE = ROOT / "include"
 LIB = PKG / "libpagekv.so"
 
 SOURCES = ["pk_api.cu", "pk_kernels.cu", "pk_attn_tc.cu", "pk_attn_wide.cu", "pk_block_manager.cpp", "pk_static.cu",
-           "pk_peer.cu"]
+           "pk_peer.cu", "pk_bounded.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -50,7 +50,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [
-        nvcc_path(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared",
+        nvcc_path(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-shared", "--threads", "0",
         "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
         "-DPK_BUILD", f"-I{INCLUDE}", f"-I{CSRC}",
         *(["-Xptxas", "-v"] if verbose else []),

@@ -1,7 +1,8 @@
 """Drop-in for pagellm's ``pagellm.cache`` paged KV cache, backed by libpagekv (CUDA, sm_100a)."""
 
 from .block_manager import BlockAllocator, BlockManager, BlockTable, OutOfBlocks, block_hash
-from .paged import PagedBatch, PagedKVPool, batched_decode_attention, paged_attention, slot_mapping
+from .paged import (PagedBatch, PagedKVPool, batched_decode_attention, evict_sequences, paged_attention,
+                    slot_mapping)
 
 __all__ = [
     "BlockAllocator",
@@ -12,6 +13,7 @@ __all__ = [
     "PagedKVPool",
     "batched_decode_attention",
     "block_hash",
+    "evict_sequences",
     "paged_attention",
     "slot_mapping",
 ]

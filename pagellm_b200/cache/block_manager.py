@@ -330,6 +330,21 @@ class BlockManager:
         ``ValueError`` if ``num_tokens`` is outside ``[0, blocks * block_size]``."""
         _ck(_L().pk_bm_truncate(self._n.ptr, int(seq_id), int(num_tokens)))
 
+    def compact(self, seq_id: int, num_tokens: int) -> tuple[list[int], list[int]]:
+        """(old, new) block tables of a sequence that ``PagedKVPool.evict`` shortens to
+        ``num_tokens``: the first blocks stay, except that a block held by other sequences too,
+        or published in the prefix cache, is exchanged for a fresh one. The rest go back to the
+        allocator, so run the eviction before anything else writes to the pool
+        (``evict_sequences`` does both). From then on the sequence publishes nothing in the
+        prefix cache: its blocks no longer hold a prefix of its tokens. Not in pagellm.
+        ``ValueError`` if ``num_tokens`` is outside ``[0, blocks * block_size]``,
+        ``OutOfBlocks`` if too few blocks are free; both change nothing."""
+        n = C.c_int64()
+        cap = max(1, len(self.block_table(seq_id)))
+        buf = (C.c_int32 * cap)()
+        _ck(_L().pk_bm_compact(self._n.ptr, int(seq_id), int(num_tokens), buf, cap, C.byref(n)))
+        return list(buf[: n.value]), self.block_table(seq_id)
+
     def block_table(self, seq_id: int) -> list[int]:
         return _ids_list(_L().pk_bm_table, self._n.ptr, int(seq_id))
 

@@ -6,6 +6,8 @@ Same names, arguments and errors as pagellm:
   GPU in a pool owned by libpagekv; ``.k/.v/.k_flat/.v_flat`` are torch views of it.
 * ``PagedBatch(pool, block_tables, starts, n_new, attn, batch_decode)`` (paged.py:383-464)
   with ``.positions``, ``.slots``, ``.offsets`` and ``write_and_attend(layer, q, k, v)``.
+* Bounded caches, which pagellm does not have: ``PagedBatch(..., window=, sinks=, weights=)``,
+  ``PagedKVPool(..., track_weights=True)``, ``PagedKVPool.evict`` and ``evict_sequences``.
 * ``slot_mapping``, ``paged_attention``, ``batched_decode_attention`` (paged.py:303-380).
 * ``BlockAllocator``, ``BlockManager``, ``BlockTable``, ``OutOfBlocks``, ``block_hash``
   (paged.py:38-274): bookkeeping on the host, free list / ref counts / LRU in C++.
@@ -35,6 +37,7 @@ __all__ = [
     "PagedKVPool",
     "batched_decode_attention",
     "block_hash",
+    "evict_sequences",
     "paged_attention",
     "slot_mapping",
 ]
@@ -121,9 +124,15 @@ class PagedKVPool:
     ``cfg`` is anything with ``n_layers``, ``n_kv_heads`` and ``head_dim`` (pagellm's
     ``ModelConfig`` works). ``dtype``: float32 (pagellm's default) or bfloat16. The pool is
     zero-filled like pagellm's ``np.zeros`` pool (paged.py:287-289).
+
+    ``track_weights``: the pool also holds ``weights``, float32 ``(layers, num_blocks,
+    kv_heads, block_size)``, zero at first: the attention weight that every cached token has
+    got, kept up by ``PagedBatch(..., weights=)``, moved by ``copy_blocks`` and ``evict``
+    (sequences that share a block share its weights).
     """
 
-    def __init__(self, cfg, num_blocks: int, block_size: int, dtype=np.float32, device=None):
+    def __init__(self, cfg, num_blocks: int, block_size: int, dtype=np.float32, device=None,
+                 track_weights: bool = False):
         torch = _torch()
         lib = _lib.load()
         self.block_size = int(block_size)
@@ -155,8 +164,15 @@ class PagedKVPool:
         flat = (self.n_layers, self.num_blocks * self.block_size, self.n_kv_heads, self.head_dim)
         self.k_flat = self.k.view(flat)
         self.v_flat = self.v.view(flat)
+        self.weights = None
+        if track_weights:
+            wp = C.c_void_p()
+            _lib.check(lib.pk_pool_track_weights(self._h.ptr, C.byref(wp)))
+            wshape = (self.n_layers, self.num_blocks, self.n_kv_heads, self.block_size)
+            self.weights = torch.as_tensor(_CudaArray(wp.value, wshape, "<f4", self._h), device=self.device)
         self._idle_batches: list[int] = []
         self._batch_prefix_mode: dict[int, int] = {}  # handle -> prefix-sharing mode it holds
+        self._batch_bounds: dict[int, tuple] = {}  # handle -> (window, sinks, weights mode) it holds
 
     # ------------------------------------------------------------------ pagellm API
     def copy_block(self, src: int, dst: int) -> None:
@@ -171,6 +187,38 @@ class PagedKVPool:
         lib = _lib.load()
         _lib.check(lib.pk_pool_copy_blocks(self._h.ptr, arr.ctypes.data_as(C.POINTER(C.c_int64)),
                                            len(arr), _stream(self.device)))
+
+    def evict(self, block_tables, lengths, budget: int, *, sinks: int = 0, recent: int = 0, new_tables=None,
+              return_kept: bool = False):
+        """Shorten cached sequences to the ``budget`` tokens worth keeping, on every layer.
+
+        Per layer, sequence and KV head: the first ``sinks`` tokens, the last ``recent``, and of
+        the rest those with the largest accumulated ``weights`` (equal ones: the lowest position
+        first; NaN counts as the largest), moved in order with their K, V and weights to
+        positions ``0..min(length, budget) - 1`` of ``new_tables`` (default: the old tables,
+        in place; ``BlockManager.compact`` gives both). A sequence of at most ``budget`` tokens
+        keeps them all. Heads keep different tokens, so from then on a position is an index
+        into the cache: a model that rotates its keys goes on counting tokens itself.
+
+        Returns the new lengths (int64 array); with ``return_kept`` also an int32 CUDA tensor
+        ``(layers, sequences, kv_heads, budget)`` of the kept positions, -1 behind the last.
+        ``ValueError`` without ``track_weights``, if ``sinks + recent`` exceed ``budget``, or if
+        a new block is read by the call (other than the same block of the same sequence)."""
+        torch = _torch()
+        lens = np.ascontiguousarray(np.asarray(lengths, dtype=np.int64).reshape(-1))
+        indptr, ids = _csr(block_tables)
+        nindptr, nids = (indptr, ids) if new_tables is None else _csr(new_tables)
+        if len(indptr) - 1 != len(lens) or len(nindptr) - 1 != len(lens):
+            raise ValueError("block_tables, new_tables and lengths differ in length")
+        kept = None
+        if return_kept:
+            kept = torch.empty((self.n_layers, len(lens), self.n_kv_heads, max(0, int(budget))), dtype=torch.int32,
+                               device=self.device)
+        _lib.check(_lib.load().pk_pool_evict(
+            self._h.ptr, len(lens), _addr(indptr), _addr(ids), _addr(lens), _addr(nindptr), _addr(nids), int(budget),
+            int(sinks), int(recent), kept.data_ptr() if return_kept and kept.numel() else None, _stream(self.device)))
+        new_lens = np.minimum(lens, int(budget))
+        return (new_lens, kept) if return_kept else new_lens
 
     @property
     def nbytes(self) -> int:
@@ -285,12 +333,36 @@ class PagedBatch:
     ``block_tables`` may also be given as a CSR pair ``(indptr int64, ids int32)``.
     ``q, k, v`` may be numpy arrays (result returned as numpy, dtype of ``q``) or float32
     CUDA tensors on the pool's device (result returned as a CUDA tensor, no host copies).
+
+    Bounded steps (not in pagellm). ``window``: the row at position ``p`` sees only the keys
+    after ``p - window``, and the first ``sinks`` tokens; blocks that no row sees a key of are
+    not read, so their table entries may name any valid block. ``weights`` (on a pool with
+    ``track_weights``): every ``write_and_attend`` / ``attend`` also sums per cached token and
+    KV head the softmax weight it gets from the step's rows and the head's query heads, and
+    adds it to the pool's ``weights`` (``"add"``) or stores it there (``"replace"``). The
+    step's own tokens start anew; tokens that no row sees keep their weight. Such a step reads
+    every block through one table entry only (``ValueError`` otherwise). In bounded steps of a
+    bf16 pool, bf16 CUDA tensors are read and written as they are.
     """
 
+    _WEIGHT_MODES = {None: 0, "add": 1, "replace": 2}
+
     def __init__(self, pool: PagedKVPool, block_tables, starts, n_new, attn: str = "gather",
-                 batch_decode: bool = True):
+                 batch_decode: bool = True, *, window: int | None = None, sinks: int = 0,
+                 weights: str | None = None):
         if attn not in ("gather", "paged"):
             raise ValueError(attn)
+        if window is not None and int(window) < 1:
+            raise ValueError(f"window must be at least 1, not {window!r}")
+        if int(sinks) < 0 or (int(sinks) > 0 and window is None):
+            raise ValueError("sinks must not be negative and need a window")
+        if weights not in self._WEIGHT_MODES:
+            raise ValueError(f"weights must be None, 'add' or 'replace', not {weights!r}")
+        if weights is not None and pool.weights is None:
+            raise ValueError("weights need a pool made with track_weights=True")
+        self.window, self.sinks, self.weights = None if window is None else int(window), int(sinks), weights
+        bounds = (min(self.window or 0, 2 ** 31 - 1), min(self.sinks, 2 ** 31 - 1), self._WEIGHT_MODES[weights])
+        self._bounded = bounds != (0, 0, 0)
         self.pool, self.attn, self.batch_decode = pool, attn, batch_decode
         self.block_tables, self.starts, self.n_new = block_tables, starts, n_new
         starts_a = np.ascontiguousarray(np.asarray(starts, dtype=np.int64).reshape(-1))
@@ -310,6 +382,9 @@ class PagedBatch:
             _lib.check(lib.pk_batch_set_prefix_sharing(self._b, 1))
             pool._batch_prefix_mode[self._b] = 1
         self._prefix_sharing = "auto"
+        if pool._batch_bounds.get(self._b, (0, 0, 0)) != bounds:
+            _lib.check(lib.pk_batch_set_bounds(self._b, *bounds))
+            pool._batch_bounds[self._b] = bounds
         rows = C.c_int64()
         _lib.check(lib.pk_batch_plan(self._b, len(n_new_a), _addr(indptr), _addr(ids), _addr(starts_a),
                                      _addr(n_new_a), C.byref(rows), _stream(pool.device)))
@@ -416,6 +491,16 @@ class PagedBatch:
             if tuple(k.shape) != want or tuple(v.shape) != want:
                 raise ValueError(f"k, v must be {want}")
         st = _stream(P.device)
+        if self._bounded and hasattr(q, "is_cuda") and P.dtype_name == "bfloat16" and str(q.dtype) == "torch.bfloat16":
+            torch = _torch()
+            qd = _aligned(q.to(P.device).contiguous())
+            out = torch.empty_like(qd)
+            kd = _aligned(k.to(P.device, torch.bfloat16).contiguous()) if append else None
+            vd = _aligned(v.to(P.device, torch.bfloat16).contiguous()) if append else None
+            _lib.check(self._lib.pk_batch_write_and_attend_bf16(
+                self._b, layer, H, qd.data_ptr(), kd.data_ptr() if append else None,
+                vd.data_ptr() if append else None, out.data_ptr(), st))
+            return out
         if hasattr(q, "is_cuda"):
             torch = _torch()
             qd = _aligned(q.to(P.device, torch.float32).contiguous())
@@ -451,6 +536,52 @@ class PagedBatch:
 
 
 # ---------------------------------------------------------------------- free functions
+def evict_sequences(pool: PagedKVPool, manager: BlockManager, seq_ids, lengths, budget: int, *, sinks: int = 0,
+                    recent: int = 0) -> np.ndarray:
+    """``BlockManager.compact`` and ``PagedKVPool.evict`` for the sequences longer than
+    ``budget``; returns every sequence's new length. Shorter ones keep their blocks.
+
+    A block that one sequence gives up may become another's, and the last holder of a shared
+    block thins it out in place; sequences whose new blocks an earlier one still reads go into
+    a later launch."""
+    seq_ids = [int(s) for s in seq_ids]
+    lens = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    if len(seq_ids) != len(lens):
+        raise ValueError("seq_ids and lengths differ in length")
+    if len(set(seq_ids)) != len(seq_ids):
+        raise ValueError("a sequence appears twice")
+    budget, sinks, recent = int(budget), int(sinks), int(recent)
+    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+        raise ValueError("budget must be at least 1 and hold sinks + recent")
+    if pool.weights is None:
+        raise ValueError("eviction needs a pool made with track_weights=True")
+    for s, n in zip(seq_ids, lens):
+        if n < 0 or n > len(manager.block_table(s)) * manager.block_size:
+            raise ValueError(f"sequence {s} does not hold {n} tokens")
+    group: list = []
+    reads: set = set()
+
+    def flush():
+        if group:
+            pool.evict([g[0] for g in group], [g[2] for g in group], budget, sinks=sinks, recent=recent,
+                       new_tables=[g[1] for g in group])
+            group.clear()
+            reads.clear()
+
+    try:
+        for s, n in zip(seq_ids, lens.tolist()):
+            if n <= budget:
+                continue
+            old, new = manager.compact(s, budget)
+            if reads.intersection(new):
+                flush()
+            group.append((old, new, n))
+            reads.update(old)
+    finally:  # sequences compacted before one that found no block are evicted all the same
+        flush()
+    return np.minimum(lens, budget)
+
+
 def slot_mapping(block_table, positions, block_size: int) -> np.ndarray:
     """Physical slot for each logical position (paged.py:303-306), computed on the GPU.
 

@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <queue>
 #include <array>
@@ -222,11 +223,19 @@ struct pk_pool {
     CUtensorMap tmk1{};
     CUtensorMap tmv1{};
     Uploader pairs_up;
+    // accumulated attention weights, [layers][num_blocks][kvh][block_size]; NULL = not tracked
+    float* weights = nullptr;
+    // evict: its tables and items, the kept positions when the caller wants none, and the end
+    // of the last call (the next one may come on another stream)
+    Uploader evict_up;
+    DevBuf evict_kept;
+    cudaEvent_t evict_done = nullptr;
 
     size_t layer_bytes() const { return static_cast<size_t>(layer_elems) * esize; }
     size_t block_bytes() const { return static_cast<size_t>(block_size) * kvh * d * esize; }
     char* k_layer(int layer) const { return static_cast<char*>(k) + layer * layer_bytes(); }
     char* v_layer(int layer) const { return static_cast<char*>(v) + layer * layer_bytes(); }
+    int64_t layer_weights() const { return num_blocks * kvh * block_size; }
 };
 
 struct pk_batch {
@@ -296,6 +305,18 @@ struct pk_batch {
     // and the slice the exchange sends when the step cannot fuse it
     pk::PeerOut peer_out{};
     DevBuf peer_slice;
+    // Bounded steps: a sliding window with sinks and / or weights (0 off, 1 add, 2 replace).
+    // Their plan uses neither shared prefixes nor the fused append. bounds_stale: set after
+    // the last plan, which does not know them.
+    int64_t window = 0, sinks = 0;
+    int weights_mode = 0;
+    bool bounds_stale = false;
+    std::vector<int32_t> t_seq, t_blk;  // touched blocks (weights): sequence, table index
+    DevBuf ml;  // [rows][H] softmax statistics of a step with weights
+    cudaStream_t plan_stream = nullptr;  // stream of the last uploads
+    cudaEvent_t ev_bounded = nullptr;    // end of the last bounded call
+    bool used = false;
+    bool bounded() const { return window > 0 || weights_mode != 0; }
     int launches = 0;
     // bytes the last pk_batch_write_and_attend_host moved: host to device, device to host
     // by a copy after the kernels, stored by the kernels straight into the caller's
@@ -720,10 +741,29 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
     B->nwsplit = static_cast<int>(B->split.size() / 4);
 }
 
+// The blocks that the rows at positions q0 .. ctx-1 of a sequence read: table indices
+// [0, head) and [head + skip, head + skip + rest), where the first part holds the sinks in
+// front of row q0's window. Without a window: all of them, head = skip = 0.
+struct VisibleBlocks {
+    int head, skip;
+    int64_t count;
+};
+VisibleBlocks visible_blocks(int64_t q0, int64_t ctx, int64_t window, int64_t sinks, int bs) {
+    const int64_t end = (ctx + bs - 1) / bs;
+    if (window <= 0) return {0, 0, end};
+    const int64_t lo = std::max<int64_t>(0, q0 - window + 1);
+    const int64_t head = (std::min(sinks, lo) + bs - 1) / bs;
+    const int64_t first = std::max(lo / bs, head);
+    return {static_cast<int>(head), static_cast<int>(first - head), head + end - first};
+}
+
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
     B->plan_H = -1;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (B->bounded() && cudaStreamIsCapturing(st, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
+        return fail(PK_ERR_UNSUPPORTED, "plan the step before a stream capture (call once with the same n_heads)");
     B->u_seq.clear(); B->u_t0.clear(); B->u_n.clear(); B->u_blk.assign(1, 0);
     B->sp_u.clear(); B->sp_c0.clear(); B->sp_c1.clear(); B->gen_rows.clear();
     B->cta_blk.assign(1, 0);
@@ -740,7 +780,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nwide = B->nprefix = B->nprefix_groups = 0;
     B->prefix_keys = B->prefix_token_keys = 0;
     B->seq_kb0.assign(B->nseq, 0);
-    const bool wide_ok = P->wide_ok && g <= 128 && 128 % g == 0;
+    if (B->bounded()) qmax = 0;
+    const bool wide_ok = !B->bounded() && P->wide_ok && g <= 128 && 128 % g == 0;
     const int tpt = wide_ok ? 128 / g : 0;  // query tokens per wide item
     std::vector<int> tc_seqs;
     for (int i = 0; i < B->nseq; ++i) {
@@ -908,6 +949,10 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         B->w_slots[x] = static_cast<int64_t>(B->ids[B->indptr[i] + blk]) * P->block_size + (pos - blk * P->block_size);
     }
     B->plan.add(B->w_slots.data(), B->w_slots.size() * 8);  // 25
+    B->plan.add(B->t_seq.data(), B->t_seq.size() * 4);  // 26
+    B->plan.add(B->t_blk.data(), B->t_blk.size() * 4);  // 27
+    if (B->weights_mode != 0)
+        PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
         PK_CUDA(B->wpart.reserve(static_cast<size_t>(B->nslots) * 2 * 128 * (128 + 2) * sizeof(float)));
     if (!B->w_seq.empty())
@@ -915,8 +960,17 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (B->nprefix > 0) PK_CUDA(B->lse.reserve(static_cast<size_t>(B->nrows) * H * sizeof(float)));
     int rc = B->plan.commit(st);
     if (rc != PK_OK) return rc;
+    B->plan_stream = st;
     B->plan_H = H;
     return PK_OK;
+}
+
+// Before the uploads of a bounded step's plan: kernels of the last bounded call, perhaps on
+// another stream, still read what they replace.
+cudaError_t wait_used(pk_batch* B, cudaStream_t st) {
+    if (!B->used) return cudaSuccess;
+    B->used = false;
+    return cudaStreamWaitEvent(st, B->ev_bounded, 0);
 }
 
 // Kinds reported by pk_batch_profile_read.
@@ -1189,6 +1243,191 @@ int attend_impl(pk_batch* B, int layer, int H, const float* q, float* out, cudaS
     return PK_OK;
 }
 
+// A step with a window or weights: append, attention, weights. io16: q, k_new, v_new and out
+// hold bf16 (bf16 pools), else float. k_new NULL: no append.
+int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_new, const void* v_new, void* out,
+                   bool io16, cudaStream_t st) {
+    pk_pool* P = B->pool;
+    if (g_inject_launch_failure.exchange(0) != 0)
+        return fail(PK_ERR_CUDA, "injected launch failure (pk_test_inject_launch_failure)");
+    if (P->d > 512) return fail(PK_ERR_UNSUPPORTED, "head_dim %d > 512", P->d);
+    if (B->plan_H != H) {
+        int rc = build_attention_plan(B, H, st);
+        if (rc != PK_OK) return rc;
+    }
+    if (B->nrows == 0) return PK_OK;
+    if (st != B->plan_stream) {
+        // the plan came over on another stream; a capture cannot wait for it, and follows a
+        // call that did (build_attention_plan)
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+        if (capturing == cudaStreamCaptureStatusNone) {
+            PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
+            PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
+        }
+    }
+    if (k_new != nullptr) {
+        const bool listed = !B->app_rows.empty();
+        const int32_t* rows = listed ? B->meta.at<int32_t>(5) : nullptr;
+        const int64_t n = listed ? static_cast<int64_t>(B->app_rows.size()) : B->nrows;
+        PK_CUDA(prof_begin(B, st));
+        if (io16)
+            PK_CUDA(pk::launch_append_rows16(P->k_layer(layer), P->v_layer(layer), k_new, v_new, B->meta.at<int32_t>(4),
+                                             B->meta.at<int32_t>(3), B->meta.at<int32_t>(2), B->meta.at<int32_t>(0),
+                                             B->meta.at<int32_t>(1), P->block_size, rows, n, P->kvh * P->d, st));
+        else
+            PK_CUDA(pk::launch_append_table(P->dtype, P->k_layer(layer), P->v_layer(layer),
+                                            static_cast<const float*>(k_new), static_cast<const float*>(v_new),
+                                            B->meta.at<int32_t>(4), B->meta.at<int32_t>(3), B->meta.at<int32_t>(2),
+                                            B->meta.at<int32_t>(0), B->meta.at<int32_t>(1), P->block_size, rows, n,
+                                            P->kvh * P->d, st));
+        PK_CUDA(prof_end(B, kProfAppend, st));
+        B->launches++;
+    }
+    pk::BoundedParams p{};
+    p.q = q;
+    p.out = out;
+    p.pool_k = P->k_layer(layer);
+    p.pool_v = P->v_layer(layer);
+    p.row_seq = B->meta.at<int32_t>(4);
+    p.indptr = B->meta.at<int32_t>(0);
+    p.ids = B->meta.at<int32_t>(1);
+    p.starts = B->meta.at<int32_t>(2);
+    p.offsets = B->meta.at<int32_t>(3);
+    p.rows = B->plan.at<int32_t>(7);
+    p.ml = B->weights_mode != 0 ? static_cast<float2*>(B->ml.ptr) : nullptr;
+    p.nrows = B->ngeneric;
+    p.H = H;
+    p.kvh = P->kvh;
+    p.D = P->d;
+    p.bs = P->block_size;
+    p.window = B->window > 0 ? static_cast<int>(B->window) : INT32_MAX;
+    p.sinks = static_cast<int>(B->sinks);
+    p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
+    if (B->ngeneric > 0) {
+        PK_CUDA(prof_begin(B, st));
+        PK_CUDA(pk::launch_bounded_rows(P->dtype, io16, p, st));
+        PK_CUDA(prof_end(B, kProfGeneric, st));
+        B->launches++;
+    }
+    if (B->weights_mode != 0) {
+        pk::WeightParams w{};
+        w.weights = P->weights + static_cast<int64_t>(layer) * P->layer_weights();
+        w.t_seq = B->plan.at<int32_t>(26);
+        w.t_blk = B->plan.at<int32_t>(27);
+        w.ntouched = static_cast<int>(B->t_seq.size());
+        w.add = B->weights_mode == 1;
+        PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
+        B->launches++;
+    }
+    if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+    if (capturing == cudaStreamCaptureStatusNone) {
+        PK_CUDA(cudaEventRecord(B->ev_bounded, st));
+        B->used = true;
+    }
+    return PK_OK;
+}
+
+// What a call of pk_pool_evict uploads, after its checks.
+struct EvictPlan {
+    std::vector<int32_t> indptr{0}, ids, new_indptr{0}, new_ids, lengths, items;
+    int max_len = 0;
+};
+
+// Checks and lays out an eviction (host only). A destination must not be a block that the call
+// reads, except the same block of the same sequence at the same table index when nothing else
+// reads it: then new positions never pass old ones, and moving in order is safe.
+int plan_evict(int64_t num_blocks, int bs, int nseq, const int64_t* table_indptr, const int32_t* table_ids,
+               const int64_t* lengths, const int64_t* new_indptr, const int32_t* new_ids, int64_t budget, int64_t sinks,
+               int64_t recent, EvictPlan* out) {
+    if (nseq < 0) return fail(PK_ERR_INVALID_ARG, "nseq < 0");
+    if (budget < 1 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
+        return fail(PK_ERR_INVALID_ARG, "budget %lld must be at least 1 and hold sinks %lld + recent %lld",
+                    (long long)budget, (long long)sinks, (long long)recent);
+    if (budget >= (int64_t(1) << 31)) return fail(PK_ERR_UNSUPPORTED, "budget %lld too large", (long long)budget);
+    if (nseq == 0) return PK_OK;
+    if (!table_indptr || !lengths || !new_indptr) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    if (table_indptr[0] != 0 || new_indptr[0] != 0) return fail(PK_ERR_INVALID_ARG, "a table's indptr[0] != 0");
+    // every block the call reads or writes: (block, kind, sequence, index), kind 0 read, 1 written
+    struct Use {
+        int32_t block, kind, seq, idx;
+    };
+    std::vector<Use> uses;
+    auto ids_ok = [&](const int32_t* t, int64_t n, int i, const char* what) {
+        for (int64_t j = 0; j < n; ++j)
+            if (t[j] < 0 || t[j] >= num_blocks)
+                return fail(PK_ERR_OUT_OF_RANGE, "seq %d: %s block id %d outside [0, %lld)", i, what, t[j],
+                            (long long)num_blocks);
+        return static_cast<int>(PK_OK);
+    };
+    for (int i = 0; i < nseq; ++i) {
+        const int64_t n = lengths[i], have = table_indptr[i + 1] - table_indptr[i], nhave = new_indptr[i + 1] - new_indptr[i];
+        if (n < 0) return fail(PK_ERR_INVALID_ARG, "seq %d: length %lld negative", i, (long long)n);
+        if (n >= (int64_t(1) << 31) - bs) return fail(PK_ERR_UNSUPPORTED, "seq %d: length %lld too long", i, (long long)n);
+        if (have < 0 || nhave < 0) return fail(PK_ERR_INVALID_ARG, "a table's indptr decreases at seq %d", i);
+        const int64_t need = (n + bs - 1) / bs, nneed = (std::min(n, budget) + bs - 1) / bs;
+        if (need > have || nneed > nhave)
+            return fail(PK_ERR_OUT_OF_RANGE, "seq %d: %lld tokens need %lld blocks and %lld new ones, the tables have %lld and %lld",
+                        i, (long long)n, (long long)need, (long long)nneed, (long long)have, (long long)nhave);
+        if ((need > 0 && !table_ids) || (nneed > 0 && !new_ids)) return fail(PK_ERR_INVALID_ARG, "NULL table ids");
+        const int32_t* t = need > 0 ? table_ids + table_indptr[i] : nullptr;
+        const int32_t* nt = nneed > 0 ? new_ids + new_indptr[i] : nullptr;
+        int rc;
+        if ((rc = ids_ok(t, need, i, "table")) != PK_OK) return rc;
+        if ((rc = ids_ok(nt, nneed, i, "new table")) != PK_OK) return rc;
+        if (out->ids.size() + need >= (size_t(1) << 31) || out->new_ids.size() + nneed >= (size_t(1) << 31))
+            return fail(PK_ERR_UNSUPPORTED, "too many table entries");
+        if (need > 0) out->ids.insert(out->ids.end(), t, t + need);
+        if (nneed > 0) out->new_ids.insert(out->new_ids.end(), nt, nt + nneed);
+        out->indptr.push_back(static_cast<int32_t>(out->ids.size()));
+        out->new_indptr.push_back(static_cast<int32_t>(out->new_ids.size()));
+        out->lengths.push_back(static_cast<int32_t>(n));
+        out->max_len = std::max(out->max_len, static_cast<int>(n));
+        for (int64_t j = 0; j < need; ++j) uses.push_back({t[j], 0, i, static_cast<int32_t>(j)});
+        for (int64_t j = 0; j < nneed; ++j) uses.push_back({nt[j], 1, i, static_cast<int32_t>(j)});
+    }
+    std::sort(uses.begin(), uses.end(), [](const Use& a, const Use& b) {
+        return a.block != b.block ? a.block < b.block : a.kind > b.kind;
+    });
+    std::vector<uint8_t> in_place(nseq, 0);
+    for (size_t x = 0; x < uses.size();) {
+        const Use& w = uses[x++];
+        if (w.kind == 1) {  // a written block comes before its reads
+            for (; x < uses.size() && uses[x].block == w.block; ++x) {
+                if (uses[x].kind == 1)
+                    return fail(PK_ERR_INVALID_ARG, "block %d appears twice in the new tables", w.block);
+                if (uses[x].seq != w.seq || uses[x].idx != w.idx)
+                    return fail(PK_ERR_INVALID_ARG,
+                                "seq %d: new block %d is read by this call; a new table may name an old block only at its "
+                                "own index and when no other sequence reads it", w.seq, w.block);
+                in_place[w.seq] = 1;
+            }
+        } else {
+            while (x < uses.size() && uses[x].block == w.block) ++x;
+        }
+    }
+    // New positions move in pieces of kRows by different blocks of the grid; in place they have
+    // to move in order, as one piece.
+    constexpr int kRows = 256;
+    for (int i = 0; i < nseq; ++i) {
+        const int m = static_cast<int>(std::min<int64_t>(out->lengths[i], budget));
+        const int step = in_place[i] ? std::max(m, 1) : kRows;
+        for (int y = 0; y < m; y += step) out->items.insert(out->items.end(), {i, y, y + std::min(m - y, step)});
+    }
+    return PK_OK;
+}
+
+// The checks that every per-layer entry point makes of a bounded batch.
+int check_bounds(const pk_batch* B) {
+    if (B->bounds_stale)
+        return fail(PK_ERR_INVALID_ARG, "pk_batch_set_bounds was called after the last pk_batch_plan: plan again");
+    if (B->weights_mode != 0 && B->pool->weights == nullptr)
+        return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
+    return PK_OK;
+}
+
 }  // namespace
 
 void pk_set_last_error(const char* msg) { g_err = msg ? msg : ""; }
@@ -1260,6 +1499,10 @@ int pk_pool_destroy(pk_pool* pool) {
     if (!pool) return PK_OK;
     DeviceScope ds(pool->device);
     pool->pairs_up.release();
+    pool->evict_up.release();
+    pool->evict_kept.release();
+    if (pool->evict_done) cudaEventDestroy(pool->evict_done);
+    if (pool->weights) cudaFree(pool->weights);
     if (pool->k) cudaFree(pool->k);
     if (pool->v) cudaFree(pool->v);
     delete pool;
@@ -1294,6 +1537,9 @@ int pk_pool_copy_blocks_dev(pk_pool* pool, const int64_t* pairs_dev, int64_t npa
                                    static_cast<int64_t>(pool->layer_bytes()),
                                    static_cast<int64_t>(pool->block_bytes()),
                                    static_cast<cudaStream_t>(stream)));
+    if (pool->weights)  // a copied block keeps its tokens' weights
+        PK_CUDA(pk::launch_copy_weights(pool->weights, pairs_dev, npairs, pool->n_layers, pool->layer_weights(),
+                                        pool->kvh * pool->block_size, static_cast<cudaStream_t>(stream)));
     return PK_OK;
 }
 
@@ -1340,8 +1586,91 @@ int pk_pool_copy_blocks(pk_pool* pool, const int64_t* pairs_host, int64_t npairs
         PK_CUDA(pk::launch_copy_blocks(pool->k, pool->v, dev + 2 * a, b - a, pool->n_layers,
                                        static_cast<int64_t>(pool->layer_bytes()),
                                        static_cast<int64_t>(pool->block_bytes()), st));
+        if (pool->weights)  // a copied block keeps its tokens' weights
+            PK_CUDA(pk::launch_copy_weights(pool->weights, dev + 2 * a, b - a, pool->n_layers, pool->layer_weights(),
+                                            pool->kvh * pool->block_size, st));
     }
     return PK_OK;
+}
+
+int pk_pool_track_weights(pk_pool* pool, float** weights_dev) {
+    if (!pool) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
+    if (!pool->weights) {
+        DeviceScope ds(pool->device);
+        const size_t bytes = static_cast<size_t>(pool->n_layers) * pool->layer_weights() * sizeof(float);
+        float* w = nullptr;
+        cudaError_t e = cudaMalloc(&w, bytes);
+        if (e == cudaSuccess) e = cudaMemset(w, 0, bytes);
+        if (e != cudaSuccess) {
+            if (w) cudaFree(w);
+            return fail(PK_ERR_CUDA, "attention weights of %zu bytes: %s", bytes, cudaGetErrorString(e));
+        }
+        pool->weights = w;
+    }
+    if (weights_dev) *weights_dev = pool->weights;
+    return PK_OK;
+}
+
+int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32_t* table_ids, const int64_t* lengths,
+                  const int64_t* new_indptr, const int32_t* new_ids, int64_t budget, int64_t sinks, int64_t recent,
+                  int32_t* kept_dev, void* stream) try {
+    if (!P) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
+    if (!P->weights) return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
+    const int bs = P->block_size;
+    EvictPlan plan;
+    int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
+                        &plan);
+    if (rc != PK_OK || nseq == 0) return rc;
+    if (static_cast<int64_t>(P->kvh) * P->n_layers > 65535)
+        return fail(PK_ERR_UNSUPPORTED, "n_layers * n_kv_heads above 65535");
+    DeviceScope ds(P->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone)
+        return fail(PK_ERR_UNSUPPORTED, "pk_pool_evict uploads from host memory and cannot be captured");
+    if (P->evict_done) PK_CUDA(cudaStreamWaitEvent(st, P->evict_done, 0));
+    else PK_CUDA(cudaEventCreateWithFlags(&P->evict_done, cudaEventDisableTiming));
+    pk::EvictParams p{};
+    if (kept_dev == nullptr) {
+        PK_CUDA(P->evict_kept.reserve(static_cast<size_t>(P->n_layers) * nseq * P->kvh * budget * sizeof(int32_t)));
+        kept_dev = static_cast<int32_t*>(P->evict_kept.ptr);
+    }
+    Uploader& up = P->evict_up;
+    up.begin();
+    up.add(plan.indptr.data(), plan.indptr.size() * 4);
+    up.add(plan.ids.data(), plan.ids.size() * 4);
+    up.add(plan.new_indptr.data(), plan.new_indptr.size() * 4);
+    up.add(plan.new_ids.data(), plan.new_ids.size() * 4);
+    up.add(plan.lengths.data(), plan.lengths.size() * 4);
+    up.add(plan.items.data(), plan.items.size() * 4);
+    rc = up.commit(st);
+    if (rc != PK_OK) return rc;
+    p.pool_k = P->k;
+    p.pool_v = P->v;
+    p.weights = P->weights;
+    p.indptr = up.at<int32_t>(0);
+    p.ids = up.at<int32_t>(1);
+    p.new_indptr = up.at<int32_t>(2);
+    p.new_ids = up.at<int32_t>(3);
+    p.lengths = up.at<int32_t>(4);
+    p.items = up.at<int32_t>(5);
+    p.kept = kept_dev;
+    p.num_blocks = P->num_blocks;
+    p.nitems = static_cast<int>(plan.items.size() / 3);
+    p.nseq = nseq;
+    p.layers = P->n_layers;
+    p.kvh = P->kvh;
+    p.bs = bs;
+    p.row_bytes = P->d * P->esize;
+    p.budget = static_cast<int>(budget);
+    p.sinks = static_cast<int>(sinks);
+    p.recent = static_cast<int>(recent);
+    PK_CUDA(pk::launch_evict(p, plan.max_len, st));
+    PK_CUDA(cudaEventRecord(P->evict_done, st));
+    return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const float* v_dev,
@@ -1395,6 +1724,8 @@ int pk_batch_destroy(pk_batch* B) {
     B->lse.release();
     B->wpart.release();
     B->qpk.release();
+    B->ml.release();
+    if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);
     if (B->ev_join) cudaEventDestroy(B->ev_join);
@@ -1405,7 +1736,7 @@ int pk_batch_destroy(pk_batch* B) {
 }
 
 int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int32_t* table_ids,
-                  const int64_t* starts, const int64_t* n_new, int64_t* n_rows, void* stream) {
+                  const int64_t* starts, const int64_t* n_new, int64_t* n_rows, void* stream) try {
     if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
     if (nseq < 0) return fail(PK_ERR_INVALID_ARG, "nseq < 0");
     if (nseq > 0 && (!table_indptr || !starts || !n_new))
@@ -1462,6 +1793,30 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
         if (rows >= (int64_t(1) << 31)) return fail(PK_ERR_UNSUPPORTED, "too many rows");
         B->offsets.push_back(static_cast<int32_t>(rows));
         for (int64_t r = 0; r < n; ++r) B->row_seq.push_back(i);
+    }
+    B->bounds_stale = false;
+    B->t_seq.clear();
+    B->t_blk.clear();
+    if (B->weights_mode != 0) {
+        if (!P->weights) return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
+        // a token's weight lives in its slot: a block that two table entries of the step read
+        // would need its sums joined across them
+        std::vector<uint8_t> seen(P->num_blocks, 0);
+        for (int i = 0; i < nseq; ++i) {
+            if (B->nnew[i] == 0) continue;
+            const VisibleBlocks vb = visible_blocks(B->starts[i], static_cast<int64_t>(B->starts[i]) + B->nnew[i],
+                                                    B->window, B->sinks, bs);
+            for (int64_t x = 0; x < vb.count; ++x) {
+                const int32_t j = static_cast<int32_t>(x < vb.head ? x : x + vb.skip);
+                const int32_t b = B->ids[B->indptr[i] + j];
+                if (seen[b])
+                    return fail(PK_ERR_INVALID_ARG, "seq %d: block %d is read twice in this step; weights need every "
+                                "block to belong to one sequence (copy shared blocks first)", i, b);
+                seen[b] = 1;
+                B->t_seq.push_back(i);
+                B->t_blk.push_back(j);
+            }
+        }
     }
     // Written blocks: which (sequence, table index) writes each; any other reference to
     // such a block, or two writers, rules the fused append out for this step.
@@ -1530,6 +1885,8 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     if (n_rows) *n_rows = rows;
     DeviceScope ds(P->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    PK_CUDA(wait_used(B, st));
+    B->plan_stream = st;
     B->meta.begin();
     B->meta.add(B->indptr.data(), B->indptr.size() * 4);
     B->meta.add(B->ids.data(), B->ids.size() * 4);
@@ -1543,6 +1900,8 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     B->rows_pending = rows > 0;  // built by the first reader (ensure_rows)
     B->rows_stream = st;
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_batch_rows(const pk_batch* B, const int64_t** positions_dev, const int64_t** slots_dev) {
@@ -1555,20 +1914,65 @@ int pk_batch_rows(const pk_batch* B, const int64_t** positions_dev, const int64_
 }
 
 int pk_batch_attend(pk_batch* B, int layer, int n_heads, const float* q_dev, float* out_dev,
-                    void* stream) {
+                    void* stream) try {
     if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
     int rc = check_heads(B, n_heads);
     if (rc != PK_OK) return rc;
     if (layer < 0 || layer >= B->pool->n_layers) return fail(PK_ERR_OUT_OF_RANGE, "layer %d", layer);
     if (B->nrows > 0 && (!q_dev || !out_dev)) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
     if ((rc = check_aligned(q_dev, "q")) || (rc = check_aligned(out_dev, "out"))) return rc;
+    if ((rc = check_bounds(B)) != PK_OK) return rc;
     DeviceScope ds(B->pool->device);
     B->launches = 0;
+    if (B->bounded())
+        return attend_bounded(B, layer, n_heads, q_dev, nullptr, nullptr, out_dev, false, static_cast<cudaStream_t>(stream));
     return attend_impl(B, layer, n_heads, q_dev, out_dev, static_cast<cudaStream_t>(stream));
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
+}
+
+int pk_batch_write_and_attend_bf16(pk_batch* B, int layer, int n_heads, const void* q_dev, const void* k_dev,
+                                   const void* v_dev, void* out_dev, void* stream) try {
+    if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
+    int rc = check_heads(B, n_heads);
+    if (rc != PK_OK) return rc;
+    if (layer < 0 || layer >= B->pool->n_layers) return fail(PK_ERR_OUT_OF_RANGE, "layer %d", layer);
+    if (B->pool->dtype != PK_BF16) return fail(PK_ERR_UNSUPPORTED, "bf16 rows need a bf16 pool");
+    if ((rc = check_bounds(B)) != PK_OK) return rc;
+    if (!B->bounded()) return fail(PK_ERR_UNSUPPORTED, "bf16 rows need a step with a window or weights (pk_batch_set_bounds)");
+    if (B->nrows > 0 && (!q_dev || !out_dev || (k_dev == nullptr) != (v_dev == nullptr)))
+        return fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    if ((rc = check_aligned(q_dev, "q")) || (rc = check_aligned(k_dev, "k")) || (rc = check_aligned(v_dev, "v")) ||
+        (rc = check_aligned(out_dev, "out")))
+        return rc;
+    DeviceScope ds(B->pool->device);
+    B->launches = 0;
+    return attend_bounded(B, layer, n_heads, q_dev, k_dev, v_dev, out_dev, true, static_cast<cudaStream_t>(stream));
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
+}
+
+int pk_batch_set_bounds(pk_batch* B, int64_t window, int64_t sinks, int weights_mode) {
+    if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
+    if (window < 0 || sinks < 0) return fail(PK_ERR_INVALID_ARG, "window %lld / sinks %lld negative", (long long)window, (long long)sinks);
+    if (sinks > 0 && window == 0) return fail(PK_ERR_INVALID_ARG, "sinks need a window");
+    if (weights_mode < 0 || weights_mode > 2) return fail(PK_ERR_INVALID_ARG, "weights mode %d not in 0..2", weights_mode);
+    if (weights_mode != 0 && B->pool->weights == nullptr)
+        return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
+    window = std::min<int64_t>(window, INT32_MAX);  // contexts are shorter
+    sinks = std::min<int64_t>(sinks, INT32_MAX);
+    if (window != B->window || sinks != B->sinks || weights_mode != B->weights_mode) {
+        B->window = window;
+        B->sinks = sinks;
+        B->weights_mode = weights_mode;
+        B->plan_H = -1;
+        B->bounds_stale = true;
+    }
+    return PK_OK;
 }
 
 int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* q_dev,
-                              const float* k_dev, const float* v_dev, float* out_dev, void* stream) {
+                              const float* k_dev, const float* v_dev, float* out_dev, void* stream) try {
     if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
     int rc = check_heads(B, n_heads);
     if (rc != PK_OK) return rc;
@@ -1579,9 +1983,11 @@ int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* 
     if ((rc = check_aligned(q_dev, "q")) || (rc = check_aligned(k_dev, "k")) ||
         (rc = check_aligned(v_dev, "v")) || (rc = check_aligned(out_dev, "out")))
         return rc;
+    if ((rc = check_bounds(B)) != PK_OK) return rc;
     DeviceScope ds(P->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     B->launches = 0;
+    if (B->bounded()) return attend_bounded(B, layer, n_heads, q_dev, k_dev, v_dev, out_dev, false, st);
     if (B->plan_H != n_heads) {
         rc = build_attention_plan(B, n_heads, st);
         if (rc != PK_OK) return rc;
@@ -1608,6 +2014,8 @@ int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* 
         B->launches++;
     }
     return attend_impl(B, layer, n_heads, q_dev, out_dev, st);
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_peer_gather_write_and_attend(pk_peer_gather* g, pk_batch* B, int layer, int n_heads,
@@ -1630,7 +2038,7 @@ int pk_peer_gather_write_and_attend(pk_peer_gather* g, pk_batch* B, int layer, i
     const int64_t row_floats = static_cast<int64_t>(n_heads) * P->d;
     // One split-KV launch writes every output row of such a step: the exchange rides on it
     // (if the launch's shared memory has room for the rows' staging).
-    if (B->nrows > 0 && B->use_tc && B->nwide == 0 && B->nprefix == 0 && B->ngeneric == 0 &&
+    if (B->nrows > 0 && !B->bounded() && B->use_tc && B->nwide == 0 && B->nprefix == 0 && B->ngeneric == 0 &&
         P->tc_smem + pk::tc_peer_stage_bytes(P->d) <= static_cast<size_t>(P->smem_optin)) {
         float* res = nullptr;
         rc = pk_peer_gather_step(g, B->nrows, row_floats, P->d, &B->peer_out, &res);
@@ -1690,7 +2098,7 @@ int pk_batch_write_and_attend_host(pk_batch* B, int layer, int n_heads, const fl
         }
         B->io_h2d = static_cast<int64_t>(qn + 2 * kn) * sizeof(float);
         // the attention plan now, while the copies run (pk_batch_write_and_attend reuses it)
-        if (layer >= 0 && layer < P->n_layers && B->plan_H != n_heads) {
+        if (layer >= 0 && layer < P->n_layers && B->plan_H != n_heads && check_bounds(B) == PK_OK) {
             rc = build_attention_plan(B, n_heads, st);
             if (rc != PK_OK) return rc;
         }
@@ -1831,6 +2239,31 @@ int pk_gather_interleave(const float* src_dev, float* dst_dev, int world, int64_
     int rc;
     if ((rc = check_aligned(src_dev, "src")) || (rc = check_aligned(dst_dev, "dst"))) return rc;
     PK_CUDA(pk::launch_interleave_heads(src_dev, dst_dev, world, rows, row_floats, static_cast<cudaStream_t>(stream)));
+    return PK_OK;
+}
+
+int pk_plan_evict(int64_t num_blocks, int block_size, int nseq, const int64_t* table_indptr, const int32_t* table_ids,
+                  const int64_t* lengths, const int64_t* new_indptr, const int32_t* new_ids, int64_t budget, int64_t sinks,
+                  int64_t recent, int64_t* n_items) try {
+    if (num_blocks <= 0 || block_size <= 0) return fail(PK_ERR_INVALID_ARG, "bad sizes");
+    EvictPlan plan;
+    int rc = plan_evict(num_blocks, block_size, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks,
+                        recent, &plan);
+    if (rc == PK_OK && n_items) *n_items = static_cast<int64_t>(plan.items.size() / 3);
+    return rc;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
+}
+
+int pk_plan_visible_blocks(int64_t first_position, int64_t context, int64_t window, int64_t sinks, int block_size,
+                           int64_t* blocks3) {
+    if (first_position < 0 || context <= first_position || context >= (int64_t(1) << 31) || window < 0 || sinks < 0 ||
+        (sinks > 0 && window == 0) || block_size <= 0 || !blocks3)
+        return fail(PK_ERR_INVALID_ARG, "bad arguments");
+    const VisibleBlocks v = visible_blocks(first_position, context, window, sinks, block_size);
+    blocks3[0] = v.head;
+    blocks3[1] = v.skip;
+    blocks3[2] = v.count;
     return PK_OK;
 }
 

@@ -9,9 +9,11 @@
 // doubly-linked list over block ids in release order, so allocate evicts the
 // least-recently released cached block in O(1) and incref revives any block in O(1).
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -35,6 +37,7 @@ int bm_fail(int code, const char* fmt, ...) {
 struct SeqTable {
     std::vector<int32_t> blocks;
     std::vector<std::string> hashes;  // digests of the leading full blocks (prefix chain)
+    bool compacted = false;           // no longer holds a prefix of its tokens: publishes nothing
 };
 
 }  // namespace
@@ -411,6 +414,7 @@ PK_API int pk_bm_seq_push_hashes(pk_block_manager* m, int64_t seq, const uint8_t
     SeqTable* t;
     int rc = get_table(m, seq, &t);
     if (rc) return rc;
+    if (t->compacted) return PK_OK;
     for (int64_t k = 0; k < count; ++k) {
         const size_t i = t->hashes.size();
         if (i >= t->blocks.size()) return bm_fail(PK_ERR_OUT_OF_RANGE, "hash chain longer than the table");
@@ -483,6 +487,50 @@ PK_API int pk_bm_truncate(pk_block_manager* m, int64_t seq, int64_t n_tokens) {
         }
     }
     return PK_OK;
+}
+
+// The table of a sequence whose tokens pk_pool_evict thins out to n_tokens: in place where the
+// block is this sequence's alone and unpublished, else a fresh block (the shared or cached
+// content stays for its other readers). pagellm has no eviction within a sequence.
+PK_API int pk_bm_compact(pk_block_manager* m, int64_t seq, int64_t n_tokens, int32_t* old_out, int64_t cap,
+                         int64_t* n_old) try {
+    if (!m || !n_old) return bm_fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    SeqTable* t;
+    int rc = get_table(m, seq, &t);
+    if (rc) return rc;
+    const int64_t have = static_cast<int64_t>(t->blocks.size());
+    if (n_tokens < 0 || n_tokens > have * m->block_size)
+        return bm_fail(PK_ERR_INVALID_ARG, "cannot compact a %lld-token table to %lld tokens",
+                       (long long)(have * m->block_size), (long long)n_tokens);
+    if (old_out && cap < have) return bm_fail(PK_ERR_INVALID_ARG, "old table buffer too small");
+    const int64_t keep = m->blocks_needed(n_tokens);
+    auto own = [&](int32_t b) { return m->ref[b] == 1 && !m->has_hash[b]; };
+    int64_t need = 0;
+    for (int64_t i = 0; i < keep; ++i) need += !own(t->blocks[i]);
+    if (need > m->num_free())
+        return bm_fail(PK_ERR_OUT_OF_BLOCKS, "compaction needs %lld free blocks", (long long)need);
+    std::vector<int32_t> fresh(static_cast<size_t>(keep)), drop;
+    drop.reserve(static_cast<size_t>(have));
+    for (int64_t i = 0; i < keep; ++i) {
+        fresh[i] = t->blocks[i];
+        if (own(fresh[i])) continue;
+        drop.push_back(t->blocks[i]);
+        rc = m->allocate(&fresh[i]);  // cannot run out: counted above
+        if (rc) return rc;
+    }
+    drop.insert(drop.end(), t->blocks.begin() + keep, t->blocks.end());
+    *n_old = have;
+    if (old_out) std::copy(t->blocks.begin(), t->blocks.end(), old_out);
+    t->blocks.swap(fresh);
+    t->hashes.clear();
+    t->compacted = true;
+    for (auto b = drop.rbegin(); b != drop.rend(); ++b) {
+        rc = m->decref(*b);
+        if (rc) return rc;
+    }
+    return PK_OK;
+} catch (const std::exception& e) {
+    return bm_fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 PK_API int pk_bm_table(const pk_block_manager* m, int64_t seq, int32_t* out, int64_t cap, int64_t* n) {

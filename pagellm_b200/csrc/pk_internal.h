@@ -175,6 +175,64 @@ struct WideParams {
     float qscale;
 };
 
+// Windowed attention on the CUDA cores: any pool, rows of `q` / `out` in the pool's input type.
+// A row at position p sees the keys j <= p with j < sinks or j > p - window.
+struct BoundedParams {
+    const void* q;   // [rows][H][D], float or bf16
+    void* out;
+    const void* pool_k;  // layer base
+    const void* pool_v;
+    const int32_t* row_seq;
+    const int32_t* indptr;
+    const int32_t* ids;
+    const int32_t* starts;
+    const int32_t* offsets;
+    const int32_t* rows;  // rows to process (indices into q / out)
+    float2* ml;  // [rows][H] softmax statistics of each row: (max, 1 / sum), log2 domain; NULL = not kept
+    int nrows;
+    int H;
+    int kvh;
+    int D;
+    int bs;
+    int window;  // >= 1; INT32_MAX without a window
+    int sinks;
+    float qscale;  // log2(e) / sqrt(D)
+};
+
+// The touched blocks of a step - those with a key that some row sees - and the layer's
+// accumulated weights [num_blocks][kvh][bs].
+struct WeightParams {
+    float* weights;
+    const int32_t* t_seq;  // [ntouched] sequence
+    const int32_t* t_blk;  // [ntouched] block of its table
+    int ntouched;
+    int add;  // add to the weights of tokens cached before the step (else store)
+};
+
+struct EvictParams {
+    void* pool_k;
+    void* pool_v;
+    float* weights;        // [layers][num_blocks][kvh][bs]
+    const int32_t* lengths;  // [nseq]
+    const int32_t* indptr;   // block tables before and after
+    const int32_t* ids;
+    const int32_t* new_indptr;
+    const int32_t* new_ids;
+    int32_t* kept;         // [layers][nseq][kvh][budget] kept positions, ascending, -1 behind the last
+    const int32_t* items;  // [nitems][3] sequence, first and end new position
+    int64_t num_blocks;
+    int nitems;
+    int nseq;
+    int layers;
+    int kvh;
+    int bs;
+    int row_bytes;  // bytes of one (slot, KV head) row of K or V
+    int budget;
+    int sinks;
+    int recent;
+    int cache_cap;  // sequences up to this length keep their weights in shared memory
+};
+
 // Read-only view of a pool's fields for entry points outside pk_api.cu.
 struct PoolView {
     int device;
@@ -242,6 +300,9 @@ cudaError_t launch_append_table(int dtype, void* pool_k_layer, void* pool_v_laye
                                 const int32_t* rows, int64_t n, int rowlen, cudaStream_t st);
 cudaError_t launch_copy_blocks(void* k, void* v, const int64_t* pairs, int64_t npairs, int layers,
                                int64_t layer_bytes, int64_t block_bytes, cudaStream_t st);
+// The accumulated weights of copied blocks: pairs as in launch_copy_blocks, `block` floats each.
+cudaError_t launch_copy_weights(float* weights, const int64_t* pairs, int64_t npairs, int layers, int64_t layer_floats,
+                                int block, cudaStream_t st);
 cudaError_t launch_bounded_wait_selftest(int* err, unsigned long long limit_ns, cudaStream_t st);
 // Three device-addressable host arrays (float counts multiples of 4, 16-byte aligned) into
 // device buffers, one launch.
@@ -253,6 +314,16 @@ cudaError_t launch_interleave_heads(const float* src, float* dst, int world, int
                                     cudaStream_t st);
 cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const int64_t* positions,
                                 int64_t n, int bs, int64_t* slots, int32_t* err, cudaStream_t st);
+
+cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
+cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
+// launch_append_table for rows given as bf16 (bf16 pools).
+cudaError_t launch_append_rows16(void* pool_k_layer, void* pool_v_layer, const void* k, const void* v,
+                                 const int32_t* row_seq, const int32_t* offsets, const int32_t* starts,
+                                 const int32_t* indptr, const int32_t* ids, int bs, const int32_t* rows, int64_t n,
+                                 int rowlen, cudaStream_t st);
+// Chooses the tokens that stay and moves them (two launches); max_len: the longest sequence.
+cudaError_t launch_evict(const EvictParams& p, int max_len, cudaStream_t st);
 
 }  // namespace pk
 
