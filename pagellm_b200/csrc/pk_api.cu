@@ -312,6 +312,12 @@ struct pk_batch {
     int weights_mode = 0;
     bool bounds_stale = false;
     std::vector<int32_t> t_seq, t_blk;  // touched blocks (weights): sequence, table index
+    int ntouch_tc = 0;                  // the first ones belong to sequences on the split-KV kernel
+    std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
+    std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
+    std::vector<uint8_t> seq_tc;        // scratch: sequence is on the split-KV kernel
+    DevBuf score;                       // raw scores of a split-KV launch with weights
+    bool use_scores = false;
     DevBuf ml;  // [rows][H] softmax statistics of a step with weights
     cudaStream_t plan_stream = nullptr;  // stream of the last uploads
     cudaEvent_t ev_bounded = nullptr;    // end of the last bounded call
@@ -474,6 +480,7 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 // CTAs than blocks.
 constexpr int64_t kMinBlocksPerCta = 16;
 constexpr int64_t kUnitsPerCta = 3;
+constexpr int64_t kMaxScoreBytes = int64_t(1) << 30;
 constexpr int kFuseMaxNew = 1;  // fuse the append only when split-KV sequences add <= 1 token
 
 int64_t split_kv_ctas(int64_t T, int64_t nu, int64_t max_ctas) {
@@ -780,7 +787,6 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nwide = B->nprefix = B->nprefix_groups = 0;
     B->prefix_keys = B->prefix_token_keys = 0;
     B->seq_kb0.assign(B->nseq, 0);
-    if (B->bounded()) qmax = 0;
     const bool wide_ok = !B->bounded() && P->wide_ok && g <= 128 && 128 % g == 0;
     const int tpt = wide_ok ? 128 / g : 0;  // query tokens per wide item
     std::vector<int> tc_seqs;
@@ -815,13 +821,28 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (wide_ok && B->prefix_sharing != 0 && tc_seqs.size() >= 2) plan_shared_prefixes(B, qmax, tpt, tc_seqs);
     B->nprefix = static_cast<int>(B->w_seq.size()) - B->nwide;
     int64_t T = 0;
+    int64_t score_floats = 0;
+    B->u_bound.clear();
+    B->seq_u.assign(static_cast<size_t>(B->nseq) + 1, 0);
+    B->seq_tc.assign(B->nseq, 0);
     for (int i : tc_seqs) {
         const int n = B->nnew[i];
         const int kb0 = B->seq_kb0[i];
+        B->seq_tc[i] = 1;
         for (int t0 = 0; t0 < n; t0 += qmax) {
             const int nu = std::min(qmax, n - t0);
             const int64_t ctx = static_cast<int64_t>(B->starts[i]) + t0 + nu;
-            T += ceil_div(ctx, P->block_size) - kb0;
+            if (B->bounded()) {
+                const VisibleBlocks vb = visible_blocks(static_cast<int64_t>(B->starts[i]) + t0, ctx, B->window, B->sinks,
+                                                        P->block_size);
+                T += vb.count;
+                B->u_bound.insert(B->u_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(static_cast<uint32_t>(score_floats)),
+                                                     static_cast<int32_t>(score_floats >> 32)});
+                score_floats += vb.count * P->block_size * ((nu * g + 1) & ~1) * P->kvh;
+                B->seq_u[i + 1]++;
+            } else {
+                T += ceil_div(ctx, P->block_size) - kb0;
+            }
             B->u_seq.push_back(i);
             B->u_t0.push_back(t0);
             B->u_n.push_back(nu);
@@ -831,6 +852,27 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         }
     }
     if (T >= (int64_t(1) << 31)) return fail(PK_ERR_UNSUPPORTED, "step reads 2^31 blocks or more");
+    for (int i = 0; i < B->nseq; ++i) B->seq_u[i + 1] += B->seq_u[i];
+    if (!B->bounded()) B->seq_u.clear();
+    // Weights from kept scores, unless those would take more memory than kMaxScoreBytes (a long
+    // chunk cut into many units): then from K once more.
+    B->use_scores = B->weights_mode != 0 && score_floats > 0 &&
+                    score_floats * static_cast<int64_t>(sizeof(float)) <= kMaxScoreBytes;
+    if (B->use_scores) PK_CUDA(B->score.reserve(static_cast<size_t>(score_floats) * sizeof(float)));
+    B->ntouch_tc = 0;
+    if (B->weights_mode != 0) {  // touched blocks of split-KV sequences first
+        std::vector<int32_t> a, b, c, d;
+        for (size_t x = 0; x < B->t_seq.size(); ++x) {
+            const bool tc = B->use_scores && B->seq_tc[B->t_seq[x]];
+            (tc ? a : c).push_back(B->t_seq[x]);
+            (tc ? b : d).push_back(B->t_blk[x]);
+        }
+        B->ntouch_tc = static_cast<int>(a.size());
+        a.insert(a.end(), c.begin(), c.end());
+        b.insert(b.end(), d.begin(), d.end());
+        B->t_seq.swap(a);
+        B->t_blk.swap(b);
+    }
     // Wide CTAs take two items each: neighbouring items of one sequence (chunk) or of one
     // prefix group, which read the same block table. Within each kind the pairs with the
     // most keys go first, so the longest CTAs start in the first wave.
@@ -951,6 +993,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan.add(B->w_slots.data(), B->w_slots.size() * 8);  // 25
     B->plan.add(B->t_seq.data(), B->t_seq.size() * 4);  // 26
     B->plan.add(B->t_blk.data(), B->t_blk.size() * 4);  // 27
+    B->plan.add(B->u_bound.data(), B->u_bound.size() * 4);  // 28
+    B->plan.add(B->seq_u.data(), B->seq_u.size() * 4);  // 29
     if (B->weights_mode != 0)
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
@@ -1044,6 +1088,47 @@ pk::WideParams wide_params(pk_batch* B, int layer, int H, const float* q, float*
     return w;
 }
 
+// Split-KV launch parameters of the plan, without the append.
+pk::TcParams tc_params(pk_batch* B, int layer, int H, const float* q, float* out) {
+    pk_pool* P = B->pool;
+    pk::TcParams p{};
+    p.q = q;
+    p.out = out;
+    p.part_o = static_cast<float*>(B->ws.ptr);
+    p.part_ml = static_cast<float*>(B->ws.ptr) + B->ws_part_o_floats;
+    p.err = static_cast<int*>(B->err.ptr);
+    p.indptr = B->meta.at<int32_t>(0);
+    p.ids = B->meta.at<int32_t>(1);
+    p.starts = B->meta.at<int32_t>(2);
+    p.offsets = B->meta.at<int32_t>(3);
+    p.u_seq = B->plan.at<int32_t>(0);
+    p.u_t0 = B->plan.at<int32_t>(1);
+    p.u_n = B->plan.at<int32_t>(2);
+    p.u_blk = B->plan.at<int32_t>(3);
+    p.u_kb0 = B->nprefix > 0 ? B->plan.at<int32_t>(15) : nullptr;
+    p.lse = B->nprefix > 0 ? static_cast<float*>(B->lse.ptr) : nullptr;
+    p.nu = B->nu;
+    p.total_blocks = B->total_blocks;
+    p.ncta = B->ncta;
+    p.cta_blk = B->plan.at<int32_t>(21);
+    p.u_cta = B->plan.at<int32_t>(23);
+    p.u_meta = B->nu > 0 ? B->plan.at<int4>(24) : nullptr;
+    p.kvh = P->kvh;
+    p.g = H / P->kvh;
+    p.H = H;
+    p.bs = P->block_size;
+    p.stages = P->tc_stages;
+    p.virt = P->tc_virt;
+    p.per_head_layout = P->tc_per_head;
+    p.layer_slot0 = static_cast<int64_t>(layer) * P->num_blocks * P->block_size;
+    p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
+    p.counters = B->plan.at<int>(22);
+    p.unit_counters = p.counters + (static_cast<size_t>(B->nu) + B->ncta) * P->kvh;
+    p.pool_k = reinterpret_cast<__nv_bfloat16*>(P->k_layer(layer));
+    p.pool_v = reinterpret_cast<__nv_bfloat16*>(P->v_layer(layer));
+    return p;
+}
+
 // Host-side fault injection for tests: the next attention call of any batch fails as a
 // launch error would, before it launches anything.
 std::atomic<int> g_inject_launch_failure{0};
@@ -1127,47 +1212,13 @@ int attend_impl(pk_batch* B, int layer, int H, const float* q, float* out, cudaS
         PK_CUDA(prof_end(B, kProfWide, ws));
     }
     if (B->use_tc) {
-        pk::TcParams p{};
-        p.q = q;
-        p.out = out;
-        p.part_o = static_cast<float*>(B->ws.ptr);
-        p.part_ml = static_cast<float*>(B->ws.ptr) + B->ws_part_o_floats;
-        p.err = static_cast<int*>(B->err.ptr);
-        p.indptr = B->meta.at<int32_t>(0);
-        p.ids = B->meta.at<int32_t>(1);
-        p.starts = B->meta.at<int32_t>(2);
-        p.offsets = B->meta.at<int32_t>(3);
-        p.u_seq = B->plan.at<int32_t>(0);
-        p.u_t0 = B->plan.at<int32_t>(1);
-        p.u_n = B->plan.at<int32_t>(2);
-        p.u_blk = B->plan.at<int32_t>(3);
-        p.u_kb0 = B->nprefix > 0 ? B->plan.at<int32_t>(15) : nullptr;
-        p.lse = B->nprefix > 0 ? static_cast<float*>(B->lse.ptr) : nullptr;
-        p.nu = B->nu;
-        p.total_blocks = B->total_blocks;
-        p.ncta = B->ncta;
-        p.cta_blk = B->plan.at<int32_t>(21);
-        p.u_cta = B->plan.at<int32_t>(23);
-        p.u_meta = B->nu > 0 ? B->plan.at<int4>(24) : nullptr;
-        p.kvh = P->kvh;
-        p.g = g;
-        p.H = H;
-        p.bs = P->block_size;
-        p.stages = P->tc_stages;
-        p.virt = P->tc_virt;
-        p.per_head_layout = P->tc_per_head;
-        p.layer_slot0 = static_cast<int64_t>(layer) * P->num_blocks * P->block_size;
-        p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
-        p.counters = B->plan.at<int>(22);
-        p.unit_counters = p.counters + (static_cast<size_t>(B->nu) + B->ncta) * P->kvh;
+        pk::TcParams p = tc_params(B, layer, H, q, out);
         p.k_new = k_new;
         p.v_new = v_new;
-        p.pool_k = reinterpret_cast<__nv_bfloat16*>(P->k_layer(layer));
-        p.pool_v = reinterpret_cast<__nv_bfloat16*>(P->v_layer(layer));
         p.peer = B->peer_out;
         const size_t smem = P->tc_smem + (p.peer.n > 0 ? pk::tc_peer_stage_bytes(P->d) : 0);
         PK_CUDA(prof_begin(B, st));
-        PK_CUDA(pk::launch_tc_attention(P->d, B->nt, &P->tmk, &P->tmv, p, smem, st));
+        PK_CUDA(pk::launch_tc_attention(P->d, B->nt, pk::kTcPlain, &P->tmk, &P->tmv, p, smem, st));
         PK_CUDA(prof_end(B, kProfTc, st));
         B->launches++;
         if (B->nsplit > 0 && p.counters == nullptr) {
@@ -1266,7 +1317,9 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
         }
     }
-    if (k_new != nullptr) {
+    // decode steps append inside the split-KV kernel, as plain steps do
+    const bool fused = k_new != nullptr && B->use_tc && B->ngeneric == 0 && B->fuse_append_ok && B->tc_max_new <= kFuseMaxNew;
+    if (k_new != nullptr && !fused) {
         const bool listed = !B->app_rows.empty();
         const int32_t* rows = listed ? B->meta.at<int32_t>(5) : nullptr;
         const int64_t n = listed ? static_cast<int64_t>(B->app_rows.size()) : B->nrows;
@@ -1304,6 +1357,23 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     p.window = B->window > 0 ? static_cast<int>(B->window) : INT32_MAX;
     p.sinks = static_cast<int>(B->sinks);
     p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
+    if (B->use_tc) {
+        pk::TcParams t = tc_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out));
+        t.u_bound = B->plan.at<int4>(28);
+        t.window = p.window;
+        t.sinks = p.sinks;
+        t.score = B->use_scores ? static_cast<float*>(B->score.ptr) : nullptr;
+        t.ml = p.ml;
+        if (fused) {
+            t.k_new = static_cast<const float*>(k_new);
+            t.v_new = static_cast<const float*>(v_new);
+        }
+        PK_CUDA(prof_begin(B, st));
+        PK_CUDA(pk::launch_tc_attention(P->d, B->nt, io16 ? pk::kTcBounded16 : pk::kTcBounded, &P->tmk, &P->tmv, t,
+                                        P->tc_smem, st));
+        PK_CUDA(prof_end(B, kProfTc, st));
+        B->launches++;
+    }
     if (B->ngeneric > 0) {
         PK_CUDA(prof_begin(B, st));
         PK_CUDA(pk::launch_bounded_rows(P->dtype, io16, p, st));
@@ -1315,10 +1385,36 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.weights = P->weights + static_cast<int64_t>(layer) * P->layer_weights();
         w.t_seq = B->plan.at<int32_t>(26);
         w.t_blk = B->plan.at<int32_t>(27);
-        w.ntouched = static_cast<int>(B->t_seq.size());
+        w.ntouched = B->ntouch_tc;
         w.add = B->weights_mode == 1;
-        PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
-        B->launches++;
+        if (w.ntouched > 0) {
+            pk::ScoreWeightParams sw{};
+            sw.w = w;
+            sw.score = static_cast<const float*>(B->score.ptr);
+            sw.ml = p.ml;
+            sw.seq_u = B->plan.at<int32_t>(29);
+            sw.u_meta = B->plan.at<int4>(24);
+            sw.u_bound = B->plan.at<int4>(28);
+            sw.indptr = p.indptr;
+            sw.ids = p.ids;
+            sw.starts = p.starts;
+            sw.offsets = p.offsets;
+            sw.kvh = p.kvh;
+            sw.g = H / p.kvh;
+            sw.H = H;
+            sw.bs = p.bs;
+            sw.window = p.window;
+            sw.sinks = p.sinks;
+            PK_CUDA(pk::launch_weight_scores(sw, st));
+            B->launches++;
+        }
+        w.t_seq += B->ntouch_tc;
+        w.t_blk += B->ntouch_tc;
+        w.ntouched = static_cast<int>(B->t_seq.size()) - B->ntouch_tc;
+        if (w.ntouched > 0) {
+            PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
+            B->launches++;
+        }
     }
     if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
@@ -1725,6 +1821,7 @@ int pk_batch_destroy(pk_batch* B) {
     B->wpart.release();
     B->qpk.release();
     B->ml.release();
+    B->score.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);
@@ -1851,7 +1948,13 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     for (int i = 0; i < nseq && B->fuse_append_ok; ++i) {
         const int32_t* t = B->ids.data() + B->indptr[i];
         const int32_t n = B->indptr[i + 1] - B->indptr[i];
-        for (int32_t j = 0; j < n; ++j) {
+        // entries outside a window are not read
+        const VisibleBlocks vb = B->window > 0 && B->nnew[i] > 0
+                                     ? visible_blocks(B->starts[i], static_cast<int64_t>(B->starts[i]) + B->nnew[i], B->window,
+                                                      B->sinks, bs)
+                                     : VisibleBlocks{0, 0, n};
+        for (int32_t x = 0; x < vb.count; ++x) {
+            const int32_t j = x < vb.head ? x : x + vb.skip;
             const int32_t b = t[j];
             if (((wbits[b >> 6] >> (b & 63)) & 1) && (B->writer_seq[b] != i || B->writer_idx[b] != j)) {
                 B->fuse_append_ok = false;

@@ -64,10 +64,10 @@ __device__ __forceinline__ int cta_of_block(int j, int T, int n, const int32_t* 
 // mt*16 + grp (+8), columns nt*8 + 2*quad + e) for the live query tokens of a unit.
 // With `lse` set, also the row's log2-domain log-sum-exp m + log2(l) ([rows][H]). With the
 // fused head exchange on (po.n > 0) every row goes to each rank's result buffer instead.
-template <int D, int NT>
+template <int D, int NT, int MODE>
 __device__ __forceinline__ void store_rows(float* out, const float (&acc)[D / 16][NT][4],
                                            const float (&m)[NT][2], const float (&l)[NT][2],
-                                           float* lse, int nq, int g, int H, int row0, int h,
+                                           float* lse, float2* ml, int nq, int g, int H, int row0, int h,
                                            int quad, int grp, const PeerOut& po) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -77,7 +77,25 @@ __device__ __forceinline__ void store_rows(float* out, const float (&acc)[D / 16
             const int tq = col / g;
             if (tq >= nq) continue;
             const float inv = 1.f / l[nt][e];
-            if (po.n == 0) {
+            if constexpr (MODE != kTcPlain) {
+                const size_t orow = static_cast<size_t>(row0 + tq) * H + h * g + col % g;
+                if (ml != nullptr && grp == 0) ml[orow] = make_float2(m[nt][e], inv);
+                if constexpr (MODE == kTcBounded16) {
+                    __nv_bfloat16* op = reinterpret_cast<__nv_bfloat16*>(out) + orow * D;
+#pragma unroll
+                    for (int mt = 0; mt < D / 16; ++mt) {
+                        op[mt * 16 + grp] = __float2bfloat16_rn(acc[mt][nt][e] * inv);
+                        op[mt * 16 + grp + 8] = __float2bfloat16_rn(acc[mt][nt][2 + e] * inv);
+                    }
+                } else {
+                    float* op = out + orow * D;
+#pragma unroll
+                    for (int mt = 0; mt < D / 16; ++mt) {
+                        op[mt * 16 + grp] = acc[mt][nt][e] * inv;
+                        op[mt * 16 + grp + 8] = acc[mt][nt][2 + e] * inv;
+                    }
+                }
+            } else if (po.n == 0) {
                 const size_t orow = static_cast<size_t>(row0 + tq) * H + h * g + col % g;
                 if (lse != nullptr && grp == 0) lse[orow] = m[nt][e] + log2f(l[nt][e]);
                 float* op = out + orow * D;
@@ -146,14 +164,32 @@ __device__ __forceinline__ UnitInfo load_unit(const TcParams& p, int u) {
     return x;
 }
 
+// What a bounded unit reads besides its UnitInfo: block i of the unit is table entry i, and i +
+// skip from i = head on (the sinks in front of the window, then the window); `score` is the
+// unit's place in the score array.
+struct UnitBound {
+    int head, skip;
+    int64_t score;
+};
+__device__ __forceinline__ UnitBound load_bound(const TcParams& p, int u) {
+    const int4 a = __ldg(p.u_bound + u);
+    return UnitBound{a.x, a.y, static_cast<int64_t>(static_cast<uint32_t>(a.z)) | (static_cast<int64_t>(a.w) << 32)};
+}
+
 // CTAs per first-level group of the two-level merge of a unit's partials.
 constexpr int kMergeGroup = 6;
 
-template <int D, int NT>
+// MODE kTcPlain: pagellm's attention over the whole cache. kTcBounded: a window with sinks and /
+// or the raw scores kept for the weights; kTcBounded16: the same with bf16 q, k, v and out rows
+// (then q enters the products as it is, and the scale is applied to the score).
+template <int D, int NT, int MODE>
 __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
     tc_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                    const __grid_constant__ TcParams p) {
     constexpr int KS = D / 16;  // k-steps over the head dim / m-tiles of O^T
+    constexpr bool kBounded = MODE != kTcPlain;
+    constexpr bool kIo16 = MODE == kTcBounded16;
+    constexpr int kIoBytes = kIo16 ? 2 : 4;
     constexpr int CH = TileGeom<D>::kChunks;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -224,8 +260,14 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 const int uend = min(hi, ui.blk1);
                 const int tbase = ui.tbase;
                 // the unit's query rows into L2 while its first blocks stream in
-                prefetch_l2_bulk(p.q + static_cast<size_t>(ui.row0) * p.H * D,
-                                 static_cast<uint32_t>(ui.n) * p.H * D * 4u);
+                prefetch_l2_bulk(reinterpret_cast<const uint8_t*>(p.q) + static_cast<size_t>(ui.row0) * p.H * D * kIoBytes,
+                                 static_cast<uint32_t>(ui.n) * p.H * D * kIoBytes);
+                int head = 0, skip = 0;  // bounded: table entries jump by skip from block `head` on
+                if constexpr (kBounded) {
+                    const UnitBound ub = load_bound(p, u);
+                    head = ui.blk0 + ub.head;
+                    skip = ub.skip;
+                }
                 for (; j < uend; ++j, ++it) {
                     const int s = it % p.stages;
                     const uint32_t k = static_cast<uint32_t>(it / p.stages);
@@ -234,7 +276,7 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                         ok = false;
                         break;
                     }
-                    const int phys = p.ids[tbase + j];
+                    const int phys = p.ids[tbase + j + (kBounded && j >= head ? skip : 0)];
                     const int slot0 = static_cast<int>(p.layer_slot0 + static_cast<int64_t>(phys) * p.bs);
                     uint8_t* kd = ring + s * 2 * tile_bytes;
                     uint8_t* vd = kd + tile_bytes;
@@ -273,6 +315,7 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
             int j = vlo, it = 0, uend = 0, tbase = 0;
             int u = has ? upper_bound_i32(p.u_blk, p.nu + 1, vlo) - 1 : 0;
             bool active = has && j < vhi, fresh = true;
+            int head = 0, skip = 0;
             unsigned long long t_last = global_ns();
             while (__any_sync(0xffffffffu, active)) {
                 bool issued = false;
@@ -281,14 +324,19 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                         const UnitInfo ui = load_unit(p, u);
                         uend = min(vhi, ui.blk1);
                         tbase = ui.tbase;
-                        prefetch_l2_bulk(p.q + static_cast<size_t>(ui.row0) * p.H * D,
-                                         static_cast<uint32_t>(ui.n) * p.H * D * 4u);
+                        prefetch_l2_bulk(reinterpret_cast<const uint8_t*>(p.q) + static_cast<size_t>(ui.row0) * p.H * D * kIoBytes,
+                                         static_cast<uint32_t>(ui.n) * p.H * D * kIoBytes);
+                        if constexpr (kBounded) {
+                            const UnitBound ub = load_bound(p, u);
+                            head = ui.blk0 + ub.head;
+                            skip = ub.skip;
+                        }
                         fresh = false;
                     }
                     const int s = it % p.stages;
                     const uint32_t k = static_cast<uint32_t>(it / p.stages);
                     if (mbar_test_wait(&pe[s], (k & 1u) ^ 1u)) {
-                        const int phys = p.ids[tbase + j];
+                        const int phys = p.ids[tbase + j + (kBounded && j >= head ? skip : 0)];
                         const int slot0 = static_cast<int>(p.layer_slot0 + static_cast<int64_t>(phys) * p.bs);
                         uint8_t* kd = vr + s * 2 * tile_bytes;
                         uint8_t* vd = kd + tile_bytes;
@@ -351,19 +399,24 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
         // Q's low half (q - bf16(q)) only where registers allow it: with two n8 tiles or
         // head_dim 256 the 168-register cap of a 9-warp CTA would spill it, so there Q is
         // used at bf16 (the precision the wide-tile kernel uses throughout).
-        constexpr bool kLo = NT == 1 && D <= 128;
+        constexpr bool kLo = NT == 1 && D <= 128 && !kIo16;
         uint32_t qh[KS][NT][2], ql[kLo ? KS : 1][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int col = nt * 8 + grp;
             const int tq = col / g;
             const bool live = tq < nq;
-            const float* qp = p.q + (static_cast<size_t>(row0 + (live ? tq : 0)) * p.H + h * g +
-                                     col % g) * D;
+            const size_t qoff = (static_cast<size_t>(row0 + (live ? tq : 0)) * p.H + h * g + col % g) * D;
+            const float* qp = p.q + qoff;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
+                    if constexpr (kIo16) {
+                        const __nv_bfloat16* q16 = reinterpret_cast<const __nv_bfloat16*>(p.q) + qoff;
+                        qh[ks][nt][half] = live ? *reinterpret_cast<const uint32_t*>(q16 + ks * 16 + half * 8 + 2 * quad) : 0u;
+                        continue;
+                    }
                     float2 x = make_float2(0.f, 0.f);
                     if (live) x = *reinterpret_cast<const float2*>(qp + ks * 16 + half * 8 + 2 * quad);
                     x.x *= p.qscale;
@@ -383,6 +436,19 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 const int tq = (nt * 8 + 2 * quad + e) / g;
                 lim[nt][e] = tq < nq ? qpos0 + tq : -1;
             }
+
+        int head = 0, skip = 0;
+        float* score = nullptr;  // bounded, weights: this (unit, KV head)'s scores [block][token][column]
+        int colp = 0;            // columns of a score row (live ones, padded to an even number)
+        if constexpr (kBounded) {
+            const UnitBound ub = load_bound(p, u);
+            head = ub.head;
+            skip = ub.skip;
+            if (p.score != nullptr) {
+                colp = (nq * g + 1) & ~1;
+                score = p.score + ub.score + static_cast<int64_t>(h) * (ublk1 - ublk0) * p.bs * colp;
+            }
+        }
 
         float m[NT][2], l[NT][2];
         float acc[KS][NT][4];
@@ -411,7 +477,8 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
             }
             const uint32_t kst = smem_u32(ring + s * 2 * tile_bytes);
             const uint32_t vst = kst + tile_bytes;
-            const int kpos0 = (j - ublk0 + kb0) * p.bs;
+            const int jump = kBounded && j - ublk0 >= head ? skip : 0;
+            const int kpos0 = (j - ublk0 + kb0 + jump) * p.bs;
             const int nvalid = min(p.bs, uctx - kpos0);
             if (nvalid < p.bs) {
                 // Slots past the context may hold anything; zero this head's V rows there so
@@ -428,6 +495,20 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 }
                 __syncwarp();
             }
+            bool cleared = false;
+            if constexpr (kBounded) {
+                // The same for rows between the sinks and the first row's window, which no row of
+                // the unit sees: the caller may have given their slots away.
+                const int a = max(0, p.sinks - kpos0), b = min(p.bs, max(0, qpos0 - p.window + 1) - kpos0);
+                if (a < b) {
+                    cleared = true;
+                    uint8_t* vgen = ring + s * 2 * tile_bytes + tile_bytes;
+                    for (int x = lane; x < (b - a) * CH * 8; x += 32)
+                        *reinterpret_cast<uint4*>(vgen + tile_off((x / 8) % CH, h, a + x / (CH * 8), x % 8, p.kvh, p.bs, CH,
+                                                                  p.per_head_layout)) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+            }
             // Rows appended in this step (positions >= the sequence's start) come from the
             // fp32 inputs, rounded to bf16, instead of from the pool; the unit whose own
             // query rows they are also stores them to the pool (the fused append).
@@ -440,13 +521,34 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     patched = true;
                     uint8_t* kgen = ring + s * 2 * tile_bytes;
                     uint8_t* vgen = kgen + tile_bytes;
-                    const int phys = p.ids[ui.tbase + j];
+                    const int phys = p.ids[ui.tbase + j + jump];
                     const int row_base = row0 - qpos0;  // row of position pos: row_base + pos
                     // (position, 4-dim) items, lane-strided; each batch issues all its loads
                     // (read-only inputs) before any store, so the rows' latencies overlap.
                     constexpr int kPerRow = D / 4;
                     constexpr int kBatch = (NT == 1 && D <= 128) ? 2 : 1;  // register budget
                     const int items = (hi_pos - lo_pos) * kPerRow;
+                    if constexpr (kIo16) {
+                        const __nv_bfloat16* k16 = reinterpret_cast<const __nv_bfloat16*>(p.k_new);
+                        const __nv_bfloat16* v16 = reinterpret_cast<const __nv_bfloat16*>(p.v_new);
+                        for (int it2 = lane; it2 < items; it2 += 32) {
+                            const int pos = lo_pos + it2 / kPerRow;
+                            const int d0 = (it2 % kPerRow) * 4;
+                            const int t = pos - kpos0;
+                            const size_t src = (static_cast<size_t>(row_base + pos) * p.kvh + h) * D + d0;
+                            const uint2 kb = __ldg(reinterpret_cast<const uint2*>(k16 + src));
+                            const uint2 vb = __ldg(reinterpret_cast<const uint2*>(v16 + src));
+                            const uint32_t off = tile_off(d0 >> 6, h, t, (d0 & 63) >> 3, p.kvh, p.bs, CH,
+                                                          p.per_head_layout) + ((d0 & 7) ? 8u : 0u);
+                            *reinterpret_cast<uint2*>(kgen + off) = kb;
+                            *reinterpret_cast<uint2*>(vgen + off) = vb;
+                            if (pos >= qpos0) {
+                                const size_t dst = (static_cast<size_t>(phys) * p.bs + t) * p.kvh * D + h * D + d0;
+                                *reinterpret_cast<uint2*>(p.pool_k + dst) = kb;
+                                *reinterpret_cast<uint2*>(p.pool_v + dst) = vb;
+                            }
+                        }
+                    } else
                     for (int base = 0; base < items; base += 32 * kBatch) {
                         float4 kx[kBatch], vx[kBatch];
 #pragma unroll
@@ -513,8 +615,23 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     float pr[4];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float xa = (kp_a <= lim[nt][e] && kp_a < uctx) ? sacc[nt][e] : -INFINITY;
-                        const float xb = (kp_b <= lim[nt][e] && kp_b < uctx) ? sacc[nt][2 + e] : -INFINITY;
+                        bool see_a = kp_a <= lim[nt][e] && kp_a < uctx;
+                        bool see_b = kp_b <= lim[nt][e] && kp_b < uctx;
+                        if constexpr (kBounded) {
+                            const int wlo = lim[nt][e] - p.window;  // keys up to it are past the window
+                            see_a = see_a && (kp_a > wlo || kp_a < p.sinks);
+                            see_b = see_b && (kp_b > wlo || kp_b < p.sinks);
+                        }
+                        if constexpr (kIo16) {
+                            sacc[nt][e] *= p.qscale;
+                            sacc[nt][2 + e] *= p.qscale;
+                        }
+                        const float xa = see_a ? sacc[nt][e] : -INFINITY;
+                        const float xb = see_b ? sacc[nt][2 + e] : -INFINITY;
+                        if constexpr (kBounded) {
+                            sacc[nt][e] = xa;
+                            sacc[nt][2 + e] = xb;
+                        }
                         float mx = fmaxf(xa, xb);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
@@ -533,6 +650,15 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                         }
                         pr[e] = pa;
                         pr[2 + e] = pbv;
+                    }
+                    if constexpr (kBounded) {
+                        // scores for the weights: 8 lanes of a quad column cover 8 keys' rows
+                        const int c0 = nt * 8 + 2 * quad;
+                        if (score != nullptr && c0 < colp) {
+                            float* sp = score + (static_cast<int64_t>(j - ublk0) * p.bs + mtile * 16 + grp) * colp + c0;
+                            *reinterpret_cast<float2*>(sp) = make_float2(sacc[nt][0], sacc[nt][1]);
+                            *reinterpret_cast<float2*>(sp + 8 * colp) = make_float2(sacc[nt][2], sacc[nt][3]);
+                        }
                     }
                     // P^T C-fragment rows grp / grp+8 -> B operand (k = token, n = column)
                     pb[nt][0] = movmatrix_trans(pack_bf16(pr[0], pr[1]));
@@ -553,7 +679,7 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 }
             }
             // Generic-proxy writes into the stage must be ordered before the next TMA fill.
-            if (nvalid < p.bs || patched) fence_proxy_async_smem();
+            if (nvalid < p.bs || patched || cleared) fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&vempty[s]);
         }
@@ -583,8 +709,8 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
         // 16-byte stores in 512-byte runs (rows of a token's g heads are contiguous there);
         // elsewhere store_rows.
         auto store_out = [&](const float (&o)[KS][NT][4], const float (&mm)[NT][2], const float (&ll)[NT][2]) {
-            if (p.peer.n == 0) {
-                store_rows<D, NT>(p.out, o, mm, ll, p.lse, nq, g, p.H, row0, h, quad, grp, p.peer);
+            if (kBounded || p.peer.n == 0) {
+                store_rows<D, NT, MODE>(p.out, o, mm, ll, p.lse, p.ml, nq, g, p.H, row0, h, quad, grp, p.peer);
                 return;
             }
             // Every rank receives the rows as whole 512-byte runs of 16-byte stores: 4 rows at a
@@ -819,7 +945,7 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
             }
         }
     }
-    if (p.peer.n > 0) {
+    if (!kBounded && p.peer.n > 0) {
         // Fused head exchange: every consumer warp (with work or not, timed out or not) counts
         // itself done with an acquire-release increment at system scope, which orders its rows'
         // stores before the count; the last of the launch, which has acquired every other
@@ -891,10 +1017,10 @@ __global__ void merge_kernel(const MergeParams p) {
     }
 }
 
-template <int D, int NT>
+template <int D, int NT, int MODE>
 cudaError_t launch_tc_t(const CUtensorMap* tmk, const CUtensorMap* tmv, const TcParams& p,
                         size_t smem, cudaStream_t st) {
-    auto kern = tc_attn_kernel<D, NT>;
+    auto kern = tc_attn_kernel<D, NT, MODE>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
@@ -918,14 +1044,22 @@ size_t tc_smem_bytes(int D, int bs, int kvh, int stages, int virt) {
            kTcMaxKvHeads * sizeof(uint64_t) + 1024;
 }
 
-cudaError_t launch_tc_attention(int D, int NT, const CUtensorMap* tmk, const CUtensorMap* tmv,
-                                const TcParams& p, size_t smem, cudaStream_t st) {
-    if (D == 64 && NT == 1) return launch_tc_t<64, 1>(tmk, tmv, p, smem, st);
-    if (D == 64 && NT == 2) return launch_tc_t<64, 2>(tmk, tmv, p, smem, st);
-    if (D == 128 && NT == 1) return launch_tc_t<128, 1>(tmk, tmv, p, smem, st);
-    if (D == 128 && NT == 2) return launch_tc_t<128, 2>(tmk, tmv, p, smem, st);
-    if (D == 256 && NT == 1) return launch_tc_t<256, 1>(tmk, tmv, p, smem, st);
+template <int MODE>
+static cudaError_t launch_tc_mode(int D, int NT, const CUtensorMap* tmk, const CUtensorMap* tmv, const TcParams& p,
+                                  size_t smem, cudaStream_t st) {
+    if (D == 64 && NT == 1) return launch_tc_t<64, 1, MODE>(tmk, tmv, p, smem, st);
+    if (D == 64 && NT == 2) return launch_tc_t<64, 2, MODE>(tmk, tmv, p, smem, st);
+    if (D == 128 && NT == 1) return launch_tc_t<128, 1, MODE>(tmk, tmv, p, smem, st);
+    if (D == 128 && NT == 2) return launch_tc_t<128, 2, MODE>(tmk, tmv, p, smem, st);
+    if (D == 256 && NT == 1) return launch_tc_t<256, 1, MODE>(tmk, tmv, p, smem, st);
     return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_tc_attention(int D, int NT, int mode, const CUtensorMap* tmk, const CUtensorMap* tmv,
+                                const TcParams& p, size_t smem, cudaStream_t st) {
+    if (mode == kTcBounded) return launch_tc_mode<kTcBounded>(D, NT, tmk, tmv, p, smem, st);
+    if (mode == kTcBounded16) return launch_tc_mode<kTcBounded16>(D, NT, tmk, tmv, p, smem, st);
+    return launch_tc_mode<kTcPlain>(D, NT, tmk, tmv, p, smem, st);
 }
 
 cudaError_t launch_merge(const MergeParams& p, int nsplit, cudaStream_t st) {

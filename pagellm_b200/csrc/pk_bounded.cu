@@ -182,6 +182,46 @@ cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, 
     return cudaGetLastError();
 }
 
+// The scores of the touched blocks are still in L2 (8 to 64 bytes per key and KV head beside the
+// 512 of its K and V), so summing them costs a fraction of reading K again. Units of a sequence in
+// order, columns in order: the sum does not depend on the schedule.
+__global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightParams p) {
+    const int64_t x = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+    const int64_t e64 = x / (p.kvh * p.bs);
+    if (e64 >= p.w.ntouched) return;
+    const int e = static_cast<int>(e64);
+    const int hx = static_cast<int>(x - e64 * (p.kvh * p.bs));
+    const int h = hx / p.bs, t = hx - h * p.bs;
+    const int seq = p.w.t_seq[e], lb = p.w.t_blk[e];
+    const int start = p.starts[seq], ctx = start + p.offsets[seq + 1] - p.offsets[seq];
+    const int j = lb * p.bs + t;
+    if (j >= ctx || (j >= p.sinks && j <= start - p.window)) return;
+    float sum = 0.f;
+    for (int u = p.seq_u[seq]; u < p.seq_u[seq + 1]; ++u) {
+        const int4 b = __ldg(p.u_bound + u);
+        const int4 m0 = __ldg(p.u_meta + 2 * u), m1 = __ldg(p.u_meta + 2 * u + 1);
+        const int nblk = m1.z - m1.y;
+        const int i = lb < b.x ? lb : lb - b.y;
+        if (i >= nblk || (lb >= b.x && i < b.x)) continue;  // not a block of this unit
+        const int ncol = m0.y * p.g, colp = (ncol + 1) & ~1;
+        const float* sp = p.score + (static_cast<int64_t>(static_cast<uint32_t>(b.z)) | (static_cast<int64_t>(b.w) << 32)) +
+                          ((static_cast<int64_t>(h) * nblk + i) * p.bs + t) * colp;
+        const float2* ml = p.ml + static_cast<size_t>(m0.w) * p.H + h * p.g;
+        for (int c = 0; c < ncol; c += 2) {
+            const float2 s = __ldcg(reinterpret_cast<const float2*>(sp + c));
+            const float2 a = __ldg(ml + (c / p.g) * p.H + c % p.g);
+            sum += exp2f(s.x - a.x) * a.y;
+            if (c + 1 < ncol) {
+                const float2 b2 = __ldg(ml + ((c + 1) / p.g) * p.H + (c + 1) % p.g);
+                sum += exp2f(s.y - b2.x) * b2.y;
+            }
+        }
+    }
+    const int phys = p.ids[p.indptr[seq] + lb];
+    float* dst = p.w.weights + (static_cast<size_t>(phys) * p.kvh + h) * p.bs + t;
+    *dst = p.w.add && j < start ? *dst + sum : sum;
+}
+
 // ------------------------------------------------------------------ append of bf16 rows
 // Step rows given as bf16 are stored as they are; the slot comes from the block table (row ->
 // sequence -> position -> block id). W: the widest word that divides a row.
@@ -388,6 +428,15 @@ cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, con
     if (dtype == 0) return io16 ? cudaErrorInvalidValue : launch_weight_rows_t<float, float>(p, w, st);
     return io16 ? launch_weight_rows_t<__nv_bfloat16, __nv_bfloat16>(p, w, st)
                 : launch_weight_rows_t<__nv_bfloat16, float>(p, w, st);
+}
+
+cudaError_t launch_weight_scores(const ScoreWeightParams& p, cudaStream_t st) {
+    if (p.w.ntouched <= 0) return cudaSuccess;
+    const int64_t threads = static_cast<int64_t>(p.w.ntouched) * p.kvh * p.bs;
+    const int64_t blocks = (threads + 255) / 256;
+    if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+    weight_scores_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(p);
+    return cudaGetLastError();
 }
 
 cudaError_t launch_append_rows16(void* pool_k_layer, void* pool_v_layer, const void* k, const void* v,

@@ -94,7 +94,15 @@ struct TcParams {
     __nv_bfloat16* pool_k;
     __nv_bfloat16* pool_v;
     PeerOut peer;  // n == 0: rows go to `out` (H heads per row)
+    // Bounded modes. q, out, k_new and v_new point at bf16 rows in kTcBounded16.
+    const int4* u_bound;  // [nu] {head, skip, score lo, score hi}: see UnitBound in the kernel
+    int window;           // >= 1; INT32_MAX without a window
+    int sinks;
+    float* score;         // masked log2-domain scores per (unit, KV head), or NULL
+    float2* ml;           // [rows][H] (max, 1 / sum) of each output row, log2 domain, or NULL
 };
+
+enum TcMode { kTcPlain = 0, kTcBounded = 1, kTcBounded16 = 2 };
 
 struct MergeParams {
     float* out;
@@ -209,6 +217,27 @@ struct WeightParams {
     int add;  // add to the weights of tokens cached before the step (else store)
 };
 
+// Weights from the scores that a bounded split-KV launch kept: one thread per (touched block, KV
+// head, token).
+struct ScoreWeightParams {
+    WeightParams w;
+    const float* score;
+    const float2* ml;
+    const int32_t* seq_u;   // [nseq + 1] first unit of each sequence
+    const int4* u_meta;     // units as in TcParams
+    const int4* u_bound;
+    const int32_t* indptr;
+    const int32_t* ids;
+    const int32_t* starts;
+    const int32_t* offsets;
+    int kvh;
+    int g;
+    int H;
+    int bs;
+    int window;
+    int sinks;
+};
+
 struct EvictParams {
     void* pool_k;
     void* pool_v;
@@ -252,7 +281,7 @@ struct PoolView {
     const CUtensorMap* tmv;
 };
 
-cudaError_t launch_tc_attention(int D, int NT, const CUtensorMap* tmk, const CUtensorMap* tmv,
+cudaError_t launch_tc_attention(int D, int NT, int mode, const CUtensorMap* tmk, const CUtensorMap* tmv,
                                 const TcParams& p, size_t smem, cudaStream_t st);
 size_t tc_smem_bytes(int D, int bs, int kvh, int stages, int virt);
 // Shared memory a launch with the fused head exchange needs beyond tc_smem_bytes (each consumer
@@ -317,6 +346,7 @@ cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const i
 
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
+cudaError_t launch_weight_scores(const ScoreWeightParams& p, cudaStream_t st);
 // launch_append_table for rows given as bf16 (bf16 pools).
 cudaError_t launch_append_rows16(void* pool_k_layer, void* pool_v_layer, const void* k, const void* v,
                                  const int32_t* row_seq, const int32_t* offsets, const int32_t* starts,

@@ -239,7 +239,7 @@ extern "C" PK_API int pk_decode_attend_static(const pk_pool* pool, int layer, in
     p.per_head_layout = P.tc_per_head;
     p.layer_slot0 = static_cast<int64_t>(layer) * P.num_blocks * bs;
     p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P.d)));
-    e = pk::launch_tc_attention(P.d, 1, P.tmk, P.tmv, p, P.tc_smem, st);
+    e = pk::launch_tc_attention(P.d, 1, pk::kTcPlain, P.tmk, P.tmv, p, P.tc_smem, st);
     if (e != cudaSuccess) return sfail(PK_ERR_CUDA, "attention launch: %s", cudaGetErrorString(e));
     if (nsplit > 0) {
         pk::MergeParams mp{};
