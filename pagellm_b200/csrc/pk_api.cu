@@ -281,6 +281,7 @@ struct pk_batch {
     std::vector<int32_t> w_pair;   // item pairs: chunk pairs, then prefix pairs
     int npair_chunk = 0, npair_prefix = 0;
     // wide-kernel schedule: per CTA a range of segments (pair, head, key tiles, slot, ph)
+    std::vector<int32_t> pair_bound;  // bounded pairs: tiles in front of the jump, the jump, first key of the window
     std::vector<int32_t> pair_kend, cta_seg, seg, ph_info, split;
     int ncta_chunk = 0, ncta_prefix = 0, nslots = 0, nph = 0, nwsplit = 0;
     int nwsplit_chunk = 0;  // the first nwsplit_chunk entries of split belong to chunk pairs
@@ -312,7 +313,10 @@ struct pk_batch {
     int weights_mode = 0;
     bool bounds_stale = false;
     std::vector<int32_t> t_seq, t_blk;  // touched blocks (weights): sequence, table index
-    int ntouch_tc = 0;                  // the first ones belong to sequences on the split-KV kernel
+    int ntouch_tc = 0, ntouch_wide = 0;  // first those of sequences on the split-KV kernel, then chunks'
+    std::vector<int32_t> pieces;        // chunks' weights: sequence, key tile, first and end query item
+    std::vector<int32_t> t_piece;       // per touched block of a chunk: first piece of its tile, pieces
+    DevBuf wpieces;                     // [pieces][kvh][128] sums
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
     std::vector<uint8_t> seq_tc;        // scratch: sequence is on the split-KV kernel
@@ -548,6 +552,22 @@ int cta_of_block(const std::vector<int32_t>& first, int64_t j) {
 }
 
 
+// The blocks that the rows at positions q0 .. ctx-1 of a sequence read: table indices
+// [0, head) and [head + skip, head + skip + rest), where the first part holds the sinks in
+// front of row q0's window. Without a window: all of them, head = skip = 0.
+struct VisibleBlocks {
+    int head, skip;
+    int64_t count;
+};
+VisibleBlocks visible_blocks(int64_t q0, int64_t ctx, int64_t window, int64_t sinks, int bs) {
+    const int64_t end = (ctx + bs - 1) / bs;
+    if (window <= 0) return {0, 0, end};
+    const int64_t lo = std::max<int64_t>(0, q0 - window + 1);
+    const int64_t head = (std::min(sinks, lo) + bs - 1) / bs;
+    const int64_t first = std::max(lo / bs, head);
+    return {static_cast<int>(head), static_cast<int>(first - head), head + end - first};
+}
+
 // Shared prefixes (cascade attention). Sequences whose block tables begin with the same
 // block ids - forks and prefix-cache hits in pagellm (cache/paged.py:187-203, :257-263) -
 // hold bit-identical K/V there. For a group of them, the wide-tile kernel attends every
@@ -660,7 +680,19 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
     B->ph_info.clear();
     B->split.clear();
     B->nslots = B->nwsplit = B->nwsplit_chunk = 0;
-    auto tiles = [&](int x) { return static_cast<int64_t>(ceil_div(B->pair_kend[x], pk::kWideKeys)); };
+    std::vector<int64_t> pair_tiles(npairs);
+    B->pair_bound.clear();
+    for (int x = 0; x < npairs; ++x) {
+        pair_tiles[x] = ceil_div(B->pair_kend[x], pk::kWideKeys);
+        if (!B->bounded()) continue;
+        // the window of the pair's first row (items and their tokens are in position order)
+        const int64_t q0 = B->tok_pos[B->w_tok0[B->w_pair[2 * x]]];
+        const VisibleBlocks vb = visible_blocks(q0, B->pair_kend[x], B->window, B->sinks, pk::kWideKeys);
+        pair_tiles[x] = vb.count;
+        const int64_t lo = B->window > 0 ? std::max<int64_t>(0, q0 - B->window + 1) : 0;
+        B->pair_bound.insert(B->pair_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(lo), 0});
+    }
+    auto tiles = [&](int x) { return pair_tiles[x]; };
     // Schedules the pair-heads of pairs [x0, x1) over at most G CTAs; returns the CTAs used.
     // whole_only: no pair-head is cut (the makespan is at least the longest pair-head).
     auto stream_k = [&](int x0, int x1, int64_t G, bool whole_only) -> int {
@@ -748,20 +780,51 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
     B->nwsplit = static_cast<int>(B->split.size() / 4);
 }
 
-// The blocks that the rows at positions q0 .. ctx-1 of a sequence read: table indices
-// [0, head) and [head + skip, head + skip + rest), where the first part holds the sinks in
-// front of row q0's window. Without a window: all of them, head = skip = 0.
-struct VisibleBlocks {
-    int head, skip;
-    int64_t count;
-};
-VisibleBlocks visible_blocks(int64_t q0, int64_t ctx, int64_t window, int64_t sinks, int bs) {
-    const int64_t end = (ctx + bs - 1) / bs;
-    if (window <= 0) return {0, 0, end};
-    const int64_t lo = std::max<int64_t>(0, q0 - window + 1);
-    const int64_t head = (std::min(sinks, lo) + bs - 1) / bs;
-    const int64_t first = std::max(lo / bs, head);
-    return {static_cast<int>(head), static_cast<int>(first - head), head + end - first};
+// Pieces of the chunks' weights: for every key tile that holds a touched block, the query items
+// that see a key of it, cut so that all pieces together (x KV heads) fill two CTAs per SM evenly. A
+// piece has at least kMinPieceItems items: it loads the key tile and fills its pipeline first.
+constexpr int64_t kMinPieceItems = 4;
+void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::vector<int32_t>& tb) {
+    pk_pool* P = B->pool;
+    struct Tile {
+        int seq, kt, i0, i1;
+    };
+    std::vector<Tile> tiles;
+    std::vector<int> of(ts.size());
+    std::vector<int> first_item(B->nseq, -1), end_item(B->nseq, 0);
+    for (int x = 0; x < B->nwide; ++x) {
+        if (first_item[B->w_seq[x]] < 0) first_item[B->w_seq[x]] = x;
+        end_item[B->w_seq[x]] = x + 1;
+    }
+    int64_t total = 0;
+    for (size_t x = 0; x < ts.size(); ++x) {
+        const int kt = tb[x] * P->block_size / pk::kWideKeys;
+        if (tiles.empty() || tiles.back().seq != ts[x] || tiles.back().kt != kt) {
+            const int64_t k0 = static_cast<int64_t>(kt) * pk::kWideKeys, k1 = k0 + pk::kWideKeys - 1;
+            Tile t{ts[x], kt, first_item[ts[x]], end_item[ts[x]]};
+            auto pos = [&](int item, bool last) {
+                return static_cast<int64_t>(B->tok_pos[B->w_tok0[item] + (last ? B->w_ntok[item] - 1 : 0)]);
+            };
+            while (t.i0 < t.i1 && pos(t.i0, true) < k0) ++t.i0;  // rows before the tile
+            if (B->window > 0 && k0 >= B->sinks)                 // rows whose window begins behind it
+                while (t.i1 > t.i0 && pos(t.i1 - 1, false) - B->window >= k1) --t.i1;
+            total += t.i1 - t.i0;
+            tiles.push_back(t);
+        }
+        of[x] = static_cast<int>(tiles.size()) - 1;
+    }
+    const int64_t per = std::max<int64_t>(kMinPieceItems, (total * P->kvh + 2 * P->num_sms - 1) / (2 * P->num_sms));
+    std::vector<int32_t> p0(tiles.size()), np(tiles.size());
+    for (size_t x = 0; x < tiles.size(); ++x) {
+        const Tile& t = tiles[x];
+        const int64_t n = t.i1 - t.i0, cuts = (n + per - 1) / per;
+        p0[x] = static_cast<int32_t>(B->pieces.size() / 4);
+        np[x] = static_cast<int32_t>(cuts);
+        for (int64_t c = 0; c < cuts; ++c)
+            B->pieces.insert(B->pieces.end(), {t.seq, t.kt, static_cast<int32_t>(t.i0 + c * n / cuts),
+                                               static_cast<int32_t>(t.i0 + (c + 1) * n / cuts)});
+    }
+    for (size_t x = 0; x < ts.size(); ++x) B->t_piece.insert(B->t_piece.end(), {p0[of[x]], np[of[x]]});
 }
 
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
@@ -787,7 +850,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nwide = B->nprefix = B->nprefix_groups = 0;
     B->prefix_keys = B->prefix_token_keys = 0;
     B->seq_kb0.assign(B->nseq, 0);
-    const bool wide_ok = !B->bounded() && P->wide_ok && g <= 128 && 128 % g == 0;
+    const bool wide_ok = P->wide_ok && g <= 128 && 128 % g == 0;
     const int tpt = wide_ok ? 128 / g : 0;  // query tokens per wide item
     std::vector<int> tc_seqs;
     for (int i = 0; i < B->nseq; ++i) {
@@ -818,7 +881,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nwide = static_cast<int>(B->w_seq.size());
     B->tc_max_new = 0;
     for (int i : tc_seqs) B->tc_max_new = std::max(B->tc_max_new, B->nnew[i]);
-    if (wide_ok && B->prefix_sharing != 0 && tc_seqs.size() >= 2) plan_shared_prefixes(B, qmax, tpt, tc_seqs);
+    if (wide_ok && !B->bounded() && B->prefix_sharing != 0 && tc_seqs.size() >= 2) plan_shared_prefixes(B, qmax, tpt, tc_seqs);
     B->nprefix = static_cast<int>(B->w_seq.size()) - B->nwide;
     int64_t T = 0;
     int64_t score_floats = 0;
@@ -859,19 +922,30 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->use_scores = B->weights_mode != 0 && score_floats > 0 &&
                     score_floats * static_cast<int64_t>(sizeof(float)) <= kMaxScoreBytes;
     if (B->use_scores) PK_CUDA(B->score.reserve(static_cast<size_t>(score_floats) * sizeof(float)));
-    B->ntouch_tc = 0;
-    if (B->weights_mode != 0) {  // touched blocks of split-KV sequences first
-        std::vector<int32_t> a, b, c, d;
+    B->ntouch_tc = B->ntouch_wide = 0;
+    B->pieces.clear();
+    B->t_piece.clear();
+    if (B->weights_mode != 0) {
+        // touched blocks by the kernel that sums them: kept scores, chunks, K once more
+        std::vector<int32_t> ts[3], tb[3];
+        std::vector<uint8_t> wide_seq(B->nseq, 0);
+        for (int i : B->w_seq) wide_seq[i] = 1;
         for (size_t x = 0; x < B->t_seq.size(); ++x) {
-            const bool tc = B->use_scores && B->seq_tc[B->t_seq[x]];
-            (tc ? a : c).push_back(B->t_seq[x]);
-            (tc ? b : d).push_back(B->t_blk[x]);
+            const int i = B->t_seq[x];
+            const int k = wide_seq[i] ? 1 : B->use_scores && B->seq_tc[i] ? 0 : 2;
+            ts[k].push_back(i);
+            tb[k].push_back(B->t_blk[x]);
         }
-        B->ntouch_tc = static_cast<int>(a.size());
-        a.insert(a.end(), c.begin(), c.end());
-        b.insert(b.end(), d.begin(), d.end());
-        B->t_seq.swap(a);
-        B->t_blk.swap(b);
+        B->ntouch_tc = static_cast<int>(ts[0].size());
+        B->ntouch_wide = static_cast<int>(ts[1].size());
+        plan_weight_pieces(B, ts[1], tb[1]);
+        B->t_seq.clear();
+        B->t_blk.clear();
+        for (int k = 0; k < 3; ++k) {
+            B->t_seq.insert(B->t_seq.end(), ts[k].begin(), ts[k].end());
+            B->t_blk.insert(B->t_blk.end(), tb[k].begin(), tb[k].end());
+        }
+        PK_CUDA(B->wpieces.reserve(B->pieces.size() / 4 * P->kvh * pk::kWideKeys * sizeof(float)));
     }
     // Wide CTAs take two items each: neighbouring items of one sequence (chunk) or of one
     // prefix group, which read the same block table. Within each kind the pairs with the
@@ -995,6 +1069,9 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan.add(B->t_blk.data(), B->t_blk.size() * 4);  // 27
     B->plan.add(B->u_bound.data(), B->u_bound.size() * 4);  // 28
     B->plan.add(B->seq_u.data(), B->seq_u.size() * 4);  // 29
+    B->plan.add(B->pair_bound.data(), B->pair_bound.size() * 4);  // 30
+    B->plan.add(B->pieces.data(), B->pieces.size() * 4);  // 31
+    B->plan.add(B->t_piece.data(), B->t_piece.size() * 4);  // 32
     if (B->weights_mode != 0)
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
@@ -1085,6 +1162,7 @@ pk::WideParams wide_params(pk_batch* B, int layer, int H, const float* q, float*
     w.bs = P->block_size;
     w.layer_slot0 = static_cast<int64_t>(layer) * P->num_blocks * P->block_size;
     w.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
+    w.sscale = 1.f;
     return w;
 }
 
@@ -1317,8 +1395,10 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
         }
     }
-    // decode steps append inside the split-KV kernel, as plain steps do
-    const bool fused = k_new != nullptr && B->use_tc && B->ngeneric == 0 && B->fuse_append_ok && B->tc_max_new <= kFuseMaxNew;
+    // decode steps append inside the split-KV kernel and chunk rows with the packing of their
+    // queries, as in plain steps
+    const bool fused = k_new != nullptr && (B->use_tc || B->nwide > 0) && B->ngeneric == 0 && B->fuse_append_ok &&
+                       B->tc_max_new <= kFuseMaxNew;
     if (k_new != nullptr && !fused) {
         const bool listed = !B->app_rows.empty();
         const int32_t* rows = listed ? B->meta.at<int32_t>(5) : nullptr;
@@ -1357,6 +1437,52 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     p.window = B->window > 0 ? static_cast<int>(B->window) : INT32_MAX;
     p.sinks = static_cast<int>(B->sinks);
     p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(P->d)));
+    // chunk items, on the side stream when split-KV work runs beside them
+    const bool fork = B->nwide > 0 && B->use_tc;
+    pk::WideParams wide{};
+    if (B->nwide > 0) {
+        cudaStream_t ws = st;
+        if (fork) {
+            if (!B->side) PK_CUDA(cudaStreamCreateWithFlags(&B->side, cudaStreamNonBlocking));
+            if (!B->ev_fork) PK_CUDA(cudaEventCreateWithFlags(&B->ev_fork, cudaEventDisableTiming));
+            if (!B->ev_join) PK_CUDA(cudaEventCreateWithFlags(&B->ev_join, cudaEventDisableTiming));
+            PK_CUDA(cudaEventRecord(B->ev_fork, st));
+            PK_CUDA(cudaStreamWaitEvent(B->side, B->ev_fork, 0));
+            ws = B->side;
+        }
+        wide = wide_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out), 0, B->ncta_chunk,
+                                       nullptr);
+        wide.pair_bound = B->plan.at<int4>(30);
+        wide.window = p.window;
+        wide.sinks = p.sinks;
+        wide.sscale = io16 ? p.qscale : 1.f;
+        wide.io16 = io16 ? 1 : 0;
+        wide.ml = p.ml;
+        pk::WideAppend a{};
+        if (fused) {
+            a.pool_k = reinterpret_cast<__nv_bfloat16*>(P->k_layer(layer));
+            a.pool_v = reinterpret_cast<__nv_bfloat16*>(P->v_layer(layer));
+            a.k = static_cast<const float*>(k_new);
+            a.v = static_cast<const float*>(v_new);
+            a.row_seq = p.row_seq;
+            a.offsets = p.offsets;
+            a.starts = p.starts;
+            a.indptr = p.indptr;
+            a.ids = p.ids;
+            a.rows = B->plan.at<int32_t>(10);
+            a.slots = B->plan.at<int64_t>(25);
+            a.n = static_cast<int64_t>(B->w_rows.size());
+            a.rowlen = P->kvh * P->d;
+            a.bs = P->block_size;
+        }
+        PK_CUDA(prof_begin(B, ws));
+        PK_CUDA(pk::launch_wide_prep(wide, B->nwide, static_cast<uint8_t*>(B->qpk.ptr), a, ws));
+        PK_CUDA(prof_end(B, kProfAppend, ws));
+        PK_CUDA(prof_begin(B, ws));
+        PK_CUDA(pk::launch_wide_attention(&P->tmk1, &P->tmv1, wide, ws));
+        PK_CUDA(prof_end(B, kProfWide, ws));
+        B->launches += 2;
+    }
     if (B->use_tc) {
         pk::TcParams t = tc_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out));
         t.u_bound = B->plan.at<int4>(28);
@@ -1379,6 +1505,10 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         PK_CUDA(pk::launch_bounded_rows(P->dtype, io16, p, st));
         PK_CUDA(prof_end(B, kProfGeneric, st));
         B->launches++;
+    }
+    if (fork) {
+        PK_CUDA(cudaEventRecord(B->ev_join, B->side));
+        PK_CUDA(cudaStreamWaitEvent(st, B->ev_join, 0));
     }
     if (B->weights_mode != 0) {
         pk::WeightParams w{};
@@ -1410,7 +1540,16 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         }
         w.t_seq += B->ntouch_tc;
         w.t_blk += B->ntouch_tc;
-        w.ntouched = static_cast<int>(B->t_seq.size()) - B->ntouch_tc;
+        w.ntouched = B->ntouch_wide;
+        if (w.ntouched > 0) {
+            PK_CUDA(pk::launch_wide_weights(&P->tmk1, wide, B->plan.at<int4>(31), static_cast<int>(B->pieces.size() / 4),
+                                            static_cast<float*>(B->wpieces.ptr), w, p.starts, p.offsets,
+                                            B->plan.at<int2>(32), st));
+            B->launches += 2;
+        }
+        w.t_seq += B->ntouch_wide;
+        w.t_blk += B->ntouch_wide;
+        w.ntouched = static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide;
         if (w.ntouched > 0) {
             PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
             B->launches++;
@@ -1822,6 +1961,7 @@ int pk_batch_destroy(pk_batch* B) {
     B->qpk.release();
     B->ml.release();
     B->score.release();
+    B->wpieces.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);
