@@ -195,6 +195,21 @@ void* mapped_host_range(const void* p, size_t bytes) {
 
 }  // namespace
 
+// What a call of pk_pool_evict uploads, after its checks.
+struct EvictPlan {
+    std::vector<int32_t> indptr, ids, new_indptr, new_ids, lengths, items;
+    int max_len = 0;
+    // Per block, the call's first reader (several: seq = -2) and whether it is written; valid where
+    // `call` is this call's number.
+    struct Use {
+        uint32_t call;
+        int32_t seq, idx;
+        bool written;
+    };
+    std::vector<Use> use;
+    uint32_t call = 0;
+};
+
 struct pk_pool {
     int device = 0;
     int n_layers = 0;
@@ -227,6 +242,7 @@ struct pk_pool {
     float* weights = nullptr;
     // evict: its tables and items, the kept positions when the caller wants none, and the end
     // of the last call (the next one may come on another stream)
+    EvictPlan evict_plan;
     Uploader evict_up;
     DevBuf evict_kept;
     cudaEvent_t evict_done = nullptr;
@@ -1565,12 +1581,6 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     return PK_OK;
 }
 
-// What a call of pk_pool_evict uploads, after its checks.
-struct EvictPlan {
-    std::vector<int32_t> indptr{0}, ids, new_indptr{0}, new_ids, lengths, items;
-    int max_len = 0;
-};
-
 // Checks and lays out an eviction (host only). A destination must not be a block that the call
 // reads, except the same block of the same sequence at the same table index when nothing else
 // reads it: then new positions never pass old ones, and moving in order is safe.
@@ -1585,11 +1595,19 @@ int plan_evict(int64_t num_blocks, int bs, int nseq, const int64_t* table_indptr
     if (nseq == 0) return PK_OK;
     if (!table_indptr || !lengths || !new_indptr) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
     if (table_indptr[0] != 0 || new_indptr[0] != 0) return fail(PK_ERR_INVALID_ARG, "a table's indptr[0] != 0");
-    // every block the call reads or writes: (block, kind, sequence, index), kind 0 read, 1 written
-    struct Use {
-        int32_t block, kind, seq, idx;
-    };
-    std::vector<Use> uses;
+    out->indptr.assign(1, 0);
+    out->new_indptr.assign(1, 0);
+    out->ids.clear();
+    out->new_ids.clear();
+    out->lengths.clear();
+    out->items.clear();
+    out->max_len = 0;
+    if (out->use.size() != static_cast<size_t>(num_blocks) || out->call == UINT32_MAX) {
+        out->use.assign(static_cast<size_t>(num_blocks), EvictPlan::Use{0, 0, 0, false});
+        out->call = 0;
+    }
+    const uint32_t call = ++out->call;
+    EvictPlan::Use* use = out->use.data();
     auto ids_ok = [&](const int32_t* t, int64_t n, int i, const char* what) {
         for (int64_t j = 0; j < n; ++j)
             if (t[j] < 0 || t[j] >= num_blocks)
@@ -1620,27 +1638,29 @@ int plan_evict(int64_t num_blocks, int bs, int nseq, const int64_t* table_indptr
         out->new_indptr.push_back(static_cast<int32_t>(out->new_ids.size()));
         out->lengths.push_back(static_cast<int32_t>(n));
         out->max_len = std::max(out->max_len, static_cast<int>(n));
-        for (int64_t j = 0; j < need; ++j) uses.push_back({t[j], 0, i, static_cast<int32_t>(j)});
-        for (int64_t j = 0; j < nneed; ++j) uses.push_back({nt[j], 1, i, static_cast<int32_t>(j)});
+        for (int64_t j = 0; j < need; ++j) {
+            EvictPlan::Use& u = use[t[j]];
+            if (u.call != call) u = EvictPlan::Use{call, i, static_cast<int32_t>(j), false};
+            else u.seq = -2;
+        }
     }
-    std::sort(uses.begin(), uses.end(), [](const Use& a, const Use& b) {
-        return a.block != b.block ? a.block < b.block : a.kind > b.kind;
-    });
     std::vector<uint8_t> in_place(nseq, 0);
-    for (size_t x = 0; x < uses.size();) {
-        const Use& w = uses[x++];
-        if (w.kind == 1) {  // a written block comes before its reads
-            for (; x < uses.size() && uses[x].block == w.block; ++x) {
-                if (uses[x].kind == 1)
-                    return fail(PK_ERR_INVALID_ARG, "block %d appears twice in the new tables", w.block);
-                if (uses[x].seq != w.seq || uses[x].idx != w.idx)
-                    return fail(PK_ERR_INVALID_ARG,
-                                "seq %d: new block %d is read by this call; a new table may name an old block only at its "
-                                "own index and when no other sequence reads it", w.seq, w.block);
-                in_place[w.seq] = 1;
+    for (int i = 0; i < nseq; ++i) {
+        const int nblk = out->new_indptr[i + 1] - out->new_indptr[i];
+        for (int j = 0; j < nblk; ++j) {
+            const int32_t b = out->new_ids[out->new_indptr[i] + j];
+            EvictPlan::Use& u = use[b];
+            if (u.call != call) {
+                u = EvictPlan::Use{call, -1, 0, true};
+                continue;
             }
-        } else {
-            while (x < uses.size() && uses[x].block == w.block) ++x;
+            if (u.written) return fail(PK_ERR_INVALID_ARG, "block %d appears twice in the new tables", b);
+            if (u.seq != i || u.idx != j)
+                return fail(PK_ERR_INVALID_ARG,
+                            "seq %d: new block %d is read by this call; a new table may name an old block only at its own "
+                            "index and when no other sequence reads it", i, b);
+            u.written = true;
+            in_place[i] = 1;
         }
     }
     // New positions move in pieces of kRows by different blocks of the grid; in place they have
@@ -1852,7 +1872,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     if (!P) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
     if (!P->weights) return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
     const int bs = P->block_size;
-    EvictPlan plan;
+    EvictPlan& plan = P->evict_plan;
     int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
                         &plan);
     if (rc != PK_OK || nseq == 0) return rc;

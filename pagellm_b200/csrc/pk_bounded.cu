@@ -267,16 +267,23 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 256;
+// Division by a size that is usually a power of two: shift >= 0 is its logarithm.
+__device__ __forceinline__ int div_by(int x, int d, int shift) { return shift >= 0 ? x >> shift : x / d; }
 
-// Which tokens of (layer, sequence, KV head) stay: one CTA each. The threshold weight - the
-// T-th largest of the middle [sinks, n - recent) - is found digit by digit from the top (radix
-// select, 8 bits per pass over the keys); then one ordered pass writes the kept positions
-// (larger than the threshold, or equal to it while ties remain to be taken, lowest first).
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
-    extern __shared__ float vals[];  // the sequence's weights, when they fit
-    __shared__ int hist[256];
-    __shared__ int warp_gt[kSelThreads / 32], warp_eq[kSelThreads / 32];
+constexpr int kSelBins = 2048;  // 11-bit digits: sign, exponent and 2 bits first, so heavy tails spread
+
+// Which tokens of (layer, sequence, KV head) stay: one CTA each, its weights in shared memory when
+// they fit. The threshold weight - the T-th largest of the middle [sinks, n - recent) - is found
+// digit by digit from the top (radix select in three passes); then one ordered pass writes the
+// kept positions (larger than the threshold, or equal to it while ties remain to be taken, lowest
+// first) and their weights. Latency bound - n loads, then barriers and passes over shared memory -
+// so everything goes four positions at a time, and few long sequences get 1024 threads each.
+template <int NT>
+__global__ void __launch_bounds__(NT) evict_select_kernel(const EvictParams p) {
+    extern __shared__ float4 vals4[];  // the sequence's weights, when they fit
+    constexpr int NW = NT / 32, PER = kSelBins / NT;
+    __shared__ int hist[kSelBins];
+    __shared__ int warp_a[32], warp_b[32];
     __shared__ int sh_digit, sh_rank;
     const int i = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -287,13 +294,27 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     float* wl = p.weights + static_cast<size_t>(layer) * p.num_blocks * p.kvh * p.bs;
     int32_t* kept = p.kept + ((static_cast<size_t>(layer) * p.nseq + i) * p.kvh + h) * p.budget;
     const bool cached = n <= p.cache_cap;
-    auto at = [&](int j) {
-        return wl + (static_cast<size_t>(tbl[j / p.bs]) * p.kvh + h) * p.bs + j % p.bs;
+    auto at = [&](const int32_t* t, int j) {
+        const int b = div_by(j, p.bs, p.bs_shift);
+        return wl + (static_cast<size_t>(t[b]) * p.kvh + h) * p.bs + (j - b * p.bs);
     };
-    if (cached)
-        for (int j = tid; j < n; j += kSelThreads) vals[j] = *at(j);
+    // weights of positions j .. j + 3 (j a multiple of 4; what lies behind the last token is unused)
+    auto fetch4 = [&](int j) {
+        if ((p.bs & 3) == 0) return *reinterpret_cast<const float4*>(at(tbl, j));
+        float4 x = make_float4(*at(tbl, j), 0.f, 0.f, 0.f);
+        if (j + 1 < n) x.y = *at(tbl, j + 1);
+        if (j + 2 < n) x.z = *at(tbl, j + 2);
+        if (j + 3 < n) x.w = *at(tbl, j + 3);
+        return x;
+    };
+    if (cached) {
+#pragma unroll 4
+        for (int j = 4 * tid; j < n; j += 4 * NT) vals4[j >> 2] = fetch4(j);
+    }
+#pragma unroll
+    for (int b = 0; b < PER; ++b) hist[b * NT + tid] = 0;
     __syncthreads();
-    auto value = [&](int j) { return cached ? vals[j] : *at(j); };
+    auto value4 = [&](int j) { return cached ? vals4[j >> 2] : fetch4(j); };
 
     const int lo = p.sinks, hi = n - p.recent;  // the middle (used only when n > budget)
     uint32_t thr = 0;
@@ -302,116 +323,175 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
         int rank = p.budget - p.sinks - p.recent;  // still to find among keys with the prefix
         if (rank > 0) {
             uint32_t mask = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int b = tid; b < 256; b += kSelThreads) hist[b] = 0;
-                __syncthreads();
-                for (int j = lo + tid; j < hi; j += kSelThreads) {
-                    const uint32_t k = weight_key(value(j));
-                    if ((k & mask) == thr) atomicAdd(&hist[(k >> shift) & 255], 1);
+            // digits of 11, 11 and 10 bits
+            for (int pass = 0; pass < 3; ++pass) {
+                const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+                const int bins = pass == 2 ? 1024 : kSelBins;
+#pragma unroll 2
+                for (int j = (lo & ~3) + 4 * tid; j < hi; j += 4 * NT) {
+                    const float4 x = value4(j);
+                    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t k = weight_key(v[r]);
+                        if (j + r >= lo && j + r < hi && (k & mask) == thr) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+                    }
                 }
                 __syncthreads();
-                if (tid == 0) {
-                    int left = rank, b = 255;
-                    while (hist[b] < left) left -= hist[b--];  // rank <= keys counted: ends at b >= 0
-                    sh_digit = b;
-                    sh_rank = left;
+                // suffix sums from the largest bin: thread t owns bins kSelBins - 1 - (t * PER ..)
+                int cnt[PER], own = 0;
+#pragma unroll
+                for (int b = 0; b < PER; ++b) {
+                    cnt[b] = hist[kSelBins - 1 - (tid * PER + b)];
+                    own += cnt[b];
                 }
+                int scan = own;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, scan, o);
+                    if (lane >= o) scan += y;
+                }
+                if (lane == 31) warp_a[warp] = scan;
+                __syncthreads();
+                int front = lane < warp ? warp_a[lane] : 0;  // NW <= 32
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) front += __shfl_xor_sync(0xffffffffu, front, o);
+                int above = front + scan - own;  // keys in larger bins than this thread's
+                if (above < rank && rank <= above + own) {  // one thread
+#pragma unroll
+                    for (int b = 0; b < PER; ++b) {
+                        if (above < rank && rank <= above + cnt[b]) {
+                            sh_digit = kSelBins - 1 - (tid * PER + b);
+                            sh_rank = rank - above;
+                        }
+                        above += cnt[b];
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < PER; ++b) hist[kSelBins - 1 - (tid * PER + b)] = 0;
                 __syncthreads();
                 thr |= static_cast<uint32_t>(sh_digit) << shift;
-                mask |= 255u << shift;
+                mask |= static_cast<uint32_t>(bins - 1) << shift;
                 rank = sh_rank;
-                __syncthreads();
             }
             ties = rank;
         } else {
             thr = 0xFFFFFFFFu;  // nothing of the middle is kept: no key is larger, no tie is taken
         }
     }
-    // ordered pass: kept positions before this tile, ties before this tile
-    int base = 0, eq_base = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelThreads) {
-        const int j = j0 + tid;
-        bool gt = false, eq = false;
-        if (j < n) {
-            if (n <= p.budget || j < lo || j >= hi) {
-                gt = true;
-            } else {
-                const uint32_t k = weight_key(value(j));
-                gt = k > thr;
-                eq = k == thr;
+    // Ordered pass: a thread judges 4 consecutive positions of a tile; kept positions and ties are
+    // counted by a scan over the threads.
+    int base = 0, eq_base = 0;  // larger ones and ties in earlier tiles
+    for (int j0 = 0; j0 < n; j0 += 4 * NT) {
+        unsigned gt = 0, eq = 0;
+        const int jb = j0 + 4 * tid;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (jb < n) {
+            const float4 x = value4(jb);
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = jb + r;
+                if (j >= n) continue;
+                if (n <= p.budget || j < lo || j >= hi) {
+                    gt |= 1u << r;
+                } else {
+                    const uint32_t k = weight_key(v[r]);
+                    gt |= (k > thr ? 1u : 0u) << r;
+                    eq |= (k == thr ? 1u : 0u) << r;
+                }
             }
         }
-        const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) {
-            warp_gt[warp] = __popc(bg);
-            warp_eq[warp] = __popc(be);
+        // both counts in one scan: a tile has at most 4096 of each
+        const int own = __popc(gt) | __popc(eq) << 16;
+        int scan = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += y;
         }
+        if (lane == 31) warp_b[warp] = scan;
         __syncthreads();
-        int g0 = base, e0 = eq_base, gall = 0, eall = 0;
-        for (int w = 0; w < kSelThreads / 32; ++w) {
-            if (w < warp) {
-                g0 += warp_gt[w];
-                e0 += warp_eq[w];
+        const int mine = lane < NW ? warp_b[lane] : 0;
+        int front = lane < warp ? mine : 0, all = mine;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            front += __shfl_xor_sync(0xffffffffu, front, o);
+            all += __shfl_xor_sync(0xffffffffu, all, o);
+        }
+        front += scan - own;
+        int g0 = base + (front & 0xFFFF), e0 = eq_base + (front >> 16);
+        base += all & 0xFFFF;
+        eq_base += all >> 16;
+        // uncached: every source of this tile has been read (the barrier above) before a weight
+        // moves; destinations never pass their sources, so later tiles' sources stay whole
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool g = gt >> r & 1, q = eq >> r & 1;
+            if (g || (q && e0 < ties)) {
+                const int y = g0 + min(e0, ties);  // larger ones before it, and the ties taken so far
+                kept[y] = jb + r;
+                *at(ntbl, y) = v[r];
             }
-            gall += warp_gt[w];
-            eall += warp_eq[w];
+            g0 += g;
+            e0 += q;
         }
-        const unsigned below = (1u << lane) - 1;
-        const int eq_before = e0 + __popc(be & below);  // ties at lower positions
-        // kept before j: larger ones (counted in g0) and the ties taken so far
-        const int y = g0 + __popc(bg & below) + min(eq_before, ties);
-        if (gt || (eq && eq_before < ties)) kept[y] = j;
-        base += gall;
-        eq_base += eall;
         __syncthreads();
     }
-    for (int y = m + tid; y < p.budget; y += kSelThreads) kept[y] = -1;
-    __syncthreads();
-    // The weights move with their tokens. New position y <= old position, so a tile's values are
-    // read before any of them is overwritten, and later tiles' sources lie behind this one's
-    // destinations (new_tables may name the old blocks, position by position).
-    for (int y0 = 0; y0 < m; y0 += kSelThreads) {
-        const int y = y0 + tid;
-        float x = 0.f;
-        if (y < m) x = value(kept[y]);
-        __syncthreads();
-        if (y < m) wl[(static_cast<size_t>(ntbl[y / p.bs]) * p.kvh + h) * p.bs + y % p.bs] = x;
-    }
+    for (int y = m + tid; y < p.budget; y += NT) kept[y] = -1;
 }
 
 // Kept K (blockIdx.z even) or V rows into the new blocks: one CTA per work item (rows
-// [y0, y1) of a sequence's new positions), (layer, KV head), tensor. Within an item rows move
-// in tiles, all of a tile read before any is written; a sequence whose new table names some of
-// its old blocks is one item, so that its tiles run in order (see evict_select_kernel).
+// [y0, y1) of a sequence's new positions), (layer, KV head), tensor. Rows move in tiles of up to
+// kMoveWords words: the tile's row addresses first (one chain of loads, kept position -> block ->
+// slot, per row and not per word), then every word of it is read before any is written. A sequence
+// whose new table names some of its old blocks is one item, so that its tiles run in order (see
+// evict_select_kernel). HBM bound: every kept row is read and written once.
+constexpr int kMoveThreads = 256, kMovePer = 8, kMoveWords = kMoveThreads * kMovePer;
 template <typename W>
-__global__ void __launch_bounds__(256) evict_move_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+    __shared__ int64_t src[kMoveThreads], dst[kMoveThreads];  // first word of each row of the tile
     const int item = blockIdx.x;
     const int i = p.items[3 * item], y0 = p.items[3 * item + 1], y1 = p.items[3 * item + 2];
     const int h = blockIdx.y % p.kvh, layer = blockIdx.y / p.kvh;
-    uint8_t* base = static_cast<uint8_t*>(blockIdx.z == 0 ? p.pool_k : p.pool_v) +
-                    static_cast<size_t>(layer) * p.num_blocks * p.bs * p.kvh * p.row_bytes;
+    const int words = p.row_words;
+    W* base = static_cast<W*>(blockIdx.z == 0 ? p.pool_k : p.pool_v) +
+              (static_cast<size_t>(layer) * p.num_blocks * p.bs * p.kvh + h) * words;
     const int32_t* tbl = p.ids + p.indptr[i];
     const int32_t* ntbl = p.new_ids + p.new_indptr[i];
     const int32_t* kept = p.kept + ((static_cast<size_t>(layer) * p.nseq + i) * p.kvh + h) * p.budget;
-    const int words = p.row_bytes / static_cast<int>(sizeof(W));
-    const int64_t total = static_cast<int64_t>(y1 - y0) * words;
-    constexpr int kPer = 4;
-    auto row_at = [&](const int32_t* t, int j) {
-        return reinterpret_cast<W*>(base + ((static_cast<size_t>(t[j / p.bs]) * p.bs + j % p.bs) * p.kvh + h) * p.row_bytes);
+    const int64_t stride = static_cast<int64_t>(p.kvh) * words;  // words from one slot to the next
+    const int rows = min(kMoveThreads, kMoveWords / words);
+    auto word_of = [&](const int32_t* t, int j) {
+        const int b = div_by(j, p.bs, p.bs_shift);
+        return (static_cast<int64_t>(t[b]) * p.bs + (j - b * p.bs)) * stride;
     };
-    for (int64_t x0 = 0; x0 < total; x0 += 256 * kPer) {
-        W val[kPer];
+    for (int y = y0; y < y1; y += rows) {
+        const int nr = min(rows, y1 - y), total = nr * words;
+        if (threadIdx.x < nr) {
+            src[threadIdx.x] = word_of(tbl, kept[y + threadIdx.x]);
+            dst[threadIdx.x] = word_of(ntbl, y + threadIdx.x);
+        }
+        __syncthreads();
+        W val[kMovePer];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const int64_t x = x0 + e * 256 + threadIdx.x;
-            if (x < total) val[e] = row_at(tbl, kept[y0 + x / words])[x % words];
+        for (int e = 0; e < kMovePer; ++e) {
+            const int x = e * kMoveThreads + threadIdx.x;
+            if (x < total) {
+                const int r = div_by(x, words, p.words_shift);
+                val[e] = base[src[r] + (x - r * words)];
+            }
         }
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            const int64_t x = x0 + e * 256 + threadIdx.x;
-            if (x < total) row_at(ntbl, y0 + static_cast<int>(x / words))[x % words] = val[e];
+        for (int e = 0; e < kMovePer; ++e) {
+            const int x = e * kMoveThreads + threadIdx.x;
+            if (x < total) {
+                const int r = div_by(x, words, p.words_shift);
+                base[dst[r] + (x - r * words)] = val[e];
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -469,20 +549,34 @@ cudaError_t launch_copy_weights(float* weights, const int64_t* pairs, int64_t np
 cudaError_t launch_evict(const EvictParams& p, int max_len, cudaStream_t st) {
     if (p.nseq <= 0) return cudaSuccess;
     EvictParams q = p;
+    const auto log2_of = [](int x) {
+        int s = 0;
+        while ((1 << s) < x) ++s;
+        return (1 << s) == x ? s : -1;
+    };
     // the weights of a sequence are kept in shared memory while they fit
     constexpr int kMaxCached = 40960;  // floats: 160 KB
     q.cache_cap = std::min(max_len, kMaxCached);
-    const size_t smem = static_cast<size_t>(q.cache_cap) * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    q.bs_shift = log2_of(p.bs);
+    const size_t smem = (static_cast<size_t>(q.cache_cap) * sizeof(float) + 15) & ~size_t(15);
+    // 1024 threads a CTA where one CTA per SM is all there is to run, or fits beside its weights
+    const int64_t ctas = static_cast<int64_t>(p.nseq) * p.kvh * p.layers;
+    const bool wide = max_len > 2048 && (ctas <= 2 * 148 || max_len > 16384);
+    auto sel = wide ? evict_select_kernel<1024> : evict_select_kernel<256>;
+    cudaError_t e = cudaFuncSetAttribute(sel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kMaxCached * static_cast<int>(sizeof(float)));
     if (e != cudaSuccess) return e;
-    evict_select_kernel<<<dim3(p.nseq, p.kvh, p.layers), kSelThreads, smem, st>>>(q);
+    sel<<<dim3(p.nseq, p.kvh, p.layers), wide ? 1024 : 256, smem, st>>>(q);
     e = cudaGetLastError();
     if (e != cudaSuccess || p.nitems <= 0) return e;
     const dim3 grid(p.nitems, p.kvh * p.layers, 2);
-    if (p.row_bytes % 16 == 0) evict_move_kernel<uint4><<<grid, 256, 0, st>>>(q);
-    else if (p.row_bytes % 4 == 0) evict_move_kernel<uint32_t><<<grid, 256, 0, st>>>(q);
-    else evict_move_kernel<uint16_t><<<grid, 256, 0, st>>>(q);
+    // the widest word that divides a row
+    const int w = p.row_bytes % 16 == 0 ? 16 : p.row_bytes % 4 == 0 ? 4 : 2;
+    q.row_words = p.row_bytes / w;
+    q.words_shift = log2_of(q.row_words);
+    if (w == 16) evict_move_kernel<uint4><<<grid, kMoveThreads, 0, st>>>(q);
+    else if (w == 4) evict_move_kernel<uint32_t><<<grid, kMoveThreads, 0, st>>>(q);
+    else evict_move_kernel<uint16_t><<<grid, kMoveThreads, 0, st>>>(q);
     return cudaGetLastError();
 }
 

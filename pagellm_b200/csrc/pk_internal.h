@@ -266,7 +266,12 @@ struct EvictParams {
     int budget;
     int sinks;
     int recent;
-    int cache_cap;  // sequences up to this length keep their weights in shared memory
+    // set by launch_evict: sequences up to this length keep their weights in shared memory; words of
+    // a row; logarithms of bs and row_words (-1: no power of two)
+    int cache_cap;
+    int row_words;
+    int bs_shift;
+    int words_shift;
 };
 
 // Read-only view of a pool's fields for entry points outside pk_api.cu.
