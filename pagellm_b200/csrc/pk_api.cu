@@ -297,7 +297,7 @@ struct pk_batch {
     std::vector<int32_t> w_pair;   // item pairs: chunk pairs, then prefix pairs
     int npair_chunk = 0, npair_prefix = 0;
     // wide-kernel schedule: per CTA a range of segments (pair, head, key tiles, slot, ph)
-    std::vector<int32_t> pair_bound;  // bounded pairs: tiles in front of the jump, the jump, first key of the window
+    std::vector<int32_t> pair_bound;  // bounded pairs: tiles in front of the jump, the jump, first key of the window, tiles
     std::vector<int32_t> pair_kend, cta_seg, seg, ph_info, split;
     int ncta_chunk = 0, ncta_prefix = 0, nslots = 0, nph = 0, nwsplit = 0;
     int nwsplit_chunk = 0;  // the first nwsplit_chunk entries of split belong to chunk pairs
@@ -333,6 +333,7 @@ struct pk_batch {
     std::vector<int32_t> pieces;        // chunks' weights: sequence, key tile, first and end query item
     std::vector<int32_t> t_piece;       // per touched block of a chunk: first piece of its tile, pieces
     DevBuf wpieces;                     // [pieces][kvh][128] sums
+    DevBuf ml_items;                    // [chunk items][kvh][128] softmax statistics
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
     std::vector<uint8_t> seq_tc;        // scratch: sequence is on the split-KV kernel
@@ -402,6 +403,22 @@ bool encode_chunk_maps(pk_pool* P, std::string* why) {
         }
     }
     return true;
+}
+
+// bf16 query rows [nrows][H][128] as [64-dim chunk][row][head][64 dims]: one box per (128 / g
+// rows, g heads of a KV head, chunk), the rows of a query tile in order.
+int encode_query_map(const pk_pool* P, const void* q, int64_t nrows, int H, CUtensorMap* out) {
+    auto enc = tensor_map_encoder();
+    if (!enc) return fail(PK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const int g = H / P->kvh;
+    const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(H), static_cast<cuuint64_t>(nrows), 2};
+    const cuuint64_t strides[3] = {256, static_cast<cuuint64_t>(H) * 256, 128};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(g), static_cast<cuuint32_t>(128 / g), 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(q), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? PK_OK : fail(PK_ERR_CUDA, "cuTensorMapEncodeTiled(queries) returned %d", (int)r);
 }
 
 bool encode_pool_maps(pk_pool* P, int layout, std::string* why) {
@@ -706,7 +723,7 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
         const VisibleBlocks vb = visible_blocks(q0, B->pair_kend[x], B->window, B->sinks, pk::kWideKeys);
         pair_tiles[x] = vb.count;
         const int64_t lo = B->window > 0 ? std::max<int64_t>(0, q0 - B->window + 1) : 0;
-        B->pair_bound.insert(B->pair_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(lo), 0});
+        B->pair_bound.insert(B->pair_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(lo), static_cast<int32_t>(vb.count)});
     }
     auto tiles = [&](int x) { return pair_tiles[x]; };
     // Schedules the pair-heads of pairs [x0, x1) over at most G CTAs; returns the CTAs used.
@@ -797,9 +814,11 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
 }
 
 // Pieces of the chunks' weights: for every key tile that holds a touched block, the query items
-// that see a key of it, cut so that all pieces together (x KV heads) fill two CTAs per SM evenly. A
-// piece has at least kMinPieceItems items: it loads the key tile and fills its pipeline first.
+// that see a key of it, cut so that all pieces together (x KV heads) give each of two CTAs per SM
+// kPiecesPerSlot of them. A piece has at least kMinPieceItems items: it loads the key tile and
+// fills its pipeline first.
 constexpr int64_t kMinPieceItems = 4;
+constexpr int64_t kPiecesPerSlot = 4;
 void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::vector<int32_t>& tb) {
     pk_pool* P = B->pool;
     struct Tile {
@@ -829,7 +848,8 @@ void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::
         }
         of[x] = static_cast<int>(tiles.size()) - 1;
     }
-    const int64_t per = std::max<int64_t>(kMinPieceItems, (total * P->kvh + 2 * P->num_sms - 1) / (2 * P->num_sms));
+    const int64_t slots = 2 * kPiecesPerSlot * static_cast<int64_t>(P->num_sms);
+    const int64_t per = std::max<int64_t>(kMinPieceItems, (total * P->kvh + slots - 1) / slots);
     std::vector<int32_t> p0(tiles.size()), np(tiles.size());
     for (size_t x = 0; x < tiles.size(); ++x) {
         const Tile& t = tiles[x];
@@ -961,6 +981,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
             B->t_seq.insert(B->t_seq.end(), ts[k].begin(), ts[k].end());
             B->t_blk.insert(B->t_blk.end(), tb[k].begin(), tb[k].end());
         }
+        PK_CUDA(B->ml_items.reserve(static_cast<size_t>(B->nwide) * P->kvh * 128 * sizeof(float2)));
         PK_CUDA(B->wpieces.reserve(B->pieces.size() / 4 * P->kvh * pk::kWideKeys * sizeof(float)));
     }
     // Wide CTAs take two items each: neighbouring items of one sequence (chunk) or of one
@@ -1456,6 +1477,11 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     // chunk items, on the side stream when split-KV work runs beside them
     const bool fork = B->nwide > 0 && B->use_tc;
     pk::WideParams wide{};
+    CUtensorMap tmq{};
+    if (B->nwide > 0 && io16) {
+        int rc = encode_query_map(P, q, B->nrows, H, &tmq);
+        if (rc != PK_OK) return rc;
+    }
     if (B->nwide > 0) {
         cudaStream_t ws = st;
         if (fork) {
@@ -1466,16 +1492,25 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             PK_CUDA(cudaStreamWaitEvent(B->side, B->ev_fork, 0));
             ws = B->side;
         }
-        wide = wide_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out), 0, B->ncta_chunk,
-                                       nullptr);
+        wide = wide_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out), 0, 0, nullptr);
         wide.pair_bound = B->plan.at<int4>(30);
         wide.window = p.window;
         wide.sinks = p.sinks;
         wide.sscale = io16 ? p.qscale : 1.f;
         wide.io16 = io16 ? 1 : 0;
-        wide.ml = p.ml;
-        pk::WideAppend a{};
-        if (fused) {
+        wide.ml = B->weights_mode != 0 ? static_cast<float2*>(B->ml_items.ptr) : nullptr;
+        const int32_t* wrows = B->plan.at<int32_t>(10);
+        const int64_t nw = fused ? static_cast<int64_t>(B->w_rows.size()) : 0;  // chunk rows still to append
+        if (io16) {
+            if (nw > 0) {
+                PK_CUDA(prof_begin(B, ws));
+                PK_CUDA(pk::launch_append_rows16(P->k_layer(layer), P->v_layer(layer), k_new, v_new, p.row_seq, p.offsets,
+                                                 p.starts, p.indptr, p.ids, P->block_size, wrows, nw, P->kvh * P->d, ws));
+                PK_CUDA(prof_end(B, kProfAppend, ws));
+                B->launches++;
+            }
+        } else {
+            pk::WideAppend a{};
             a.pool_k = reinterpret_cast<__nv_bfloat16*>(P->k_layer(layer));
             a.pool_v = reinterpret_cast<__nv_bfloat16*>(P->v_layer(layer));
             a.k = static_cast<const float*>(k_new);
@@ -1485,19 +1520,20 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             a.starts = p.starts;
             a.indptr = p.indptr;
             a.ids = p.ids;
-            a.rows = B->plan.at<int32_t>(10);
+            a.rows = wrows;
             a.slots = B->plan.at<int64_t>(25);
-            a.n = static_cast<int64_t>(B->w_rows.size());
+            a.n = nw;
             a.rowlen = P->kvh * P->d;
             a.bs = P->block_size;
+            PK_CUDA(prof_begin(B, ws));
+            PK_CUDA(pk::launch_wide_prep(wide, B->nwide, static_cast<uint8_t*>(B->qpk.ptr), a, ws));
+            PK_CUDA(prof_end(B, kProfAppend, ws));
+            B->launches++;
         }
         PK_CUDA(prof_begin(B, ws));
-        PK_CUDA(pk::launch_wide_prep(wide, B->nwide, static_cast<uint8_t*>(B->qpk.ptr), a, ws));
-        PK_CUDA(prof_end(B, kProfAppend, ws));
-        PK_CUDA(prof_begin(B, ws));
-        PK_CUDA(pk::launch_wide_attention(&P->tmk1, &P->tmv1, wide, ws));
+        PK_CUDA(pk::launch_chunk_attention(&P->tmk1, &P->tmv1, &tmq, wide, B->npair_chunk, ws));
         PK_CUDA(prof_end(B, kProfWide, ws));
-        B->launches += 2;
+        B->launches++;
     }
     if (B->use_tc) {
         pk::TcParams t = tc_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out));
@@ -1558,7 +1594,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.t_blk += B->ntouch_tc;
         w.ntouched = B->ntouch_wide;
         if (w.ntouched > 0) {
-            PK_CUDA(pk::launch_wide_weights(&P->tmk1, wide, B->plan.at<int4>(31), static_cast<int>(B->pieces.size() / 4),
+            PK_CUDA(pk::launch_chunk_weights(&P->tmk1, &tmq, wide, B->plan.at<int4>(31), static_cast<int>(B->pieces.size() / 4),
                                             static_cast<float*>(B->wpieces.ptr), w, p.starts, p.offsets,
                                             B->plan.at<int2>(32), st));
             B->launches += 2;
@@ -1982,6 +2018,7 @@ int pk_batch_destroy(pk_batch* B) {
     B->ml.release();
     B->score.release();
     B->wpieces.release();
+    B->ml_items.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);

@@ -41,6 +41,7 @@
 
 #include "pk_device.cuh"
 #include "pk_internal.h"
+#include "pk_tcgen05.cuh"
 
 namespace pk {
 
@@ -68,119 +69,8 @@ constexpr int kOffV = kOffK + kKStages * kKVBytes;
 constexpr int kOffBar = kOffV + kVStages * kKVBytes;
 constexpr int kSmemBytes = kOffBar + 256 + 1024;
 
-// ---------------------------------------------------------------- tcgen05 wrappers
-__device__ __forceinline__ void tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
-                 "r"(ncols));
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols));
-}
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// A operand from TMEM (rows = lanes, K packed two bf16 per 32-bit column).
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_u32(bar))
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]),
-        "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]),
-        "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]),
-        "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
-        "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-        "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// 2^x on the special-function unit (approximate, flush-to-zero; 2^-inf = 0).
-__device__ __forceinline__ float ex2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle (sm_100 format: version 1).
-// lbo / sbo in bytes (multiples of 16).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFF);
-    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
-    d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
-    d |= static_cast<uint64_t>(1) << 46;  // version
-    d |= static_cast<uint64_t>(2) << 61;  // SWIZZLE_128B
-    return d;
-}
-
-// Instruction descriptor, kind::f16: bf16 x bf16 -> fp32, M = 128.
-__host__ __device__ constexpr uint32_t idesc_bf16(int n, bool b_mn_major) {
-    return (1u << 4)                  // D format f32
-           | (1u << 7)                // A bf16
-           | (1u << 10)               // B bf16
-           | (0u << 15)               // A K-major
-           | ((b_mn_major ? 1u : 0u) << 16)
-           | (static_cast<uint32_t>(n >> 3) << 17)
-           | (static_cast<uint32_t>(kWRows >> 4) << 24);
-}
-
 constexpr uint32_t kIdescS = idesc_bf16(kWKeys, false);
 constexpr uint32_t kIdescO = idesc_bf16(kWD, true);
-
-// Offset of 16-byte unit u of row r in a [rows][128 B] tile with the 128-byte swizzle.
-__device__ __forceinline__ uint32_t sw128(int r, int u) {
-    return static_cast<uint32_t>(r * 128 + ((u ^ (r & 7)) << 4));
-}
 
 // Per-CTA segment list: a segment is key tiles [t0, t1) of one (item pair, KV head).
 struct Seg {
@@ -191,21 +81,6 @@ __device__ __forceinline__ Seg load_seg(const int32_t* s, int i) {
     return Seg{e[0], e[1], e[2], e[3], e[4], e[5]};
 }
 
-// Real key tile of entry jt of a pair's tile list. A bounded pair lists the tiles of the sinks in
-// front of its first row's window, then those from the window on: they jump by `skip` from `head`.
-struct PairBound {
-    int head, skip, lo;  // lo: first key of the pair's first row's window
-};
-template <bool BOUNDED>
-__device__ __forceinline__ PairBound load_pair_bound(const WideParams& p, int pair) {
-    if constexpr (!BOUNDED) return PairBound{0, 0, 0};
-    const int4 b = __ldg(p.pair_bound + pair);
-    return PairBound{b.x, b.y, b.z};
-}
-
-// BOUNDED: windowed chunk items (with sinks), rows in float or bf16 (p.io16; bf16 queries enter the
-// products unscaled and p.sscale is applied to the scores), softmax statistics kept in p.ml.
-template <bool BOUNDED>
 __global__ void __launch_bounds__(kWThreads, 1)
     wide_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const WideParams p) {
@@ -276,10 +151,6 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 const int32_t* tbl = p.ids + p.indptr[p.w_seq[i0]];
                 const int kv_end = p.pair_kend[sg.pair];
                 const int nblk = (kv_end + p.bs - 1) / p.bs;
-                if constexpr (BOUNDED) {
-                    const PairBound pb = load_pair_bound<BOUNDED>(p, sg.pair);
-                    if (jt >= pb.head) jt += pb.skip;
-                }
                 // the tile's block ids first, as independent loads: one load latency per tile
                 int idv[kWKeys / 16];
 #pragma unroll
@@ -459,19 +330,15 @@ __global__ void __launch_bounds__(kWThreads, 1)
             const int tok0 = item >= 0 ? p.w_tok0[item] : 0;
             const int kend_t = item >= 0 ? p.w_kend[item] : 0;
             const int kv_end = p.pair_kend[sg.pair];
-            const PairBound pb = load_pair_bound<BOUNDED>(p, sg.pair);
             const int last_tile = (kv_end + kWKeys - 1) / kWKeys - 1;
             const bool live = t_row < ntok;
             // last visible key: the row's own position, and never past its item's key range
             const int qlim = live ? min(p.tok_pos[tok0 + t_row], kend_t - 1) : -1;
-            // bounded: keys up to qlo and not among the sinks are past the row's window
-            const int qlo = BOUNDED && live ? p.tok_pos[tok0 + t_row] - p.window : -1;
             const int orow = p.tok_row[tok0 + (live ? t_row : 0)];
             const size_t oidx = static_cast<size_t>(orow) * p.H + h * g + jh;
             float m = -INFINITY, l = 0.f;
             for (int jt = sg.t0; jt < sg.t1 && ok; ++jt, ++n) {
-                const int rt = BOUNDED && jt >= pb.head ? jt + pb.skip : jt;
-                const int kbase = rt * kWKeys;
+                const int kbase = jt * kWKeys;
                 const bool got = mbar_wait_bounded(&sfull[tile], static_cast<uint32_t>(n & 1));
                 if (!__all_sync(0xffffffffu, got) || *abort_flag) {
                     ok = false;
@@ -481,7 +348,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 // all 128 scores of the row, one TMEM wait; mask by absolute position only on
                 // tiles that reach past this row's limit (earlier tiles are fully visible; dead
                 // rows mask everything)
-                const bool masked = kbase + kWKeys - 1 > qlim || (BOUNDED && kbase <= qlo && kbase + kWKeys > p.sinks);
+                const bool masked = kbase + kWKeys - 1 > qlim;
                 float sv[kWKeys];
 #pragma unroll
                 for (int c = 0; c < kWKeys / 32; ++c) tmem_ld32(tS + c * 32, sv + c * 32);
@@ -489,7 +356,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < kWKeys; ++i)
-                        if (kbase + i > qlim || (BOUNDED && kbase + i <= qlo && kbase + i >= p.sinks)) sv[i] = -INFINITY;
+                        if (kbase + i > qlim) sv[i] = -INFINITY;
                 }
                 // row max as 8 independent chains
                 float mx8[8];
@@ -499,9 +366,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
 #pragma unroll
                     for (int i = kq + 8; i < kWKeys; i += 8) mx8[kq] = fmaxf(mx8[kq], sv[i]);
                 }
-                float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                 fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-                if constexpr (BOUNDED) mx *= p.sscale;
+                const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
                 // Lazy rescale: keep the exponent base of earlier tiles unless this tile's max
                 // exceeds it by more than 8 (P stays <= 2^8 in bf16, l and O in fp32), so O in
                 // TMEM is rescaled only when the base actually moves.
@@ -517,9 +383,8 @@ __global__ void __launch_bounds__(kWThreads, 1)
                     uint32_t pk[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float s0 = sv[half * 64 + 2 * i], s1 = sv[half * 64 + 2 * i + 1];
-                        const float a = ex2_approx(BOUNDED ? fmaf(s0, p.sscale, -base) : s0 - base);
-                        const float b = ex2_approx(BOUNDED ? fmaf(s1, p.sscale, -base) : s1 - base);
+                        const float a = ex2_approx(sv[half * 64 + 2 * i] - base);
+                        const float b = ex2_approx(sv[half * 64 + 2 * i + 1] - base);
                         sum8[i & 7] += a + b;
                         pk[i] = pack_bf16(a, b);
                     }
@@ -550,12 +415,9 @@ __global__ void __launch_bounds__(kWThreads, 1)
                     }
                     tmem_wait_st();
                 }
-                // keys past the context in the last tile (and, bounded, keys [za, zb) between the
-                // sinks and the pair's window): zero their V rows so P = 0 meets 0 (tile 0's P.V is
-                // issued first, so tile 1's sees the zeros too)
-                const bool tail = rt == last_tile && kv_end < kbase + kWKeys;
-                const int za = BOUNDED ? max(0, p.sinks - kbase) : 0, zb = BOUNDED ? min(kWKeys, pb.lo - kbase) : 0;
-                if (tile == 0 && (tail || (BOUNDED && za < zb))) {
+                if (tile == 0 && jt == last_tile && kv_end < kbase + kWKeys) {
+                    // keys past the context in the last tile: zero their V rows so P = 0 meets 0
+                    // (tile 0's P.V is issued first, so tile 1's sees the zeros too)
                     const int s = n % kVStages;
                     const bool landed = mbar_wait_bounded(&vfull[s], static_cast<uint32_t>(n / kVStages) & 1u);
                     if (!__all_sync(0xffffffffu, landed)) {
@@ -563,15 +425,13 @@ __global__ void __launch_bounds__(kWThreads, 1)
                         break;
                     }
                     uint8_t* vd = smem + kOffV + s * kKVBytes;
-                    auto zero_rows = [&](int first, int end) {
-                        for (int x = threadIdx.x - 64; x < (end - first) * 2 * 8; x += 128) {
-                            const int key = first + x / 16;
-                            const int c = (x / 8) & 1;
-                            *reinterpret_cast<uint4*>(vd + c * (kWKeys * 128) + sw128(key, x & 7)) = make_uint4(0, 0, 0, 0);
-                        }
-                    };
-                    if (tail) zero_rows(kv_end - kbase, kWKeys);
-                    if (BOUNDED && za < zb) zero_rows(za, zb);
+                    const int first = kv_end - kbase;
+                    const int units = (kWKeys - first) * 2 * 8;
+                    for (int x = threadIdx.x - 64; x < units; x += 128) {
+                        const int key = first + x / 16;
+                        const int c = (x / 8) & 1;
+                        *reinterpret_cast<uint4*>(vd + c * (kWKeys * 128) + sw128(key, x & 7)) = make_uint4(0, 0, 0, 0);
+                    }
                     fence_proxy_async_smem();  // the zeroed V rows (generic writes) before the MMA reads them
                 }
                 tc_fence_before();
@@ -600,8 +460,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 // split-KV kernel wrote (normalised, log-sum-exp lse_s):
                 //   (o * 2^(m-M) + out * 2^(lse_s-M)) / (l * 2^(m-M) + 2^(lse_s-M)).
                 float wo = l > 0.f ? 1.f / l : 0.f, wr = 0.f;
-                if (BOUNDED && ok && live && p.ml != nullptr) p.ml[oidx] = make_float2(m, wo);
-                if (!BOUNDED && ok && p.lse != nullptr && live) {
+                if (ok && p.lse != nullptr && live) {
                     const float ls = p.lse[oidx];
                     const float mm = fmaxf(l > 0.f ? m : -INFINITY, ls);
                     const float a = l > 0.f ? exp2f(m - mm) : 0.f;
@@ -620,10 +479,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                 for (int kk = 0; kk < 8; ++kk) {
                     const int src = 4 * kk + sub;
                     const unsigned long long oi = __shfl_sync(0xffffffffu, oidx64, src);
-                    // (bf16 rows are half as long: an offset in units of the row's own type)
-                    orow[kk] = BOUNDED && p.io16
-                                   ? reinterpret_cast<float*>(reinterpret_cast<__nv_bfloat16*>(p.out) + static_cast<size_t>(oi) * kWD + 4 * cq)
-                                   : p.out + static_cast<size_t>(oi) * kWD + 4 * cq;
+                    orow[kk] = p.out + static_cast<size_t>(oi) * kWD + 4 * cq;
                     wrr[kk] = __shfl_sync(0xffffffffu, wr, src);
                     liv[kk] = __shfl_sync(0xffffffffu, live ? 1 : 0, src) != 0;
                 }
@@ -637,7 +493,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
                         *stg4(lane, i) = make_float4(o[4 * i] * wo, o[4 * i + 1] * wo, o[4 * i + 2] * wo, o[4 * i + 3] * wo);
                     __syncwarp();
                     float4 y[8];
-                    if (!BOUNDED && p.lse != nullptr) {
+                    if (p.lse != nullptr) {
 #pragma unroll
                         for (int kk = 0; kk < 8; ++kk)
                             y[kk] = liv[kk] ? *reinterpret_cast<const float4*>(orow[kk] + c * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -645,15 +501,7 @@ __global__ void __launch_bounds__(kWThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < 8; ++kk) {
                         float4 x = *stg4(4 * kk + sub, cq);
-                        if constexpr (BOUNDED) {
-                            if (p.io16) {
-                                if (liv[kk])
-                                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(orow[kk]) + c * 32) =
-                                        make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-                                continue;
-                            }
-                        }
-                        if (!BOUNDED && p.lse != nullptr) {
+                        if (p.lse != nullptr) {
                             x.x += y[kk].x * wrr[kk];
                             x.y += y[kk].y * wrr[kk];
                             x.z += y[kk].z * wrr[kk];
@@ -775,238 +623,9 @@ __global__ void __launch_bounds__(256) wide_merge_kernel(const WideParams p, con
     *op = make_float4(acc.x * wo + y.x * wr, acc.y * wo + y.y * wr, acc.z * wo + y.z * wr, acc.w * wo + y.w * wr);
 }
 
-// ---------------------------------------------------------------- weights of chunk items
-// Attention weight of every key of a 128-key tile: a[j] = sum over query rows c of
-// 2^(s[j, c] - m[c]) / l[c], the row statistics from wide_attn_kernel. The score tile is computed
-// transposed, S^T = K . Q^T with keys as the MMA rows, so that a thread owns one key and sums its
-// row alone: no reduction across threads, and a fixed order. A CTA takes one piece: a key tile of
-// one KV head against consecutive query items [i0, i1) (their packed tiles); the pieces of a tile
-// are added in order by weight_pieces_kernel. Q tiles stream through a 2-slot ring and S^T through
-// two TMEM buffers; at 99 KB of shared memory and 256 TMEM columns two CTAs share an SM, so one's
-// exponentials run beside the other's loads and MMAs. Bound: one exponential per score (16 per
-// clock and SM), 4x the MMA's time.
-constexpr int kGThreads = 192;  // producer, MMA issuer, 4 epilogue warps
-constexpr int kGOffK = 0;
-constexpr int kGOffQ = kGOffK + kKVBytes;
-constexpr int kGOffStat = kGOffQ + 2 * kQBytes;             // [2][128] {m, 1/l} and [2][128] positions
-constexpr int kGOffBar = kGOffStat + 2 * 128 * (8 + 4);
-constexpr int kGSmemBytes = kGOffBar + 128 + 1024;
-
-__global__ void __launch_bounds__(kGThreads, 2)
-    wide_weight_kernel(const __grid_constant__ CUtensorMap tmk, const WideParams p, const int4* __restrict__ pieces,
-                       float* __restrict__ part) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float2* st_ml = reinterpret_cast<float2*>(smem + kGOffStat);
-    int* st_pos = reinterpret_cast<int*>(smem + kGOffStat + 2 * 128 * 8);
-    uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + kGOffBar);
-    uint64_t* qfull = kfull + 1;
-    uint64_t* qempty = qfull + 2;
-    uint64_t* sfull = qempty + 2;
-    uint64_t* sempty = sfull + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sempty + 2);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int4 pc = __ldg(pieces + blockIdx.x);
-    const int seq = pc.x, kt = pc.y, i0 = pc.z, n = pc.w - pc.z;
-    const int head = blockIdx.y;
-    const int kbase = kt * kWKeys;
-
-    if (threadIdx.x == 0) {
-        mbar_init(kfull, 1);
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&qfull[b], 1);
-            mbar_init(&qempty[b], 1);
-            mbar_init(&sfull[b], 1);
-            mbar_init(&sempty[b], 4);
-        }
-        *abort_flag = 0;
-        fence_mbar_init();
-    }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, 2 * kWKeys);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const uint32_t smem_base = smem_u32(smem);
-
-    if (warp == 0) {
-        if (lane == 0) {
-            prefetch_tensormap(&tmk);
-            const int per_tile = kWKeys / p.bs;
-            const int32_t* tbl = p.ids + p.indptr[seq];
-            const int nblk = p.indptr[seq + 1] - p.indptr[seq];
-            mbar_arrive_expect_tx(kfull, kKVBytes);
-            for (int b = 0; b < per_tile; ++b) {
-                const int id = __ldg(tbl + min(kt * per_tile + b, nblk - 1));  // past the end: valid, not written
-                const int slot0 = static_cast<int>(p.layer_slot0 + static_cast<int64_t>(id) * p.bs);
-                for (int c = 0; c < 2; ++c)
-                    tma_load_4d(smem + kGOffK + c * (kWKeys * 128) + b * p.bs * 128, &tmk, 0, slot0, head, c, kfull);
-            }
-            int issued = 0;
-            for (int x = 0; x < n; ++x) {
-                if (!mbar_wait_bounded(&qempty[x & 1], ((x >> 1) & 1u) ^ 1u) || *abort_flag) {
-                    *abort_flag = 1;
-                    atomicExch(p.err, kErrTimeout);
-                    break;
-                }
-                mbar_arrive_expect_tx(&qfull[x & 1], kQBytes);
-                bulk_load(smem + kGOffQ + (x & 1) * kQBytes, p.qpk + static_cast<size_t>((i0 + x) * p.kvh + head) * kQBytes,
-                          kQBytes, &qfull[x & 1]);
-                issued = x + 1;
-            }
-            // never leave the CTA with copies still landing in its shared memory
-            mbar_wait_bounded(kfull, 0u);
-            for (int x = max(0, issued - 2); x < issued; ++x) mbar_wait_bounded(&qfull[x & 1], (x >> 1) & 1u);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint64_t kd0 = smem_desc(smem_base + kGOffK, 16, 1024);
-            const uint64_t qd0 = smem_desc(smem_base + kGOffQ, 16, 1024);
-            bool ok = mbar_wait_bounded(kfull, 0u);
-            for (int x = 0; x < n && ok; ++x) {
-                const int b = x & 1;
-                ok = mbar_wait_bounded(&qfull[b], (x >> 1) & 1u) && mbar_wait_bounded(&sempty[b], ((x >> 1) & 1u) ^ 1u) &&
-                     !*abort_flag;
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int kk = 0; kk < kWD / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * (kWKeys * 128) + (kk & 3) * 32;
-                    umma_bf16(tmem + b * kWKeys, kd0 + (off >> 4), qd0 + ((b * kQBytes + off) >> 4), kIdescS, kk > 0 ? 1u : 0u);
-                }
-                umma_commit(&sfull[b]);
-                umma_commit(&qempty[b]);
-            }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicExch(p.err, kErrTimeout);
-            }
-        }
-    } else {
-        const int q4 = warp & 3;  // TMEM lanes 32 * q4 .. + 31
-        const int tid = threadIdx.x - 64;
-        const int key = 32 * q4 + lane;
-        const int j = kbase + key;
-        const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
-        // column tid of item x: its statistics and position (a dead column weighs nothing)
-        const int ct = tid / p.g, ch = head * p.g + tid % p.g;
-        auto column = [&](int x, float2& ml, int& pos) {
-            const int item = i0 + x;
-            ml = make_float2(0.f, 0.f);
-            pos = -1;
-            if (ct < __ldg(p.w_ntok + item)) {
-                const int tok = __ldg(p.w_tok0 + item) + ct;
-                pos = __ldg(p.tok_pos + tok);
-                ml = __ldg(p.ml + static_cast<size_t>(__ldg(p.tok_row + tok)) * p.H + ch);
-            }
-        };
-        float2 ml;
-        int pos;
-        column(0, ml, pos);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        bool ok = true;
-        for (int x = 0; x < n; ++x) {
-            const int b = x & 1;
-            st_ml[b * 128 + tid] = ml;
-            st_pos[b * 128 + tid] = pos;
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the epilogue warps: statistics of item x are there
-            if (x + 1 < n) column(x + 1, ml, pos);
-            // after a timeout only the barriers among these warps are kept up
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&sfull[b], (x >> 1) & 1u) && !*abort_flag);
-            if (!ok) continue;
-            tc_fence_after();
-            // the item's first and last live positions: is every (key, column) visible?
-            const int item = i0 + x;
-            const int tok0 = __ldg(p.w_tok0 + item), ntok = __ldg(p.w_ntok + item);
-            const int pa = __ldg(p.tok_pos + tok0), pb = __ldg(p.tok_pos + tok0 + ntok - 1);
-            const bool masked = kbase + kWKeys - 1 > pa || (kbase + kWKeys > p.sinks && kbase <= pb - p.window);
-#pragma unroll 1
-            for (int c0 = 0; c0 < kWRows; c0 += 32) {
-                float sv[32];
-                tmem_ld32(trow + b * kWKeys + c0, sv);
-                tmem_wait_ld();
-                const float4* mlp = reinterpret_cast<const float4*>(st_ml + b * 128 + c0);
-                if (!masked) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 a = mlp[i];
-                        sum[(2 * i) & 3] = fmaf(ex2_approx(fmaf(sv[2 * i], p.sscale, -a.x)), a.y, sum[(2 * i) & 3]);
-                        sum[(2 * i + 1) & 3] = fmaf(ex2_approx(fmaf(sv[2 * i + 1], p.sscale, -a.z)), a.w, sum[(2 * i + 1) & 3]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float2 a = st_ml[b * 128 + c0 + i];
-                        const int ps = st_pos[b * 128 + c0 + i];
-                        const bool see = j <= ps && (j < p.sinks || j > ps - p.window);
-                        const float e = see ? ex2_approx(fmaf(sv[i], p.sscale, -a.x)) : 0.f;
-                        sum[i & 3] = fmaf(e, a.y, sum[i & 3]);
-                    }
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sempty[b]);
-        }
-        if (ok) part[(static_cast<size_t>(blockIdx.x) * p.kvh + head) * kWKeys + key] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (!ok) {
-            *abort_flag = 1;
-            if (lane == 0) atomicExch(p.err, kErrTimeout);
-        }
-    }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem, 2 * kWKeys);
-    }
-}
-
-// Adds up a touched block's pieces, in order, into its weights: one thread per (block, KV head,
-// token). t_piece: first piece of the block's key tile and how many.
-__global__ void __launch_bounds__(256) weight_pieces_kernel(const WideParams p, const WeightParams w,
-                                                            const int32_t* __restrict__ starts,
-                                                            const int32_t* __restrict__ offsets,
-                                                            const int2* __restrict__ t_piece, const float* __restrict__ part) {
-    const int64_t x = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-    const int64_t e64 = x / (p.kvh * p.bs);
-    if (e64 >= w.ntouched) return;
-    const int e = static_cast<int>(e64);
-    const int hx = static_cast<int>(x - e64 * (p.kvh * p.bs));
-    const int h = hx / p.bs, t = hx - h * p.bs;
-    const int seq = w.t_seq[e], lb = w.t_blk[e];
-    const int start = starts[seq], ctx = start + offsets[seq + 1] - offsets[seq];
-    const int j = lb * p.bs + t;
-    if (j >= ctx || (j >= p.sinks && j <= start - p.window)) return;
-    const int2 pr = t_piece[e];
-    float sum = 0.f;
-    for (int i = 0; i < pr.y; ++i) sum += __ldcg(part + (static_cast<size_t>(pr.x + i) * p.kvh + h) * kWKeys + j % kWKeys);
-    float* dst = w.weights + (static_cast<size_t>(p.ids[p.indptr[seq] + lb]) * p.kvh + h) * p.bs + t;
-    *dst = w.add && j < start ? *dst + sum : sum;
-}
-
 }  // namespace
 
 size_t wide_smem_bytes() { return kSmemBytes; }
-
-cudaError_t launch_wide_weights(const CUtensorMap* tmk1, const WideParams& p, const int4* pieces, int npieces, float* part,
-                                const WeightParams& w, const int32_t* starts, const int32_t* offsets, const int2* t_piece,
-                                cudaStream_t st) {
-    if (npieces <= 0 || w.ntouched <= 0) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(wide_weight_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGSmemBytes);
-    if (e != cudaSuccess) return e;
-    wide_weight_kernel<<<dim3(npieces, p.kvh), kGThreads, kGSmemBytes, st>>>(*tmk1, p, pieces, part);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const int64_t blocks = (static_cast<int64_t>(w.ntouched) * p.kvh * p.bs + 255) / 256;
-    if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    weight_pieces_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, w, starts, offsets, t_piece, part);
-    return cudaGetLastError();
-}
 
 cudaError_t launch_wide_merge(const WideParams& p, const int32_t* split, int nsplit, cudaStream_t st) {
     if (nsplit <= 0) return cudaSuccess;
@@ -1020,7 +639,6 @@ cudaError_t launch_wide_merge(const WideParams& p, const int32_t* split, int nsp
 // rounded to bf16, in the exact shared-memory image the S MMA reads ([64-dim chunk][row]
 // [64], 128-byte swizzle), so that a CTA fetches it with one 32 KB bulk copy. Rows past the
 // item's tokens are zero, and so is the extra last tile (the empty half of a pair).
-template <bool IO16>
 __device__ __forceinline__ void pack_q_tile(const WideParams& p, int ntiles, uint8_t* __restrict__ qpk, int b) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* dst = qpk + static_cast<size_t>(b) * kQBytes;
@@ -1030,21 +648,6 @@ __device__ __forceinline__ void pack_q_tile(const WideParams& p, int ntiles, uin
     const int tok0 = real ? p.w_tok0[item] : 0;
     const int g = p.g;
     const int c = lane >> 4, u = (lane & 15) >> 1, half = lane & 1;
-    if constexpr (IO16) {  // bf16 queries as they are
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-            const int r = 32 * warp + i;
-            uint2 x = make_uint2(0, 0);
-            if (r / g < ntok) {
-                const int row = p.tok_row[tok0 + r / g];
-                const __nv_bfloat16* qp = reinterpret_cast<const __nv_bfloat16*>(p.q) +
-                                          (static_cast<size_t>(row) * p.H + h * g + r % g) * kWD;
-                x = __ldg(reinterpret_cast<const uint2*>(qp) + lane);
-            }
-            *reinterpret_cast<uint2*>(dst + c * (kWRows * 128) + sw128(r, u) + half * 8) = x;
-        }
-        return;
-    }
 #pragma unroll 1
     for (int i0 = 0; i0 < 32; i0 += 16) {
         float4 x[16];
@@ -1069,17 +672,16 @@ __device__ __forceinline__ void pack_q_tile(const WideParams& p, int ntiles, uin
 }
 
 __global__ void __launch_bounds__(128) wide_q_pack_kernel(const WideParams p, int ntiles, uint8_t* __restrict__ qpk) {
-    pack_q_tile<false>(p, ntiles, qpk, blockIdx.x);
+    pack_q_tile(p, ntiles, qpk, blockIdx.x);
 }
 
 // The pack and the append of the chunk rows (rows[0..n) of the step, fp32 -> the bf16
 // pool, slot from the block table: sequence row_seq[r], position starts[s] + r - offsets[s])
 // in one launch: CTAs 0..ntiles pack, the rest append 4 dims per thread.
-template <bool IO16>
 __global__ void __launch_bounds__(128) wide_prep_kernel(const WideParams p, int ntiles, uint8_t* __restrict__ qpk,
                                                         const WideAppend a) {
     if (static_cast<int>(blockIdx.x) <= ntiles) {
-        pack_q_tile<IO16>(p, ntiles, qpk, blockIdx.x);
+        pack_q_tile(p, ntiles, qpk, blockIdx.x);
         return;
     }
     const int per_row = a.rowlen / 4;
@@ -1089,16 +691,8 @@ __global__ void __launch_bounds__(128) wide_prep_kernel(const WideParams p, int 
         const int64_t ri = i / per_row;
         const int c = static_cast<int>(i - ri * per_row) * 4;
         const int64_t r = a.rows[ri];
-        uint2 kb, vb;
-        if constexpr (IO16) {
-            kb = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(a.k) + r * a.rowlen + c);
-            vb = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(a.v) + r * a.rowlen + c);
-        } else {
-            const float4 kx = *reinterpret_cast<const float4*>(a.k + r * a.rowlen + c);
-            const float4 vx = *reinterpret_cast<const float4*>(a.v + r * a.rowlen + c);
-            kb = make_uint2(pack_bf16(kx.x, kx.y), pack_bf16(kx.z, kx.w));
-            vb = make_uint2(pack_bf16(vx.x, vx.y), pack_bf16(vx.z, vx.w));
-        }
+        const float4 kx = *reinterpret_cast<const float4*>(a.k + r * a.rowlen + c);
+        const float4 vx = *reinterpret_cast<const float4*>(a.v + r * a.rowlen + c);
         int64_t slot;
         if (a.slots != nullptr) {
             slot = a.slots[ri];  // from the plan: one load instead of a chain of five
@@ -1109,8 +703,8 @@ __global__ void __launch_bounds__(128) wide_prep_kernel(const WideParams p, int 
             slot = static_cast<int64_t>(a.ids[a.indptr[sq] + blk]) * a.bs + (pos - blk * a.bs);
         }
         const int64_t dst = slot * a.rowlen + c;
-        *reinterpret_cast<uint2*>(a.pool_k + dst) = kb;
-        *reinterpret_cast<uint2*>(a.pool_v + dst) = vb;
+        *reinterpret_cast<uint2*>(a.pool_k + dst) = make_uint2(pack_bf16(kx.x, kx.y), pack_bf16(kx.z, kx.w));
+        *reinterpret_cast<uint2*>(a.pool_v + dst) = make_uint2(pack_bf16(vx.x, vx.y), pack_bf16(vx.z, vx.w));
     }
 }
 
@@ -1126,19 +720,16 @@ cudaError_t launch_wide_prep(const WideParams& p, int nitems, uint8_t* qpk, cons
     const int ntiles = nitems * p.kvh;
     const int64_t items = a.n * (a.rowlen / 4);
     const int64_t ablocks = std::min<int64_t>((items + 127) / 128, 148 * 16);
-    const unsigned grid = static_cast<unsigned>(ntiles + 1 + std::max<int64_t>(ablocks, 1));
-    if (p.io16) wide_prep_kernel<true><<<grid, 128, 0, st>>>(p, ntiles, qpk, a);
-    else wide_prep_kernel<false><<<grid, 128, 0, st>>>(p, ntiles, qpk, a);
+    wide_prep_kernel<<<static_cast<unsigned>(ntiles + 1 + std::max<int64_t>(ablocks, 1)), 128, 0, st>>>(p, ntiles, qpk, a);
     return cudaGetLastError();
 }
 
 cudaError_t launch_wide_attention(const CUtensorMap* tmk1, const CUtensorMap* tmv1, const WideParams& p,
                                   cudaStream_t st) {
     if (p.nctas <= 0) return cudaSuccess;
-    auto kern = p.pair_bound != nullptr ? wide_attn_kernel<true> : wide_attn_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(wide_attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
-    kern<<<p.nctas, kWThreads, kSmemBytes, st>>>(*tmk1, *tmv1, p);
+    wide_attn_kernel<<<p.nctas, kWThreads, kSmemBytes, st>>>(*tmk1, *tmv1, p);
     return cudaGetLastError();
 }
 

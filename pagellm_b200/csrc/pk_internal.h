@@ -181,13 +181,13 @@ struct WideParams {
     int bs;
     int64_t layer_slot0;
     float qscale;
-    // Bounded chunk items (pair_bound NULL: off).
-    const int4* pair_bound;  // [pairs] {head, skip, lo, 0}: see PairBound in the kernel
+    // Bounded chunk items (chunk_attn_kernel, chunk_weight_kernel).
+    const int4* pair_bound;  // [pairs] {head, skip, lo, tiles}: see PairBound in the kernels
     int window;              // >= 1; INT32_MAX without a window
     int sinks;
     float sscale;            // applied to the scores: 1 when the packed queries are scaled, else qscale
-    int io16;                // q and out (and the appended rows) hold bf16
-    float2* ml;              // [rows][H] (max, 1 / sum) of each output row, log2 domain, or NULL
+    int io16;                // q and out hold bf16
+    float2* ml;              // [items][kvh][128] (max, 1 / sum) of each query row, log2 domain, or NULL
 };
 
 // Windowed attention on the CUDA cores: any pool, rows of `q` / `out` in the pool's input type.
@@ -358,12 +358,17 @@ cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const i
 
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
-// Weights of chunk items: pieces {sequence, key tile, first and end query item} scored on the
-// tensor cores into part[npieces][kvh][128], then added up into the touched blocks of `w` (t_piece:
-// first piece of each block's key tile and how many).
-cudaError_t launch_wide_weights(const CUtensorMap* tmk1, const WideParams& p, const int4* pieces, int npieces, float* part,
-                                const WeightParams& w, const int32_t* starts, const int32_t* offsets, const int2* t_piece,
-                                cudaStream_t st);
+// Chunk items of a bounded step: `npairs` pairs x KV heads. tmq: the tensor map of bf16 queries
+// (p.io16; unread otherwise).
+size_t chunk_smem_bytes();
+cudaError_t launch_chunk_attention(const CUtensorMap* tmk1, const CUtensorMap* tmv1, const CUtensorMap* tmq,
+                                   const WideParams& p, int npairs, cudaStream_t st);
+// Their weights: pieces {sequence, key tile, first and end query item} scored into
+// part[npieces][kvh][128], then added up into the touched blocks of `w` (t_piece: first piece of
+// each block's key tile and how many).
+cudaError_t launch_chunk_weights(const CUtensorMap* tmk1, const CUtensorMap* tmq, const WideParams& p, const int4* pieces,
+                                 int npieces, float* part, const WeightParams& w, const int32_t* starts,
+                                 const int32_t* offsets, const int2* t_piece, cudaStream_t st);
 cudaError_t launch_weight_scores(const ScoreWeightParams& p, cudaStream_t st);
 // launch_append_table for rows given as bf16 (bf16 pools).
 cudaError_t launch_append_rows16(void* pool_k_layer, void* pool_v_layer, const void* k, const void* v,
