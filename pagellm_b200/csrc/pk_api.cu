@@ -237,6 +237,9 @@ struct pk_pool {
     bool wide_ok = false;
     CUtensorMap tmk1{};
     CUtensorMap tmv1{};
+    // bounded chunk kernel: the same with at most kChunkKeys slots of a block per box
+    CUtensorMap tmk2{};
+    CUtensorMap tmv2{};
     Uploader pairs_up;
     // accumulated attention weights, [layers][num_blocks][kvh][block_size]; NULL = not tracked
     float* weights = nullptr;
@@ -387,13 +390,15 @@ bool encode_chunk_maps(pk_pool* P, std::string* why) {
     const cuuint64_t slots = static_cast<cuuint64_t>(P->n_layers) * P->num_blocks * P->block_size;
     cuuint64_t dims[4] = {64, slots, static_cast<cuuint64_t>(P->kvh), static_cast<cuuint64_t>(P->d / 64)};
     cuuint64_t strides[3] = {static_cast<cuuint64_t>(P->kvh) * P->d * 2, static_cast<cuuint64_t>(P->d) * 2, 128};
-    // one 64-dim chunk of one block per box, for K and V alike
-    const cuuint32_t box_k[4] = {64, static_cast<cuuint32_t>(P->block_size), 1, 1};
-    const cuuint32_t box_v[4] = {64, static_cast<cuuint32_t>(P->block_size), 1, 1};
+    // one 64-dim chunk of one block (maps 1) or of at most kChunkKeys of its slots (maps 2) per box
+    const cuuint32_t slots1 = static_cast<cuuint32_t>(P->block_size);
+    const cuuint32_t box1[4] = {64, slots1, 1, 1};
+    const cuuint32_t box2[4] = {64, std::min<cuuint32_t>(slots1, pk::kChunkKeys), 1, 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
-    for (int t = 0; t < 2; ++t) {
-        CUresult r = enc(t == 0 ? &P->tmk1 : &P->tmv1, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                         t == 0 ? P->k : P->v, dims, strides, t == 0 ? box_k : box_v, estr,
+    for (int t = 0; t < 4; ++t) {
+        CUtensorMap* map = t == 0 ? &P->tmk1 : t == 1 ? &P->tmv1 : t == 2 ? &P->tmk2 : &P->tmv2;
+        CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                         t % 2 == 0 ? P->k : P->v, dims, strides, t < 2 ? box1 : box2, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -720,7 +725,7 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
         if (!B->bounded()) continue;
         // the window of the pair's first row (items and their tokens are in position order)
         const int64_t q0 = B->tok_pos[B->w_tok0[B->w_pair[2 * x]]];
-        const VisibleBlocks vb = visible_blocks(q0, B->pair_kend[x], B->window, B->sinks, pk::kWideKeys);
+        const VisibleBlocks vb = visible_blocks(q0, B->pair_kend[x], B->window, B->sinks, pk::kChunkKeys);
         pair_tiles[x] = vb.count;
         const int64_t lo = B->window > 0 ? std::max<int64_t>(0, q0 - B->window + 1) : 0;
         B->pair_bound.insert(B->pair_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(lo), static_cast<int32_t>(vb.count)});
@@ -1531,7 +1536,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             B->launches++;
         }
         PK_CUDA(prof_begin(B, ws));
-        PK_CUDA(pk::launch_chunk_attention(&P->tmk1, &P->tmv1, &tmq, wide, B->npair_chunk, ws));
+        PK_CUDA(pk::launch_chunk_attention(&P->tmk2, &P->tmv2, &tmq, wide, B->npair_chunk, ws));
         PK_CUDA(prof_end(B, kProfWide, ws));
         B->launches++;
     }

@@ -12,6 +12,7 @@ namespace pk {
 constexpr int kMaxCols = 16;
 // Largest number of KV heads the tensor-core kernel maps to warps of one CTA.
 constexpr int kTcMaxKvHeads = 8;
+constexpr int kChunkKeys = 64;  // keys per tile of the bounded chunk kernel
 constexpr int kWideKeys = 128;  // keys per tile of the wide-tile kernel (a multiple of block_size)
 
 // Parameters of the split-KV tensor-core attention kernel (bf16 pool).
@@ -359,9 +360,9 @@ cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const i
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
 // Chunk items of a bounded step: `npairs` pairs x KV heads. tmq: the tensor map of bf16 queries
-// (p.io16; unread otherwise).
+// (p.io16; unread otherwise); tmk2 / tmv2: boxes of min(block_size, kChunkKeys) slots.
 size_t chunk_smem_bytes();
-cudaError_t launch_chunk_attention(const CUtensorMap* tmk1, const CUtensorMap* tmv1, const CUtensorMap* tmq,
+cudaError_t launch_chunk_attention(const CUtensorMap* tmk2, const CUtensorMap* tmv2, const CUtensorMap* tmq,
                                    const WideParams& p, int npairs, cudaStream_t st);
 // Their weights: pieces {sequence, key tile, first and end query item} scored into
 // part[npieces][kvh][128], then added up into the touched blocks of `w` (t_piece: first piece of
