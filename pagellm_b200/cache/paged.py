@@ -43,12 +43,18 @@ __all__ = [
 ]
 
 
-def _torch():
-    import torch
+_TORCH = None  # torch, once a device has been seen
 
-    if not torch.cuda.is_available():
-        raise RuntimeError("pagellm_b200 needs a CUDA device (B200, sm_100a); none is visible")
-    return torch
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+
+        if not torch.cuda.is_available():
+            raise RuntimeError("pagellm_b200 needs a CUDA device (B200, sm_100a); none is visible")
+        _TORCH = torch
+    return _TORCH
 
 
 def _stream(device) -> int:

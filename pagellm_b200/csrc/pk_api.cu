@@ -340,6 +340,12 @@ struct pk_batch {
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
     std::vector<uint8_t> seq_tc;        // scratch: sequence is on the split-KV kernel
+    // rows on the CUDA cores (cc_attn_kernel): records, splits of the visible keys, whether their
+    // weights are summed in the same launch
+    bool use_cc = false, cc_weights = false;
+    int cc_nsplit = 1, cc_max_vis = 0;
+    std::vector<int32_t> cc_meta, cc_zero;
+    DevBuf cc_part;
     DevBuf score;                       // raw scores of a split-KV launch with weights
     bool use_scores = false;
     DevBuf ml;  // [rows][H] softmax statistics of a step with weights
@@ -868,6 +874,48 @@ void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::
     for (size_t x = 0; x < ts.size(); ++x) B->t_piece.insert(B->t_piece.end(), {p0[of[x]], np[of[x]]});
 }
 
+// Bounded rows on the CUDA cores. Splits: enough CTAs for kCcCtasPerSm per SM, as long as a split
+// keeps kCcMinKeys visible keys of the average row. Weights are summed in the same launch when every
+// such sequence has one row, a CTA has all of its KV head's query heads and all keys, and the scores
+// fit kCcScoreBytes of shared memory.
+constexpr int64_t kCcCtasPerSm = 4, kCcMinKeys = 128, kCcScoreBytes = 64 * 1024;
+int plan_cc(pk_batch* B, int H) {
+    pk_pool* P = B->pool;
+    const int g = H / P->kvh;
+    B->use_cc = B->bounded() && B->ngeneric > 0 && P->d % 4 == 0 && P->d <= 512;
+    B->cc_meta.clear();
+    B->cc_zero.clear();
+    B->cc_weights = false;
+    if (!B->use_cc) return PK_OK;
+    int64_t vis = 0, most = 0;
+    bool single = true;
+    for (int r : B->gen_rows) {
+        const int i = B->row_seq[r];
+        const int64_t pos = static_cast<int64_t>(B->starts[i]) + (r - B->offsets[i]);
+        const int64_t lo = B->window > 0 ? std::max<int64_t>(0, pos - B->window + 1) : 0;
+        const int64_t n = std::min(B->sinks, lo) + pos - lo + 1;
+        vis += n;
+        most = std::max(most, n);
+        single = single && B->nnew[i] == 1;
+        B->cc_meta.insert(B->cc_meta.end(), {r, B->indptr[i], static_cast<int32_t>(pos), B->starts[i], B->offsets[i], 0, 0, 0});
+    }
+    const int G = pk::cc_group(g);
+    const int64_t groups = static_cast<int64_t>(P->kvh) * ceil_div(g, G);
+    const int64_t ctas = static_cast<int64_t>(B->ngeneric) * groups;
+    if (groups > 65535) return fail(PK_ERR_UNSUPPORTED, "n_heads %d too large", H);
+    const int64_t want = (kCcCtasPerSm * P->num_sms + ctas - 1) / ctas;
+    const int64_t room = std::max<int64_t>(1, vis / B->ngeneric / kCcMinKeys);
+    B->cc_nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, room, 256})));
+    B->cc_max_vis = static_cast<int>(most);
+    B->cc_weights = B->weights_mode != 0 && single && g <= G && most * G * 4 <= kCcScoreBytes;
+    if (B->cc_weights) B->cc_nsplit = 1;
+    if (B->cc_nsplit > 1) {
+        PK_CUDA(B->cc_part.reserve(static_cast<size_t>(ctas) * B->cc_nsplit * G * (P->d + 2) * sizeof(float)));
+        B->cc_zero.assign(static_cast<size_t>(ctas), 0);
+    }
+    return PK_OK;
+}
+
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
@@ -1114,6 +1162,10 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan.add(B->pair_bound.data(), B->pair_bound.size() * 4);  // 30
     B->plan.add(B->pieces.data(), B->pieces.size() * 4);  // 31
     B->plan.add(B->t_piece.data(), B->t_piece.size() * 4);  // 32
+    int rc = plan_cc(B, H);
+    if (rc != PK_OK) return rc;
+    B->plan.add(B->cc_meta.data(), B->cc_meta.size() * 4);  // 33
+    B->plan.add(B->cc_zero.data(), B->cc_zero.size() * 4);  // 34
     if (B->weights_mode != 0)
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
@@ -1121,7 +1173,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (!B->w_seq.empty())
         PK_CUDA(B->qpk.reserve((B->w_seq.size() * P->kvh + 1) * static_cast<size_t>(pk::kWideQTileBytes)));
     if (B->nprefix > 0) PK_CUDA(B->lse.reserve(static_cast<size_t>(B->nrows) * H * sizeof(float)));
-    int rc = B->plan.commit(st);
+    rc = B->plan.commit(st);
     if (rc != PK_OK) return rc;
     B->plan_stream = st;
     B->plan_H = H;
@@ -1439,8 +1491,11 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     }
     // decode steps append inside the split-KV kernel and chunk rows with the packing of their
     // queries, as in plain steps
-    const bool fused = k_new != nullptr && (B->use_tc || B->nwide > 0) && B->ngeneric == 0 && B->fuse_append_ok &&
-                       B->tc_max_new <= kFuseMaxNew;
+    const bool fused_tc = k_new != nullptr && (B->use_tc || B->nwide > 0) && B->ngeneric == 0 && B->fuse_append_ok &&
+                          B->tc_max_new <= kFuseMaxNew;
+    // (a step wholly on cc_attn_kernel appends there)
+    const bool fused_cc = k_new != nullptr && B->use_cc && !B->use_tc && B->nwide == 0 && B->fuse_append_ok;
+    const bool fused = fused_tc || fused_cc;
     if (k_new != nullptr && !fused) {
         const bool listed = !B->app_rows.empty();
         const int32_t* rows = listed ? B->meta.at<int32_t>(5) : nullptr;
@@ -1557,7 +1612,37 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         PK_CUDA(prof_end(B, kProfTc, st));
         B->launches++;
     }
-    if (B->ngeneric > 0) {
+    if (B->use_cc) {
+        pk::CcParams c{};
+        c.q = q;
+        c.out = out;
+        c.pool_k = p.pool_k;
+        c.pool_v = p.pool_v;
+        c.k_new = fused_cc ? k_new : nullptr;
+        c.v_new = fused_cc ? v_new : nullptr;
+        c.ids = p.ids;
+        c.meta = B->plan.at<int4>(33);
+        c.ml = B->cc_weights ? nullptr : p.ml;
+        c.weights = B->cc_weights ? P->weights + static_cast<int64_t>(layer) * P->layer_weights() : nullptr;
+        c.part = static_cast<float*>(B->cc_part.ptr);
+        c.counters = B->plan.at<int>(34);
+        c.nrows = B->ngeneric;
+        c.nsplit = B->cc_nsplit;
+        c.max_vis = B->cc_max_vis;
+        c.H = H;
+        c.kvh = p.kvh;
+        c.D = p.D;
+        c.bs = p.bs;
+        c.bs_shift = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(p.bs)) : -1;
+        c.window = p.window;
+        c.sinks = p.sinks;
+        c.add = B->weights_mode == 1;
+        c.qscale = p.qscale;
+        PK_CUDA(prof_begin(B, st));
+        PK_CUDA(pk::launch_cc_attention(P->dtype, io16, c, st));
+        PK_CUDA(prof_end(B, kProfGeneric, st));
+        B->launches++;
+    } else if (B->ngeneric > 0) {
         PK_CUDA(prof_begin(B, st));
         PK_CUDA(pk::launch_bounded_rows(P->dtype, io16, p, st));
         PK_CUDA(prof_end(B, kProfGeneric, st));
@@ -1606,7 +1691,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         }
         w.t_seq += B->ntouch_wide;
         w.t_blk += B->ntouch_wide;
-        w.ntouched = static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide;
+        w.ntouched = B->cc_weights ? 0 : static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide;
         if (w.ntouched > 0) {
             PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
             B->launches++;
@@ -2022,6 +2107,7 @@ int pk_batch_destroy(pk_batch* B) {
     B->qpk.release();
     B->ml.release();
     B->score.release();
+    B->cc_part.release();
     B->wpieces.release();
     B->ml_items.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);

@@ -215,6 +215,36 @@ struct BoundedParams {
     float qscale;  // log2(e) / sqrt(D)
 };
 
+// Windowed attention on the CUDA cores for rows of 4-element multiples (cc_attn_kernel).
+struct CcParams {
+    const void* q;       // [rows][H][D], float or bf16 as k_new, v_new and out
+    void* out;
+    const void* pool_k;  // layer base
+    const void* pool_v;
+    const void* k_new;   // fused append: the step's rows [rows][kvh][D]; NULL = off
+    const void* v_new;
+    const int32_t* ids;
+    const int4* meta;    // [nrows][2] {row, first table entry, position, sequence start}, {sequence's first row, ..}
+    float2* ml;          // [rows][H] (max, 1 / sum), log2 domain, or NULL
+    float* weights;      // fused weights of the layer, or NULL
+    float* part;         // [nrows][grid.y][nsplit][G][D + 2] partials (nsplit > 1)
+    int* counters;       // [nrows][grid.y], zero between launches
+    int nrows;
+    int nsplit;
+    int max_vis;         // most visible keys of a row (fused weights)
+    int H;
+    int kvh;
+    int D;
+    int bs;
+    int bs_shift;        // log2 of bs, or -1
+    int window;          // >= 1; INT32_MAX without a window
+    int sinks;
+    int add;
+    float qscale;        // log2(e) / sqrt(D)
+};
+// Query heads of a KV head that a CTA of cc_attn_kernel takes together.
+inline int cc_group(int g) { return g == 1 ? 1 : g == 2 ? 2 : 4; }
+
 // The touched blocks of a step - those with a key that some row sees - and the layer's
 // accumulated weights [num_blocks][kvh][bs].
 struct WeightParams {
@@ -357,6 +387,7 @@ cudaError_t launch_interleave_heads(const float* src, float* dst, int world, int
 cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const int64_t* positions,
                                 int64_t n, int bs, int64_t* slots, int32_t* err, cudaStream_t st);
 
+cudaError_t launch_cc_attention(int dtype, bool io16, const CcParams& p, cudaStream_t st);
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
 // Chunk items of a bounded step: `npairs` pairs x KV heads. tmq: the tensor map of bf16 queries
