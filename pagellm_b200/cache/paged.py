@@ -308,13 +308,21 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _rows(t, device, dtype):
+    """``t`` as a contiguous, 16-byte aligned tensor of ``dtype`` on ``device``: itself when it is
+    one already (every step of a running model), else a copy."""
+    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+        t = t.to(device, dtype).contiguous()
+    return _aligned(t)
+
+
 def _csr(block_tables):
     """(indptr int64, ids int32) from a list of per-sequence block lists / arrays."""
     if isinstance(block_tables, tuple) and len(block_tables) == 2 and isinstance(block_tables[0], np.ndarray) \
             and block_tables[0].ndim == 1 and len(block_tables[0]) and block_tables[0][0] == 0 \
             and block_tables[1].dtype == np.int32:
         return np.ascontiguousarray(block_tables[0], np.int64), np.ascontiguousarray(block_tables[1])
-    lens = np.fromiter((len(t) for t in block_tables), dtype=np.int64, count=len(block_tables))
+    lens = np.fromiter(map(len, block_tables), dtype=np.int64, count=len(block_tables))
     indptr = np.zeros(len(lens) + 1, dtype=np.int64)
     np.cumsum(lens, out=indptr[1:])
     total = int(indptr[-1])
@@ -497,16 +505,26 @@ class PagedBatch:
             if tuple(k.shape) != want or tuple(v.shape) != want:
                 raise ValueError(f"k, v must be {want}")
         st = _stream(P.device)
-        if self._bounded and hasattr(q, "is_cuda") and P.dtype_name == "bfloat16" and str(q.dtype) == "torch.bfloat16":
+        if self._bounded and hasattr(q, "is_cuda"):
             torch = _torch()
-            qd = _aligned(q.to(P.device).contiguous())
+            # bf16 rows on a bf16 pool as they are, anything else as float32
+            io16 = q.dtype == torch.bfloat16 and P.dtype_name == "bfloat16"
+            dt = torch.bfloat16 if io16 else torch.float32
+            qd = _rows(q, P.device, dt)
             out = torch.empty_like(qd)
-            kd = _aligned(k.to(P.device, torch.bfloat16).contiguous()) if append else None
-            vd = _aligned(v.to(P.device, torch.bfloat16).contiguous()) if append else None
-            _lib.check(self._lib.pk_batch_write_and_attend_bf16(
-                self._b, layer, H, qd.data_ptr(), kd.data_ptr() if append else None,
-                vd.data_ptr() if append else None, out.data_ptr(), st))
-            return out
+            kp = vp = None
+            if append:
+                kd, vd = _rows(k, P.device, dt), _rows(v, P.device, dt)
+                kp, vp = kd.data_ptr(), vd.data_ptr()
+            if io16:
+                rc = self._lib.pk_batch_write_and_attend_bf16(self._b, layer, H, qd.data_ptr(), kp, vp, out.data_ptr(), st)
+            elif append:
+                rc = self._lib.pk_batch_write_and_attend(self._b, layer, H, qd.data_ptr(), kp, vp, out.data_ptr(), st)
+            else:
+                rc = self._lib.pk_batch_attend(self._b, layer, H, qd.data_ptr(), out.data_ptr(), st)
+            if rc:
+                _lib.check(rc)
+            return out if io16 or q.dtype == torch.float32 else out.to(q.dtype)
         if hasattr(q, "is_cuda"):
             torch = _torch()
             qd = _aligned(q.to(P.device, torch.float32).contiguous())

@@ -339,6 +339,7 @@ struct pk_batch {
     DevBuf ml_items;                    // [chunk items][kvh][128] softmax statistics
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
+    std::vector<int32_t> t_meta;        // records of the first ntouch_tc touched blocks
     std::vector<uint8_t> seq_tc;        // scratch: sequence is on the split-KV kernel
     // rows on the CUDA cores (cc_attn_kernel): records, splits of the visible keys, whether their
     // weights are summed in the same launch
@@ -519,6 +520,9 @@ void setup_tc(pk_pool* P) {
     P->wide_ok = P->d == 128 && pk::kWideKeys % P->block_size == 0 && P->tc_per_head == 0 &&
                  static_cast<size_t>(optin) >= pk::wide_smem_bytes() && encode_chunk_maps(P, &why2);
 }
+
+// log2 of a power of two, else -1
+int log2_or_minus(int x) { return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(x)) : -1; }
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -1158,7 +1162,13 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan.add(B->t_seq.data(), B->t_seq.size() * 4);  // 26
     B->plan.add(B->t_blk.data(), B->t_blk.size() * 4);  // 27
     B->plan.add(B->u_bound.data(), B->u_bound.size() * 4);  // 28
-    B->plan.add(B->seq_u.data(), B->seq_u.size() * 4);  // 29
+    B->t_meta.clear();
+    for (int x = 0; x < B->ntouch_tc; ++x) {
+        const int i = B->t_seq[x];
+        B->t_meta.insert(B->t_meta.end(), {B->ids[B->indptr[i] + B->t_blk[x]], B->t_blk[x], B->seq_u[i], B->seq_u[i + 1],
+                                           B->starts[i], B->starts[i] + B->nnew[i], 0, 0});
+    }
+    B->plan.add(B->t_meta.data(), B->t_meta.size() * 4);  // 29
     B->plan.add(B->pair_bound.data(), B->pair_bound.size() * 4);  // 30
     B->plan.add(B->pieces.data(), B->pieces.size() * 4);  // 31
     B->plan.add(B->t_piece.data(), B->t_piece.size() * 4);  // 32
@@ -1633,7 +1643,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         c.kvh = p.kvh;
         c.D = p.D;
         c.bs = p.bs;
-        c.bs_shift = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(p.bs)) : -1;
+        c.bs_shift = log2_or_minus(p.bs);
         c.window = p.window;
         c.sinks = p.sinks;
         c.add = B->weights_mode == 1;
@@ -1664,17 +1674,14 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             sw.w = w;
             sw.score = static_cast<const float*>(B->score.ptr);
             sw.ml = p.ml;
-            sw.seq_u = B->plan.at<int32_t>(29);
+            sw.t_meta = B->plan.at<int4>(29);
             sw.u_meta = B->plan.at<int4>(24);
             sw.u_bound = B->plan.at<int4>(28);
-            sw.indptr = p.indptr;
-            sw.ids = p.ids;
-            sw.starts = p.starts;
-            sw.offsets = p.offsets;
             sw.kvh = p.kvh;
             sw.g = H / p.kvh;
             sw.H = H;
             sw.bs = p.bs;
+            sw.bs_shift = log2_or_minus(p.bs);
             sw.window = p.window;
             sw.sinks = p.sinks;
             PK_CUDA(pk::launch_weight_scores(sw, st));

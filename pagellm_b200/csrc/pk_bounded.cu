@@ -183,43 +183,66 @@ cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, 
 }
 
 // The scores of the touched blocks are still in L2 (8 to 64 bytes per key and KV head beside the
-// 512 of its K and V), so summing them costs a fraction of reading K again. Units of a sequence in
-// order, columns in order: the sum does not depend on the schedule.
+// 512 of its K and V), so summing them costs a fraction of reading K again. One warp per touched
+// block, its (KV head, token) pairs over the lanes, four of them in flight; records from the plan, so
+// that the chain is record -> unit -> scores. Units of a sequence in order, columns in order: the sum
+// does not depend on the schedule.
 __global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightParams p) {
-    const int64_t x = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-    const int64_t e64 = x / (p.kvh * p.bs);
-    if (e64 >= p.w.ntouched) return;
-    const int e = static_cast<int>(e64);
-    const int hx = static_cast<int>(x - e64 * (p.kvh * p.bs));
-    const int h = hx / p.bs, t = hx - h * p.bs;
-    const int seq = p.w.t_seq[e], lb = p.w.t_blk[e];
-    const int start = p.starts[seq], ctx = start + p.offsets[seq + 1] - p.offsets[seq];
-    const int j = lb * p.bs + t;
-    if (j >= ctx || (j >= p.sinks && j <= start - p.window)) return;
-    float sum = 0.f;
-    for (int u = p.seq_u[seq]; u < p.seq_u[seq + 1]; ++u) {
-        const int4 b = __ldg(p.u_bound + u);
-        const int4 m0 = __ldg(p.u_meta + 2 * u), m1 = __ldg(p.u_meta + 2 * u + 1);
-        const int nblk = m1.z - m1.y;
-        const int i = lb < b.x ? lb : lb - b.y;
-        if (i >= nblk || (lb >= b.x && i < b.x)) continue;  // not a block of this unit
-        const int ncol = m0.y * p.g, colp = (ncol + 1) & ~1;
-        const float* sp = p.score + (static_cast<int64_t>(static_cast<uint32_t>(b.z)) | (static_cast<int64_t>(b.w) << 32)) +
-                          ((static_cast<int64_t>(h) * nblk + i) * p.bs + t) * colp;
-        const float2* ml = p.ml + static_cast<size_t>(m0.w) * p.H + h * p.g;
-        for (int c = 0; c < ncol; c += 2) {
-            const float2 s = __ldcg(reinterpret_cast<const float2*>(sp + c));
-            const float2 a = __ldg(ml + (c / p.g) * p.H + c % p.g);
-            sum += exp2f(s.x - a.x) * a.y;
-            if (c + 1 < ncol) {
-                const float2 b2 = __ldg(ml + ((c + 1) / p.g) * p.H + (c + 1) % p.g);
-                sum += exp2f(s.y - b2.x) * b2.y;
+    const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (e >= p.w.ntouched) return;
+    const int4 r0 = __ldg(p.t_meta + 2 * e), r1 = __ldg(p.t_meta + 2 * e + 1);
+    const int phys = r0.x, lb = r0.y, u0 = r0.z, u1 = r0.w, start = r1.x, ctx = r1.y;
+    const int pairs = p.kvh * p.bs;
+    float* wb = p.w.weights + static_cast<size_t>(phys) * pairs;
+    constexpr int kPer = 4;
+    for (int x0 = lane; x0 < pairs; x0 += 32 * kPer) {
+        float sum[kPer], old[kPer];
+        int h[kPer], t[kPer];
+        bool live[kPer];
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const int x = x0 + 32 * k;
+            h[k] = p.bs_shift >= 0 ? x >> p.bs_shift : x / p.bs;
+            t[k] = x - h[k] * p.bs;
+            const int j = lb * p.bs + t[k];
+            live[k] = x < pairs && j < ctx && (j < p.sinks || j > start - p.window);
+            sum[k] = 0.f;
+            old[k] = live[k] && p.w.add && j < start ? wb[x] : 0.f;
+        }
+        for (int u = u0; u < u1; ++u) {
+            const int4 b = __ldg(p.u_bound + u);
+            const int4 m0 = __ldg(p.u_meta + 2 * u), m1 = __ldg(p.u_meta + 2 * u + 1);
+            const int nblk = m1.z - m1.y;
+            const int i = lb < b.x ? lb : lb - b.y;
+            if (i >= nblk || (lb >= b.x && i < b.x)) continue;  // not a block of this unit
+            const int ncol = m0.y * p.g, colp = (ncol + 1) & ~1;
+            const float* sp = p.score + (static_cast<int64_t>(static_cast<uint32_t>(b.z)) | (static_cast<int64_t>(b.w) << 32));
+            for (int c = 0; c < ncol; c += 2) {
+                // columns c and c + 1: query token c / g, head c % g of the KV head's
+                const int ta = c / p.g, tb = (c + 1) / p.g;
+                const size_t ra = static_cast<size_t>(m0.w + ta) * p.H + (c - ta * p.g);
+                const size_t rb = static_cast<size_t>(m0.w + tb) * p.H + (c + 1 - tb * p.g);
+                float2 s[kPer], ma[kPer], mb[kPer];
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    if (!live[k]) continue;
+                    s[k] = __ldcg(reinterpret_cast<const float2*>(
+                        sp + ((static_cast<int64_t>(h[k]) * nblk + i) * p.bs + t[k]) * colp + c));
+                    ma[k] = __ldg(p.ml + ra + h[k] * p.g);
+                    if (c + 1 < ncol) mb[k] = __ldg(p.ml + rb + h[k] * p.g);
+                }
+#pragma unroll
+                for (int k = 0; k < kPer; ++k) {
+                    if (!live[k]) continue;
+                    sum[k] += exp2f(s[k].x - ma[k].x) * ma[k].y;
+                    if (c + 1 < ncol) sum[k] += exp2f(s[k].y - mb[k].x) * mb[k].y;
+                }
             }
         }
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+            if (live[k]) wb[x0 + 32 * k] = old[k] + sum[k];
     }
-    const int phys = p.ids[p.indptr[seq] + lb];
-    float* dst = p.w.weights + (static_cast<size_t>(phys) * p.kvh + h) * p.bs + t;
-    *dst = p.w.add && j < start ? *dst + sum : sum;
 }
 
 // ------------------------------------------------------------------ append of bf16 rows
@@ -512,10 +535,7 @@ cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, con
 
 cudaError_t launch_weight_scores(const ScoreWeightParams& p, cudaStream_t st) {
     if (p.w.ntouched <= 0) return cudaSuccess;
-    const int64_t threads = static_cast<int64_t>(p.w.ntouched) * p.kvh * p.bs;
-    const int64_t blocks = (threads + 255) / 256;
-    if (blocks > INT32_MAX) return cudaErrorInvalidValue;
-    weight_scores_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(p);
+    weight_scores_kernel<<<(p.w.ntouched + 7) / 8, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 

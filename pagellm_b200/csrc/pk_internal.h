@@ -255,23 +255,20 @@ struct WeightParams {
     int add;  // add to the weights of tokens cached before the step (else store)
 };
 
-// Weights from the scores that a bounded split-KV launch kept: one thread per (touched block, KV
-// head, token).
+// Weights from the scores that a bounded split-KV launch kept, one warp per touched block.
 struct ScoreWeightParams {
     WeightParams w;
+    const int4* t_meta;     // [ntouched][2] {block id, table index, first and end unit of the sequence},
+                            // {first new position, context, 0, 0}
     const float* score;
     const float2* ml;
-    const int32_t* seq_u;   // [nseq + 1] first unit of each sequence
     const int4* u_meta;     // units as in TcParams
     const int4* u_bound;
-    const int32_t* indptr;
-    const int32_t* ids;
-    const int32_t* starts;
-    const int32_t* offsets;
     int kvh;
     int g;
     int H;
     int bs;
+    int bs_shift;           // log2 of bs, or -1
     int window;
     int sinks;
 };
