@@ -311,9 +311,9 @@ def _aligned(t):
 def _rows(t, device, dtype):
     """``t`` as a contiguous, 16-byte aligned tensor of ``dtype`` on ``device``: itself when it is
     one already (every step of a running model), else a copy."""
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.device != device or not t.is_contiguous():
         t = t.to(device, dtype).contiguous()
-    return _aligned(t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _csr(block_tables):

@@ -246,7 +246,8 @@ struct pk_pool {
     // evict: its tables and items, the kept positions when the caller wants none, and the end
     // of the last call (the next one may come on another stream)
     EvictPlan evict_plan;
-    Uploader evict_up;
+    Uploader evict_up[3];  // in turn: a call need not wait until the last one's copy has run
+    unsigned evict_turn = 0;
     DevBuf evict_kept;
     cudaEvent_t evict_done = nullptr;
 
@@ -833,7 +834,7 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
 // kPiecesPerSlot of them. A piece has at least kMinPieceItems items: it loads the key tile and
 // fills its pipeline first.
 constexpr int64_t kMinPieceItems = 4;
-constexpr int64_t kPiecesPerSlot = 4;
+constexpr int64_t kPiecesPerSlot = 4;  // 1 / 2 / 4 / 8: 262 / 242 / 234 / 242 us for a 2048-token chunk's attention and weights
 void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::vector<int32_t>& tb) {
     pk_pool* P = B->pool;
     struct Tile {
@@ -934,7 +935,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nu = B->total_blocks = B->ncta = B->nsplit = B->ngeneric = 0;
     B->nt = 1;
     int qmax = 0;
-    if (P->tc_ok && g <= pk::kMaxCols) {
+    // (bounded modes know only the layout that one box brings per block)
+    if (P->tc_ok && g <= pk::kMaxCols && !(B->bounded() && P->tc_per_head)) {
         qmax = std::max(1, pk::kMaxCols / g);
         if (P->d == 256) qmax = g <= 8 ? std::max(1, 8 / g) : 0;  // one n8 tile only at D=256
     }
@@ -1887,7 +1889,7 @@ int pk_pool_destroy(pk_pool* pool) {
     if (!pool) return PK_OK;
     DeviceScope ds(pool->device);
     pool->pairs_up.release();
-    pool->evict_up.release();
+    for (Uploader& u : pool->evict_up) u.release();
     pool->evict_kept.release();
     if (pool->evict_done) cudaEventDestroy(pool->evict_done);
     if (pool->weights) cudaFree(pool->weights);
@@ -2024,7 +2026,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
         PK_CUDA(P->evict_kept.reserve(static_cast<size_t>(P->n_layers) * nseq * P->kvh * budget * sizeof(int32_t)));
         kept_dev = static_cast<int32_t*>(P->evict_kept.ptr);
     }
-    Uploader& up = P->evict_up;
+    Uploader& up = P->evict_up[P->evict_turn++ % 3];
     up.begin();
     up.add(plan.indptr.data(), plan.indptr.size() * 4);
     up.add(plan.ids.data(), plan.ids.size() * 4);

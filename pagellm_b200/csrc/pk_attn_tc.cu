@@ -118,6 +118,13 @@ __device__ __forceinline__ void store_rows(float* out, const float (&acc)[D / 16
         }
 }
 
+// 2^x on the special-function unit (flushes denormals; 2^-inf = 0).
+__device__ __forceinline__ float ex2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <int D>
 struct TileGeom {
     static constexpr int kChunks = D / 64;  // 128-byte swizzle rows per token and head
@@ -381,6 +388,12 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
     const int g = p.g;
     const int quad = lane & 3;   // column pair within an n8 tile
     const int grp = lane >> 2;   // row within an 8-row group
+    // Bounded modes: this lane's ldmatrix rows in a stage tile. A head's token rows start at a
+    // multiple of 8 (layout 0), so the swizzle of a row depends on the lane alone: 16-byte unit u of
+    // the lane's row sits at offset (u ^ (lane & 7)) * 16, and addresses are sums of constants.
+    const uint32_t k_row = static_cast<uint32_t>(h * p.bs + (lane & 7) + ((lane >> 3) & 1) * 8) * 128u;
+    const uint32_t v_row = static_cast<uint32_t>(h * p.bs + (lane & 7) + (lane >> 4) * 8) * 128u;
+    const uint32_t chunk_bytes = static_cast<uint32_t>(p.kvh * p.bs) * 128u;
     int it = 0;
     bool alive = true;
     for (int j = lo, u = u_first; j < hi && alive; ++u) {
@@ -584,6 +597,9 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     __syncwarp();
                 }
             }
+            // a block that every live row sees whole needs no masks (what dead columns hold is not used)
+            const bool open = kBounded && kpos0 + p.bs - 1 <= qpos0 &&
+                              (kpos0 > qpos0 + nq - 1 - p.window || kpos0 + p.bs <= p.sinks);
             for (int mtile = 0; mtile < p.bs / 16; ++mtile) {
                 // ---- S^T = K . Q^T
                 float sacc[NT][4];
@@ -597,8 +613,11 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     for (int ks = 0; ks < KS; ++ks) {
                         const int u16 = (ks & 3) * 2 + (lane >> 4);
                         uint32_t a[4];
-                        ldmatrix_x4(a, kst + tile_off(ks >> 2, h, tk, u16, p.kvh, p.bs, CH,
-                                                      p.per_head_layout));
+                        if constexpr (kBounded)
+                            ldmatrix_x4(a, kst + k_row + mtile * 2048u + (ks >> 2) * chunk_bytes + ((u16 ^ (lane & 7)) << 4));
+                        else
+                            ldmatrix_x4(a, kst + tile_off(ks >> 2, h, tk, u16, p.kvh, p.bs, CH,
+                                                          p.per_head_layout));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             mma_bf16_16816(sacc[nt], a, qh[ks][nt][0], qh[ks][nt][1]);
@@ -610,28 +629,89 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 const int kp_a = kpos0 + mtile * 16 + grp;  // rows held: grp and grp + 8
                 const int kp_b = kp_a + 8;
                 uint32_t pb[NT][2];
+                if constexpr (kBounded) {
+                    // The same, all columns side by side: the maxima's shuffles are in flight together,
+                    // one vote decides whether anything is rescaled (rarely, once the maximum has been
+                    // met), and 2^x is the special-function unit's (relative error 2^-22). Column by
+                    // column this took 1350 of a 16-token block's 2800 clocks with two n8 tiles.
+                    float mx[NT][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float xa = sacc[nt][e], xb = sacc[nt][2 + e];
+                            if constexpr (kIo16) {
+                                xa *= p.qscale;
+                                xb *= p.qscale;
+                            }
+                            if (!open) {
+                                const int wlo = lim[nt][e] - p.window;  // keys up to it are past the window
+                                if (!(kp_a <= lim[nt][e] && kp_a < uctx && (kp_a > wlo || kp_a < p.sinks))) xa = -INFINITY;
+                                if (!(kp_b <= lim[nt][e] && kp_b < uctx && (kp_b > wlo || kp_b < p.sinks))) xb = -INFINITY;
+                            }
+                            sacc[nt][e] = xa;
+                            sacc[nt][2 + e] = xb;
+                            mx[nt][e] = fmaxf(xa, xb);
+                        }
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) mx[nt][e] = fmaxf(mx[nt][e], __shfl_xor_sync(0xffffffffu, mx[nt][e], o));
+                    if (score != nullptr) {
+                        // scores for the weights: 8 lanes of a quad column cover 8 keys' rows
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const int c0 = nt * 8 + 2 * quad;
+                            if (c0 >= colp) continue;
+                            float* sp = score + (static_cast<int64_t>(j - ublk0) * p.bs + mtile * 16 + grp) * colp + c0;
+                            *reinterpret_cast<float2*>(sp) = make_float2(sacc[nt][0], sacc[nt][1]);
+                            *reinterpret_cast<float2*>(sp + 8 * colp) = make_float2(sacc[nt][2], sacc[nt][3]);
+                        }
+                    }
+                    bool grows = false;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) grows = grows || mx[nt][e] > m[nt][e];
+                    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float mnew = fmaxf(m[nt][e], mx[nt][e]);
+                                const float corr = ex2_fast(m[nt][e] - (mnew == -INFINITY ? 0.f : mnew));
+                                m[nt][e] = mnew;
+                                l[nt][e] *= corr;
+#pragma unroll
+                                for (int mt = 0; mt < KS; ++mt) {
+                                    acc[mt][nt][e] *= corr;
+                                    acc[mt][nt][2 + e] *= corr;
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float pr[4];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float base = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                            pr[e] = ex2_fast(sacc[nt][e] - base);
+                            pr[2 + e] = ex2_fast(sacc[nt][2 + e] - base);
+                            l[nt][e] += pr[e] + pr[2 + e];
+                        }
+                        pb[nt][0] = movmatrix_trans(pack_bf16(pr[0], pr[1]));
+                        pb[nt][1] = movmatrix_trans(pack_bf16(pr[2], pr[3]));
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < (kBounded ? 0 : NT); ++nt) {
                     float pr[4];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        bool see_a = kp_a <= lim[nt][e] && kp_a < uctx;
-                        bool see_b = kp_b <= lim[nt][e] && kp_b < uctx;
-                        if constexpr (kBounded) {
-                            const int wlo = lim[nt][e] - p.window;  // keys up to it are past the window
-                            see_a = see_a && (kp_a > wlo || kp_a < p.sinks);
-                            see_b = see_b && (kp_b > wlo || kp_b < p.sinks);
-                        }
-                        if constexpr (kIo16) {
-                            sacc[nt][e] *= p.qscale;
-                            sacc[nt][2 + e] *= p.qscale;
-                        }
-                        const float xa = see_a ? sacc[nt][e] : -INFINITY;
-                        const float xb = see_b ? sacc[nt][2 + e] : -INFINITY;
-                        if constexpr (kBounded) {
-                            sacc[nt][e] = xa;
-                            sacc[nt][2 + e] = xb;
-                        }
+                        const float xa = (kp_a <= lim[nt][e] && kp_a < uctx) ? sacc[nt][e] : -INFINITY;
+                        const float xb = (kp_b <= lim[nt][e] && kp_b < uctx) ? sacc[nt][2 + e] : -INFINITY;
                         float mx = fmaxf(xa, xb);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
@@ -651,15 +731,6 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                         pr[e] = pa;
                         pr[2 + e] = pbv;
                     }
-                    if constexpr (kBounded) {
-                        // scores for the weights: 8 lanes of a quad column cover 8 keys' rows
-                        const int c0 = nt * 8 + 2 * quad;
-                        if (score != nullptr && c0 < colp) {
-                            float* sp = score + (static_cast<int64_t>(j - ublk0) * p.bs + mtile * 16 + grp) * colp + c0;
-                            *reinterpret_cast<float2*>(sp) = make_float2(sacc[nt][0], sacc[nt][1]);
-                            *reinterpret_cast<float2*>(sp + 8 * colp) = make_float2(sacc[nt][2], sacc[nt][3]);
-                        }
-                    }
                     // P^T C-fragment rows grp / grp+8 -> B operand (k = token, n = column)
                     pb[nt][0] = movmatrix_trans(pack_bf16(pr[0], pr[1]));
                     pb[nt][1] = movmatrix_trans(pack_bf16(pr[2], pr[3]));
@@ -671,8 +742,11 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     for (int mt = 0; mt < KS; ++mt) {
                         const int u16 = (mt & 3) * 2 + ((lane >> 3) & 1);
                         uint32_t a[4];
-                        ldmatrix_x4_trans(a, vst + tile_off(mt >> 2, h, tv, u16, p.kvh, p.bs, CH,
-                                                            p.per_head_layout));
+                        if constexpr (kBounded)
+                            ldmatrix_x4_trans(a, vst + v_row + mtile * 2048u + (mt >> 2) * chunk_bytes + ((u16 ^ (lane & 7)) << 4));
+                        else
+                            ldmatrix_x4_trans(a, vst + tile_off(mt >> 2, h, tv, u16, p.kvh, p.bs, CH,
+                                                                p.per_head_layout));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma_bf16_16816(acc[mt][nt], a, pb[nt][0], pb[nt][1]);
                     }

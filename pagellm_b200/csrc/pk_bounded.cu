@@ -302,7 +302,7 @@ constexpr int kSelBins = 2048;  // 11-bit digits: sign, exponent and 2 bits firs
 // first) and their weights. Latency bound - n loads, then barriers and passes over shared memory -
 // so everything goes four positions at a time, and few long sequences get 1024 threads each.
 template <int NT>
-__global__ void __launch_bounds__(NT) evict_select_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(const EvictParams p) {
     extern __shared__ float4 vals4[];  // the sequence's weights, when they fit
     constexpr int NW = NT / 32, PER = kSelBins / NT;
     __shared__ int hist[kSelBins];
