@@ -394,7 +394,8 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
     const uint32_t k_row = static_cast<uint32_t>(h * p.bs + (lane & 7) + ((lane >> 3) & 1) * 8) * 128u;
     const uint32_t v_row = static_cast<uint32_t>(h * p.bs + (lane & 7) + (lane >> 4) * 8) * 128u;
     const uint32_t chunk_bytes = static_cast<uint32_t>(p.kvh * p.bs) * 128u;
-    int it = 0;
+    int s = 0;            // ring stage and phase of the next block
+    uint32_t phase = 0u;
     bool alive = true;
     for (int j = lo, u = u_first; j < hi && alive; ++u) {
         const UnitInfo ui = load_unit(p, u);
@@ -475,11 +476,10 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                 for (int i = 0; i < 4; ++i) acc[mt][nt][i] = 0.f;
         }
 
-        for (; j < uend; ++j, ++it) {
-            const int s = it % p.stages;
+        for (; j < uend; ++j, s = s + 1 == p.stages ? 0 : s + 1, phase ^= s == 0 ? 1u : 0u) {
             // Every lane waits; the verdict is made warp-uniform (and the warp reconverged)
             // before the .sync.aligned matrix instructions below.
-            const bool got = mbar_wait_bounded(&vfull[s], static_cast<uint32_t>(it / p.stages) & 1u);
+            const bool got = mbar_wait_bounded(&vfull[s], phase);
             if (!__all_sync(0xffffffffu, got)) {
                 if (lane == 0) {
                     atomicExch(p.err, kErrTimeout);
