@@ -105,7 +105,11 @@ struct Uploader {
         offs.push_back(off);
         return off;
     }
-    int commit(cudaStream_t st) {
+    // by_kernel: small uploads are fetched from the page-locked buffer by a kernel instead of the copy
+    // engine, which a stream of short kernels waits for on both sides (an eviction of 8 short
+    // sequences: 36 us with the engine's copy, 25 us without).
+    static constexpr size_t kKernelBytes = size_t(1) << 20;
+    int commit(cudaStream_t st, bool by_kernel = false) {
         size_t total = parts.empty() ? 0 : offs.back() + parts.back().second;
         if (total == 0) return PK_OK;
         if (!done) PK_CUDA(cudaEventCreateWithFlags(&done, cudaEventDisableTiming));
@@ -113,18 +117,24 @@ struct Uploader {
             PK_CUDA(cudaEventSynchronize(done));
             pending = false;
         }
-        if (total > host_cap) {
+        if (total + 16 > host_cap) {
             if (host) PK_CUDA(cudaFreeHost(host));
             host = nullptr;
             host_cap = 0;
-            size_t want = std::max<size_t>(total + total / 4, 4096);
+            size_t want = std::max<size_t>(total + total / 4 + 16, 4096);
             PK_CUDA(cudaMallocHost(&host, want));
             host_cap = want;
         }
-        PK_CUDA(dev.reserve(total));
+        PK_CUDA(dev.reserve(total + 16));
         for (size_t i = 0; i < parts.size(); ++i)
             if (parts[i].second) std::memcpy(static_cast<char*>(host) + offs[i], parts[i].first, parts[i].second);
-        PK_CUDA(cudaMemcpyAsync(dev.ptr, host, total, cudaMemcpyHostToDevice, st));
+        if (by_kernel && total <= kKernelBytes) {
+            const int64_t floats = static_cast<int64_t>((total + 15) / 16) * 4;  // both buffers are longer
+            PK_CUDA(pk::launch_h2d_gather(static_cast<const float*>(host), static_cast<float*>(dev.ptr), floats, nullptr,
+                                          nullptr, 0, nullptr, nullptr, 0, st));
+        } else {
+            PK_CUDA(cudaMemcpyAsync(dev.ptr, host, total, cudaMemcpyHostToDevice, st));
+        }
         PK_CUDA(cudaEventRecord(done, st));
         pending = true;
         return PK_OK;
@@ -2034,7 +2044,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     up.add(plan.new_ids.data(), plan.new_ids.size() * 4);
     up.add(plan.lengths.data(), plan.lengths.size() * 4);
     up.add(plan.items.data(), plan.items.size() * 4);
-    rc = up.commit(st);
+    rc = up.commit(st, true);
     if (rc != PK_OK) return rc;
     p.pool_k = P->k;
     p.pool_v = P->v;
