@@ -294,6 +294,9 @@ __device__ __forceinline__ uint32_t weight_key(float x) {
 __device__ __forceinline__ int div_by(int x, int d, int shift) { return shift >= 0 ? x >> shift : x / d; }
 
 constexpr int kSelBins = 2048;  // 11-bit digits: sign, exponent and 2 bits first, so heavy tails spread
+// Place of a bin in shared memory: every eighth word is skipped, so that threads which own 8
+// consecutive bins each touch different banks.
+__device__ __forceinline__ int bin_at(int b) { return b + (b >> 3); }
 
 // Which tokens of (layer, sequence, KV head) stay: one CTA each, its weights in shared memory when
 // they fit. The threshold weight - the T-th largest of the middle [sinks, n - recent) - is found
@@ -305,7 +308,7 @@ template <int NT>
 __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(const EvictParams p) {
     extern __shared__ float4 vals4[];  // the sequence's weights, when they fit
     constexpr int NW = NT / 32, PER = kSelBins / NT;
-    __shared__ int hist[kSelBins];
+    __shared__ int hist[kSelBins + kSelBins / 8];
     __shared__ int warp_a[32], warp_b[32];
     __shared__ int sh_digit, sh_rank;
     const int i = blockIdx.x, h = blockIdx.y, layer = blockIdx.z;
@@ -334,8 +337,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
 #pragma unroll 4
         for (int j = 4 * tid; j < n; j += 4 * NT) vals4[j >> 2] = fetch4(j);
     }
-#pragma unroll
-    for (int b = 0; b < PER; ++b) hist[b * NT + tid] = 0;
+    for (int b = tid; b < kSelBins + kSelBins / 8; b += NT) hist[b] = 0;
     __syncthreads();
     auto value4 = [&](int j) { return cached ? vals4[j >> 2] : fetch4(j); };
 
@@ -357,7 +359,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const uint32_t k = weight_key(v[r]);
-                        if (j + r >= lo && j + r < hi && (k & mask) == thr) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+                        if (j + r >= lo && j + r < hi && (k & mask) == thr) atomicAdd(&hist[bin_at((k >> shift) & (bins - 1))], 1);
                     }
                 }
                 __syncthreads();
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
                 int cnt[PER], own = 0;
 #pragma unroll
                 for (int b = 0; b < PER; ++b) {
-                    cnt[b] = hist[kSelBins - 1 - (tid * PER + b)];
+                    cnt[b] = hist[bin_at(kSelBins - 1 - (tid * PER + b))];
                     own += cnt[b];
                 }
                 int scan = own;
@@ -391,7 +393,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
                     }
                 }
 #pragma unroll
-                for (int b = 0; b < PER; ++b) hist[kSelBins - 1 - (tid * PER + b)] = 0;
+                for (int b = 0; b < PER; ++b) hist[bin_at(kSelBins - 1 - (tid * PER + b))] = 0;
                 __syncthreads();
                 thr |= static_cast<uint32_t>(sh_digit) << shift;
                 mask |= static_cast<uint32_t>(bins - 1) << shift;
