@@ -529,7 +529,8 @@ void setup_tc(pk_pool* P) {
     // wide tiles: head_dim 128, 128-key tiles made of whole blocks, the layout-0 view
     std::string why2;
     P->wide_ok = P->d == 128 && pk::kWideKeys % P->block_size == 0 && P->tc_per_head == 0 &&
-                 static_cast<size_t>(optin) >= pk::wide_smem_bytes() && encode_chunk_maps(P, &why2);
+                 static_cast<size_t>(optin) >= std::max(pk::wide_smem_bytes(), pk::chunk_smem_bytes()) &&
+                 encode_chunk_maps(P, &why2);
 }
 
 // log2 of a power of two, else -1
@@ -725,6 +726,7 @@ void plan_shared_prefixes(pk_batch* B, int qmax, int tpt, const std::vector<int>
 // Chunk pair-heads (run beside the split-KV kernel on a second stream) are never cut: one CTA
 // each. Shared-prefix work (after the split-KV kernel) gets all SMs, fewer when shares would
 // be under kWideMinTilesPerCta tiles.
+constexpr int64_t kMinCutTiles = 16;
 void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
     pk_pool* P = B->pool;
     const int kvh = P->kvh;
@@ -822,6 +824,50 @@ void build_wide_schedule(pk_batch* B, int64_t chunk_ctas) {
         }
         return used;
     };
+    if (B->bounded()) {
+        // Chunks of a bounded step, one CTA per SM. Pair-heads stay whole, longest first, each to the
+        // least loaded CTA: cutting some to even 256 pair-heads of 66 tiles over 148 CTAs cost more in
+        // partials than it gained (160 against 154 us). Only where they would leave half of the SMs idle
+        // are their lists cut, into pieces of at least kMinCutTiles tiles.
+        const int nph = B->npair_chunk * kvh;
+        B->ncta_chunk = 0;
+        if (nph > 0) {
+            std::vector<int> order(nph);
+            int64_t W = 0;
+            for (int q = 0; q < nph; ++q) {
+                order[q] = q;
+                W += tiles(q / kvh);
+            }
+            const int64_t cut = std::min<int64_t>(P->num_sms, W / kMinCutTiles);
+            if (2 * nph <= P->num_sms && cut > nph) {
+                B->ncta_chunk = stream_k(0, B->npair_chunk, cut, false);
+            } else {
+                const int64_t G = std::min<int64_t>(P->num_sms, nph);
+                std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return tiles(a / kvh) > tiles(b / kvh); });
+                using LoadCta = std::pair<int64_t, int64_t>;
+                std::priority_queue<LoadCta, std::vector<LoadCta>, std::greater<LoadCta>> heap;
+                for (int64_t c = 0; c < G; ++c) heap.push({0, c});
+                std::vector<std::vector<int>> of(G);
+                for (int q : order) {
+                    LoadCta top = heap.top();
+                    heap.pop();
+                    of[top.second].push_back(q);
+                    top.first += tiles(q / kvh);
+                    heap.push(top);
+                }
+                for (const auto& list : of) {
+                    for (int q : list)
+                        B->seg.insert(B->seg.end(), {q / kvh, q % kvh, 0, static_cast<int32_t>(tiles(q / kvh)), -1, 0});
+                    B->cta_seg.push_back(static_cast<int32_t>(B->seg.size() / 6));
+                }
+                B->ncta_chunk = static_cast<int>(G);
+            }
+        }
+        B->nwsplit_chunk = B->nwsplit = static_cast<int>(B->split.size() / 4);
+        B->ncta_prefix = 0;
+        B->nph = 0;
+        return;
+    }
     int64_t Wc = 0, Wp = 0;
     for (int x = 0; x < B->npair_chunk; ++x) Wc += tiles(x) * kvh;
     for (int x = B->npair_chunk; x < npairs; ++x) Wp += tiles(x) * kvh;
@@ -1574,12 +1620,13 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             PK_CUDA(cudaStreamWaitEvent(B->side, B->ev_fork, 0));
             ws = B->side;
         }
-        wide = wide_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out), 0, 0, nullptr);
+        wide = wide_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out), 0, B->ncta_chunk, nullptr);
         wide.pair_bound = B->plan.at<int4>(30);
         wide.window = p.window;
         wide.sinks = p.sinks;
         wide.sscale = io16 ? p.qscale : 1.f;
         wide.io16 = io16 ? 1 : 0;
+        wide.bs_shift = log2_or_minus(P->block_size);
         wide.ml = B->weights_mode != 0 ? static_cast<float2*>(B->ml_items.ptr) : nullptr;
         const int32_t* wrows = B->plan.at<int32_t>(10);
         const int64_t nw = fused ? static_cast<int64_t>(B->w_rows.size()) : 0;  // chunk rows still to append
@@ -1613,9 +1660,9 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             B->launches++;
         }
         PK_CUDA(prof_begin(B, ws));
-        PK_CUDA(pk::launch_chunk_attention(&P->tmk2, &P->tmv2, &tmq, wide, B->npair_chunk, ws));
+        PK_CUDA(pk::launch_chunk_attention(&P->tmk2, &P->tmv2, &tmq, wide, B->plan.at<int32_t>(20), B->nwsplit_chunk, ws));
         PK_CUDA(prof_end(B, kProfWide, ws));
-        B->launches++;
+        B->launches += B->nwsplit_chunk > 0 ? 2 : 1;
     }
     if (B->use_tc) {
         pk::TcParams t = tc_params(B, layer, H, static_cast<const float*>(q), static_cast<float*>(out));

@@ -7,8 +7,8 @@
 // Work item = 128/g consecutive tokens x the g query heads of one KV head = 128 query rows; two
 // neighbouring items of a sequence make a pair, so that a K/V tile of 64 keys serves 256 rows. A
 // pair lists the key tiles of the sinks in front of its first row's window, then those from the
-// window on (PairBound): tiles that nobody sees are neither read nor computed. One CTA per (pair,
-// KV head), pairs with the most keys first.
+// window on: tiles that nobody sees are neither read nor computed. The (pair, KV head)s are dealt to
+// one CTA per SM, whole where that balances, else cut (build_chunk_schedule).
 
 #include "pk_device.cuh"
 #include "pk_internal.h"
@@ -25,14 +25,22 @@ constexpr int kTile = kRows * kDim * 2;  // 32 KB: 128 query rows or keys, [64-d
 constexpr uint32_t kIdescS = idesc_bf16(kKeys, false);
 constexpr uint32_t kIdescO = idesc_bf16(kDim, true);
 
-// What a pair reads: entry jt of its tile list is key tile jt, and jt + skip from jt = head on;
-// lo = first key of the window of its first row.
-struct PairBound {
-    int head, skip, lo, ntiles;
+// A CTA's work item: entries [t0, t1) of a pair's tile list for one KV head. Entry jt is key tile
+// jt, and jt + skip from jt = head on; lo = first key of the window of the pair's first row. slot:
+// where the partial goes when the list is cut between CTAs, or -1.
+struct Segment {
+    int pair, kvhead, t0, t1, slot;
+    int head, skip, lo;
+    __device__ __forceinline__ int tile(int jt) const { return jt >= head ? jt + skip : jt; }
 };
-__device__ __forceinline__ PairBound load_pair(const int4* p, int pair) {
-    const int4 b = __ldg(p + pair);
-    return PairBound{b.x, b.y, b.z, b.w};
+__device__ __forceinline__ Segment load_segment(const WideParams& p, int i) {
+    const int32_t* e = p.seg + 6 * i;
+    Segment s{e[0], e[1], e[2], e[3], e[4], 0, 0, 0};
+    const int4 b = __ldg(p.pair_bound + s.pair);
+    s.head = b.x;
+    s.skip = b.y;
+    s.lo = b.z;
+    return s;
 }
 
 // One tile of 128 keys of KV head `head` (key tile kt of a table of nblk blocks): its block ids as
@@ -69,30 +77,34 @@ __device__ __forceinline__ void load_query_tile(const CUtensorMap* tmq, uint8_t*
 }
 
 // ---------------------------------------------------------------- attention
-// Warps: 0 producer (K and V rings of 64-key tiles, TMA), 1 and 2 MMA issuers of query tile 0 and 1
-// (1 owns the TMEM), then 4 softmax warps per query tile, thread = row. Per tile of 64 keys: S_t = Q_t.K^T (M=128 N=64 K=128) into
-// TMEM; a row's 64 scores are read and S_t is given back at once, so that the next S_t is computed
-// while this one's exponentials run; P_t (bf16) goes to columns of its own and O_t += P_t.V
-// (M=128 N=128 K=64, A from TMEM).
+// One CTA per SM walks a list of segments. Warps: 0 and 1 producers (rings of 64-key K and V tiles and
+// the next segment's queries, TMA), 2 and 3 MMA issuers of query tile 0 and 1 (2 owns the TMEM), then 4
+// softmax warps per query tile, thread = row. Per tile of 64 keys: S_t = Q_t.K^T (M=128 N=64 K=128)
+// into TMEM; a row's 64 scores are read and S_t is given back at once, so that the next S_t is
+// computed while this one's exponentials run; P_t (bf16) goes to columns of its own and
+// O_t += P_t.V (M=128 N=128 K=64, A from TMEM). At the end of a segment the next one's queries, keys
+// and first S_t are under way while O_t is written out.
 // Why 64 keys: with 128, S, P and O of two query tiles do not fit the 512 TMEM columns side by side,
-// P has to lie on S, and each tile runs as one chain softmax -> P.V -> next S. Traced on the B200
-// that chain took 4400 clocks per 128 keys (2250 softmax, 340 hand-over, 690 + 750 the two
-// products, 250 back) with the exponential unit and the tensor cores each half idle, and neither
-// twice the softmax warps nor faster copies moved it. An M=128 N=64 product costs three quarters of
-// an N=128 one (its A operand fills the shared-memory port), which the overlap more than repays.
+// P has to lie on S, and each tile runs as one chain softmax -> P.V -> next S. Traced on the B200,
+// clocks per 128 keys of 256 rows: 4400 in that form (2250 softmax, 340 hand-over, 690 + 750 the two
+// products, 250 back), with the exponential unit (2048 at least) and the tensor cores (2140) each half
+// idle; twice the softmax warps, faster copies or two issuers did not move it. Here 3800, bound by the
+// products: an M=128 N=64 one costs 51 clocks against an N=128 one's 67, because its A operand fills
+// the shared-memory port. One CTA per (pair, KV head) instead of a list cost 14 us each.
+constexpr int kTurnAfter = 16;  // pairs of exponentials after which the other tile may start its own (4 to 24: within 1 %)
 constexpr int kCKeys = kChunkKeys;  // 64
 constexpr int kCKvTile = kCKeys * kDim * 2;  // 16 KB, [64-dim chunk][key][64]
-constexpr int kTurnAfter = 16;  // pairs of exponentials after which the other tile may start its own (4 to 24: within 1 %)
 constexpr int kCStages = 4;
-constexpr int kCThreads = 32 * 3 + 2 * 128;
+constexpr int kCThreads = 32 * 4 + 2 * 128;
 constexpr uint32_t kColP = 2 * kCKeys;  // TMEM: S_0, S_1 (64 columns each), P_0, P_1 (32 each), O_0, O_1
 constexpr uint32_t kColO = 256;
 constexpr uint32_t kIdescS64 = idesc_bf16(kCKeys, false);
 constexpr int kCOffQ = 0;
 constexpr int kCOffK = kCOffQ + 2 * kTile;
 constexpr int kCOffV = kCOffK + kCStages * kCKvTile;
-constexpr int kCOffBar = kCOffV + kCStages * kCKvTile;
-constexpr int kCSmem = kCOffBar + 256 + 1024;
+constexpr int kCOffStage = kCOffV + kCStages * kCKvTile;  // 4 KB per softmax warp for O on its way out
+constexpr int kCOffBar = kCOffStage + 8 * 4096;
+constexpr int kCSmem = kCOffBar + 384 + 1024;
 
 template <bool IO16>
 __global__ void __launch_bounds__(kCThreads, 1)
@@ -104,19 +116,19 @@ __global__ void __launch_bounds__(kCThreads, 1)
     uint64_t* kempty = kfull + kCStages;  // two arrivals: S of both query tiles
     uint64_t* vfull = kempty + kCStages;
     uint64_t* vempty = vfull + kCStages;  // two arrivals: P.V of both
-    uint64_t* qfull = vempty + kCStages;  // [tile]
-    uint64_t* sfull = qfull + 2;          // [tile]
+    uint64_t* qfull = vempty + kCStages;  // [tile], per segment
+    uint64_t* qempty = qfull + 2;         // [tile], per segment: its S are done with Q
+    uint64_t* sfull = qempty + 2;         // [tile], per key tile, as the next three
     uint64_t* sfree = sfull + 2;          // [tile], one arrival per softmax warp
     uint64_t* pfull = sfree + 2;          // [tile], one arrival per softmax warp
     uint64_t* pvdone = pfull + 2;         // [tile]
-    uint64_t* turn = pvdone + 2;          // [tile][quadrant]: the tile's warp may take its exponentials
+    uint64_t* ofree = pvdone + 2;         // [tile], per segment, one arrival per softmax warp: O has been read
+    uint64_t* turn = ofree + 2;           // [tile][quadrant]: the tile's warp may take its exponentials
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int pair = blockIdx.x / p.kvh, head = blockIdx.x % p.kvh;
-    const PairBound pb = load_pair(p.pair_bound, pair);
-    const int nt = pb.ntiles;
+    const int s_begin = p.cta_seg[blockIdx.x], s_end = p.cta_seg[blockIdx.x + 1];
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kCStages; ++s) {
@@ -127,16 +139,18 @@ __global__ void __launch_bounds__(kCThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&qfull[t], 1);
+            mbar_init(&qempty[t], 1);
             mbar_init(&sfull[t], 1);
             mbar_init(&sfree[t], 4);
             mbar_init(&pfull[t], 4);
             mbar_init(&pvdone[t], 1);
+            mbar_init(&ofree[t], 4);
             for (int q = 0; q < 4; ++q) mbar_init(&turn[4 * t + q], 1);
         }
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 1) {
+    if (warp == 2) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -145,79 +159,91 @@ __global__ void __launch_bounds__(kCThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const uint32_t smem_base = smem_u32(smem);
+    auto ph = [](int n) { return static_cast<uint32_t>(n / kCStages) & 1u; };
 
-    if (warp == 0) {
-        // Lanes 0-15 load K tiles, lanes 16-31 V tiles: lane (part b, chunk c) of a tile knows its
-        // next block id before the slot is free, so that a tile's copies leave at once. A part is a
-        // block, or 64 keys of a larger one.
-        const bool is_v = lane >= 16;
-        const int cb = (lane & 15) >> 1, cc = lane & 1;
-        const int part = min(p.bs, kCKeys), parts = kCKeys / part;
-        const bool mine = cb < parts;
-        if (lane == 0) {
-            prefetch_tensormap(&tmk);
-            prefetch_tensormap(&tmv);
-            for (int t = 0; t < 2; ++t) {
-                const int item = p.w_pair[2 * pair + t];
-                if (item >= 0) {
-                    mbar_arrive_expect_tx(&qfull[t], kTile);
-                    load_query_tile<IO16>(&tmq, smem + kCOffQ + t * kTile, &qfull[t], p, item, head);
-                } else {
-                    mbar_arrive(&qfull[t]);  // no second item: whatever is there, its rows are dead
-                }
-            }
-        }
-        const int seq = p.w_seq[p.w_pair[2 * pair]];
-        const int32_t* tbl = p.ids + p.indptr[seq];
-        const int nblk = p.indptr[seq + 1] - p.indptr[seq];
-        // first slot of this lane's part of entry n of the tile list (past the table's end: its last
-        // block, masked)
-        auto slot_of = [&](int n) {
-            if (!mine) return 0;
-            const int key = (n >= pb.head ? n + pb.skip : n) * kCKeys + cb * part;
-            const int blk = min(key / p.bs, nblk - 1);
-            return static_cast<int>(p.layer_slot0 + static_cast<int64_t>(__ldg(tbl + blk)) * p.bs + key % p.bs);
-        };
+    if (warp <= 1) {
+        // ---- producers: warp 0 K tiles and queries, warp 1 V tiles. Lane b knows the first slot of part
+        // b of the next tile (a block, or 64 keys of a larger one) before the ring has room for it, and
+        // one lane issues the tile's copies: from 16 lanes of one warp, K and V together, they took 1300
+        // clocks a tile and were what the whole kernel waited for.
+        const bool is_v = warp == 1;
+        const int part = min(p.bs, kCKeys), parts = kCKeys / part;  // at most 4
         const CUtensorMap* map = is_v ? &tmv : &tmk;
-        uint8_t* dst = smem + (is_v ? kCOffV : kCOffK) + cc * (kCKeys * 128) + cb * part * 128;
+        uint8_t* ring = smem + (is_v ? kCOffV : kCOffK);
         uint64_t* full = is_v ? vfull : kfull;
         uint64_t* empty = is_v ? vempty : kempty;
-        int n = 0, slot = slot_of(0);  // this half's next tile
-        unsigned long long idle_since = global_ns();
-        while (__any_sync(0xffffffffu, n < nt)) {
-            const bool go = n < nt && mbar_test_wait(&empty[n % kCStages], ((n / kCStages) & 1u) ^ 1u);
-            // the half's lanes go together
-            const unsigned votes = __ballot_sync(0xffffffffu, go);
-            const unsigned half_mask = is_v ? 0xFFFF0000u : 0x0000FFFFu;
-            const bool all = (votes & half_mask) == half_mask;
-            if (all && (lane & 15) == 0) mbar_arrive_expect_tx(&full[n % kCStages], kCKvTile);
-            __syncwarp();
-            if (all) {
-                if (mine) tma_load_4d(dst + (n % kCStages) * kCKvTile, map, 0, slot, head, cc, &full[n % kCStages]);
-                if (++n < nt) slot = slot_of(n);
-            }
-            if ((votes & 0xFFFFu) == 0xFFFFu || (votes >> 16) == 0xFFFFu) {
-                idle_since = global_ns();
-            } else {
-                const bool give_up = __any_sync(0xffffffffu, *abort_flag || global_ns() - idle_since > kWaitLimitNs);
-                if (give_up) {
-                    if (lane == 0) {
-                        *abort_flag = 1;
-                        atomicExch(p.err, kErrTimeout);
+        if (lane == 0) prefetch_tensormap(map);
+        bool ok = true;
+        int n = 0, nq = 0;
+        for (int si = s_begin; si < s_end && ok; ++si) {
+            const Segment sg = load_segment(p, si);
+            const int seq = p.w_seq[p.w_pair[2 * sg.pair]];
+            const int32_t* tbl = p.ids + p.indptr[seq];
+            const int nblk = p.indptr[seq + 1] - p.indptr[seq];
+            // past the table's end: its last block, masked
+            auto slot_of = [&](int jt) {
+                const int key = sg.tile(jt) * kCKeys + (lane & 3) * part;
+                const int blk = min(key >> p.bs_shift, nblk - 1);
+                return static_cast<int>(p.layer_slot0 + static_cast<int64_t>(__ldg(tbl + blk)) * p.bs + (key & (p.bs - 1)));
+            };
+            int slot = slot_of(sg.t0);
+            for (int jt = sg.t0; jt < sg.t1; ++jt, ++n) {
+                ok = __all_sync(0xffffffffu, mbar_wait_fast(&empty[n % kCStages], ph(n) ^ 1u));
+                if (!ok) break;
+                int part_slot[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) part_slot[b] = __shfl_sync(0xffffffffu, slot, b);
+                uint8_t* dst = ring + (n % kCStages) * kCKvTile;
+                uint64_t* bar = &full[n % kCStages];
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar, kCKvTile);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        if (b < parts) {
+                            tma_load_4d(dst + b * part * 128, map, 0, part_slot[b], sg.kvhead, 0, bar);
+                            tma_load_4d(dst + b * part * 128 + kCKeys * 128, map, 0, part_slot[b], sg.kvhead, 1, bar);
+                        }
+                }
+                __syncwarp();
+                if (jt + 1 < sg.t1) slot = slot_of(jt + 1);
+                if (!is_v && jt == sg.t0) {
+                    // the segment's queries, once the last one's S are done with theirs
+                    if (nq > 0) {
+                        const uint32_t par = static_cast<uint32_t>((nq - 1) & 1);
+                        ok = __all_sync(0xffffffffu, mbar_wait_fast(&qempty[0], par, &qempty[1], par));
+                        if (!ok) break;
                     }
-                    break;
+                    if (lane == 0) {
+                        for (int t = 0; t < 2; ++t) {
+                            const int item = p.w_pair[2 * sg.pair + t];
+                            if (item >= 0) {
+                                mbar_arrive_expect_tx(&qfull[t], kTile);
+                                load_query_tile<IO16>(&tmq, smem + kCOffQ + t * kTile, &qfull[t], p, item, sg.kvhead);
+                            } else {
+                                mbar_arrive(&qfull[t]);  // no second item: whatever is there, its rows are dead
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    ++nq;
                 }
             }
         }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            atomicExch(p.err, kErrTimeout);
+        }
         // never leave the CTA with copies still landing in its shared memory
-        if (lane == 0)
-            for (int t = 0; t < 2; ++t) mbar_wait_bounded(&qfull[t], 0u);
-        if ((lane & 15) == 0)
+        if (lane == 0) {
+            if (nq > 0)
+                for (int t = 0; t < 2; ++t) mbar_wait_bounded(&qfull[t], static_cast<uint32_t>((nq - 1) & 1));
             for (int t = max(0, n - kCStages); t < n; ++t)
                 mbar_wait_bounded(&full[t % kCStages], static_cast<uint32_t>(t / kCStages) & 1u);
-    } else if (warp <= 2) {
-        // one issuer per query tile: S(n + 1) once the scores of n have been read, P.V(n) once P is there
-        const int t = warp - 1;
+        }
+    } else if (warp <= 3) {
+        // ---- one issuer per query tile: S(n + 1) once the scores of n have been read, P.V(n) once P is
+        // there; n counts the CTA's key tiles
+        const int t = warp - 2;
         const uint64_t qd0 = smem_desc(smem_base + kCOffQ + t * kTile, 16, 1024);
         const uint64_t kd0 = smem_desc(smem_base + kCOffK, 16, 1024);
         const uint64_t vd0 = smem_desc(smem_base + kCOffV, kCKeys * 128, 1024);
@@ -227,8 +253,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
             ok = __all_sync(0xffffffffu, mbar_wait_fast(bar_a, parity_a, bar_b, parity_b));
             return ok;
         };
-        auto ph = [](int n) { return static_cast<uint32_t>(n / kCStages) & 1u; };
-        auto issue_s = [&](int n) {
+        auto issue_s = [&](int n, bool last) {  // last: the segment's, after which Q is free
             tc_fence_after();
             const uint64_t kd = kd0 + ((n % kCStages) * (kCKvTile >> 4));
             if (elect_one()) {
@@ -238,173 +263,206 @@ __global__ void __launch_bounds__(kCThreads, 1)
                               kd + (((kk >> 2) * (kCKeys * 128) + (kk & 3) * 32) >> 4), kIdescS64, kk > 0 ? 1u : 0u);
                 umma_commit(&sfull[t]);
                 umma_commit(&kempty[n % kCStages]);
+                if (last) umma_commit(&qempty[t]);
             }
             __syncwarp();
         };
-        if (wait(&qfull[t], 0u, &kfull[0], 0u)) issue_s(0);
-        for (int n = 0; n < nt && ok; ++n) {
-            if (n + 1 < nt) {
-                if (!wait(&kfull[(n + 1) % kCStages], ph(n + 1), &sfree[t], static_cast<uint32_t>(n & 1))) break;
-                issue_s(n + 1);
-            }
-            if (!wait(&vfull[n % kCStages], ph(n), &pfull[t], static_cast<uint32_t>(n & 1))) break;
-            tc_fence_after();
-            const uint64_t vd = vd0 + ((n % kCStages) * (kCKvTile >> 4));
-            if (elect_one()) {
+        int n = 0;
+        for (int si = s_begin; si < s_end && ok; ++si) {
+            const Segment sg = load_segment(p, si);
+            const int k = si - s_begin, nt = sg.t1 - sg.t0;
+            if (!wait(&qfull[t], static_cast<uint32_t>(k & 1), &kfull[n % kCStages], ph(n))) break;
+            if (n > 0 && !wait(&sfree[t], static_cast<uint32_t>((n - 1) & 1), &sfree[t], static_cast<uint32_t>((n - 1) & 1))) break;
+            issue_s(n, nt == 1);
+            for (int i = 0; i < nt; ++i, ++n) {
+                if (i + 1 < nt) {
+                    if (!wait(&kfull[(n + 1) % kCStages], ph(n + 1), &sfree[t], static_cast<uint32_t>(n & 1))) break;
+                    issue_s(n + 1, i + 2 == nt);
+                }
+                if (!wait(&vfull[n % kCStages], ph(n), &pfull[t], static_cast<uint32_t>(n & 1))) break;
+                // the first P.V of a segment overwrites the last one's O
+                if (i == 0 && k > 0 && !wait(&ofree[t], static_cast<uint32_t>((k - 1) & 1), &ofree[t], static_cast<uint32_t>((k - 1) & 1)))
+                    break;
+                tc_fence_after();
+                const uint64_t vd = vd0 + ((n % kCStages) * (kCKvTile >> 4));
+                if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < kCKeys / 16; ++kk)
-                    umma_bf16_ts(tO, tP + kk * 8, vd + ((kk * 16 * 128) >> 4), kIdescO, (n > 0 || kk > 0) ? 1u : 0u);
-                umma_commit(&pvdone[t]);
-                umma_commit(&vempty[n % kCStages]);
+                    for (int kk = 0; kk < kCKeys / 16; ++kk)
+                        umma_bf16_ts(tO, tP + kk * 8, vd + ((kk * 16 * 128) >> 4), kIdescO, (i > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&pvdone[t]);
+                    umma_commit(&vempty[n % kCStages]);
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
             atomicExch(p.err, kErrTimeout);
         }
     } else {
-        const int tile = (warp - 3) >> 2;
+        const int tile = (warp - 4) >> 2;
         const int q4 = warp & 3;  // TMEM lanes 32 * q4 .. + 31
         const int r = 32 * q4 + lane;
         const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
         const uint32_t tS = trow + tile * kCKeys;
         const uint32_t tP = trow + kColP + tile * (kCKeys / 2);
         const uint32_t tO = trow + kColO + tile * kDim;
-        const int item = p.w_pair[2 * pair + tile];
-        const int ntok = item >= 0 ? p.w_ntok[item] : 0;
-        const int tok0 = item >= 0 ? p.w_tok0[item] : 0;
-        const int t_row = r / p.g;
-        const bool live = t_row < ntok;
-        const int kv_end = p.pair_kend[pair];
-        const int last_tile = (kv_end - 1) / kCKeys;
-        const int qlim = live ? p.tok_pos[tok0] + t_row : -1;  // last key of the row; consecutive tokens
-        const int qlo = live ? qlim - p.window : -1;           // keys up to it and not among the sinks are past the window
-        const size_t oidx = static_cast<size_t>(p.tok_row[tok0] + (live ? t_row : 0)) * p.H + head * p.g + r % p.g;
         const uint64_t scale2 = pack_f32x2(p.sscale, p.sscale);
-        float m = -INFINITY, l = 0.f;
+        float* stg = reinterpret_cast<float*>(smem + kCOffStage + (tile * 4 + q4) * 4096);
+        auto stg4 = [&](int row, int i) { return reinterpret_cast<float4*>(stg + row * 32 + 4 * (i ^ (row & 7))); };
+        const int t_row = r / p.g;
         bool ok = true;
-        for (int n = 0; n < nt; ++n) {
-            const int k0 = (n >= pb.head ? n + pb.skip : n) * kCKeys;
-            ok = __all_sync(0xffffffffu, mbar_wait_fast(&sfull[tile], static_cast<uint32_t>(n & 1)));
-            if (!ok) break;
-            tc_fence_after();
-            float sv[kCKeys];
-            tmem_ld32(tS, sv);
-            tmem_ld32(tS + 32, sv + 32);
-            tmem_wait_ld();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sfree[tile]);
-            if (k0 + kCKeys - 1 > qlim || (k0 <= qlo && k0 + kCKeys > p.sinks)) {
-#pragma unroll
-                for (int i = 0; i < kCKeys; ++i)
-                    if (k0 + i > qlim || (k0 + i <= qlo && k0 + i >= p.sinks)) sv[i] = -INFINITY;
-            }
-            float mx8[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                mx8[k] = sv[k];
-#pragma unroll
-                for (int i = k + 8; i < kCKeys; i += 8) mx8[k] = fmaxf(mx8[k], sv[i]);
-            }
-            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                   fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * p.sscale;
-            // Lazy rescale: the base of earlier tiles stays unless this tile's maximum exceeds it by
-            // more than 8 (P stays <= 2^8 in bf16, l and O in fp32).
-            const float mnew = (m == -INFINITY || mx > m + 8.f) ? mx : m;
-            const float base = mnew == -INFINITY ? 0.f : mnew;
-            const float corr = m == -INFINITY ? 0.f : ex2_approx(m - base);
-            const uint64_t base2 = pack_f32x2(-base, -base);
-            // The two tiles' warps of an SM sub-partition take turns at its exponential unit: left
-            // alone they fall into step, both in exponentials or both between them (measured: 2240
-            // clocks per 64 keys of 256 rows).
-            if (tile == 1 || n > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait_fast(&turn[4 * tile + q4], static_cast<uint32_t>((tile == 1 ? n : n - 1) & 1)));
-                if (!ok) break;
-            }
-            uint64_t s2[4] = {0, 0, 0, 0};  // the row sum, two lanes and four chains
-            uint32_t pk[kCKeys / 2];
-#pragma unroll
-            for (int i = 0; i < kCKeys / 2; ++i) {
-                float a, b;
-                unpack_f32x2(fma_f32x2(pack_f32x2(sv[2 * i], sv[2 * i + 1]), scale2, base2), a, b);
-                a = ex2_approx(a);
-                b = ex2_approx(b);
-                s2[i & 3] = add_f32x2(s2[i & 3], pack_f32x2(a, b));
-                pk[i] = pack_bf16(a, b);
-                // the other tile's turn; the (always true) condition on what has been summed keeps the
-                // exponentials before it from being scheduled behind it
-                if (i == kTurnAfter - 1) {
-                    float x, y;
-                    unpack_f32x2(add_f32x2(add_f32x2(s2[0], s2[1]), add_f32x2(s2[2], s2[3])), x, y);
-                    if (__any_sync(0xffffffffu, !(x + y < 0.f)) && lane == 0) mbar_arrive(&turn[4 * (tile ^ 1) + q4]);
-                }
-            }
-            float a, b;
-            unpack_f32x2(add_f32x2(add_f32x2(s2[0], s2[1]), add_f32x2(s2[2], s2[3])), a, b);
-            l = l * corr + (a + b);
-            m = mnew;
-            // P.V of the previous tile is done with P's columns (and with O, should it be rescaled)
-            if (n > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait_fast(&pvdone[tile], static_cast<uint32_t>((n - 1) & 1)));
+        int n = 0;  // the CTA's key tiles so far
+        for (int si = s_begin; si < s_end && ok; ++si) {
+            const Segment sg = load_segment(p, si);
+            const int item = p.w_pair[2 * sg.pair + tile];
+            const int ntok = item >= 0 ? p.w_ntok[item] : 0;
+            const int tok0 = item >= 0 ? p.w_tok0[item] : 0;
+            const bool live = t_row < ntok;
+            const int kv_end = p.pair_kend[sg.pair];
+            const int last_tile = (kv_end - 1) / kCKeys;
+            const int qlim = live ? p.tok_pos[tok0] + t_row : -1;  // last key of the row; consecutive tokens
+            const int qlo = live ? qlim - p.window : -1;  // keys up to it and not among the sinks are past the window
+            const size_t oidx = static_cast<size_t>(p.tok_row[tok0] + (live ? t_row : 0)) * p.H + sg.kvhead * p.g + r % p.g;
+            float m = -INFINITY, l = 0.f;
+            for (int jt = sg.t0; jt < sg.t1; ++jt, ++n) {
+                const bool first = jt == sg.t0;
+                const int k0 = sg.tile(jt) * kCKeys;
+                ok = __all_sync(0xffffffffu, mbar_wait_fast(&sfull[tile], static_cast<uint32_t>(n & 1)));
                 if (!ok) break;
                 tc_fence_after();
-            }
-            tmem_st32u(tP, pk);
-            if (n > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-#pragma unroll 1
-                for (int c = 0; c < kDim / 32; ++c) {
-                    float o[32];
-                    tmem_ld32(tO + c * 32, o);
-                    tmem_wait_ld();
+                float sv[kCKeys];
+                tmem_ld32(tS, sv);
+                tmem_ld32(tS + 32, sv + 32);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfree[tile]);
+                if (k0 + kCKeys - 1 > qlim || (k0 <= qlo && k0 + kCKeys > p.sinks)) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] *= corr;
-                    tmem_st32(tO + c * 32, o);
+                    for (int i = 0; i < kCKeys; ++i)
+                        if (k0 + i > qlim || (k0 + i <= qlo && k0 + i >= p.sinks)) sv[i] = -INFINITY;
                 }
-            }
-            tmem_wait_st();
-            // V rows that no row of the pair sees - past the context in the last tile, or between the
-            // sinks and the first row's window - are zeroed so that P = 0 meets 0. Each query tile
-            // does it for its own product: the two are issued in either order.
-            const int za = max(0, p.sinks - k0), zb = min(kCKeys, pb.lo - k0);
-            const bool tail = k0 == last_tile * kCKeys && kv_end < k0 + kCKeys;
-            if (tail || za < zb) {
-                const int s = n % kCStages;
-                ok = __all_sync(0xffffffffu, mbar_wait_fast(&vfull[s], static_cast<uint32_t>(n / kCStages) & 1u));
-                if (!ok) break;
-                uint8_t* vd = smem + kCOffV + s * kCKvTile;
-                auto zero_rows = [&](int first, int end) {
-                    for (int x = (threadIdx.x - 96) & 127; x < (end - first) * 16; x += 128) {
-                        const int key = first + x / 16;
-                        *reinterpret_cast<uint4*>(vd + ((x / 8) & 1) * (kCKeys * 128) + sw128(key, x & 7)) = make_uint4(0, 0, 0, 0);
+                float mx8[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    mx8[k] = sv[k];
+#pragma unroll
+                    for (int i = k + 8; i < kCKeys; i += 8) mx8[k] = fmaxf(mx8[k], sv[i]);
+                }
+                const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * p.sscale;
+                // Lazy rescale: the base of earlier tiles stays unless this tile's maximum exceeds it by
+                // more than 8 (P stays <= 2^8 in bf16, l and O in fp32).
+                const float mnew = (m == -INFINITY || mx > m + 8.f) ? mx : m;
+                const float base = mnew == -INFINITY ? 0.f : mnew;
+                const float corr = m == -INFINITY ? 0.f : ex2_approx(m - base);
+                const uint64_t base2 = pack_f32x2(-base, -base);
+                // The two tiles' warps of an SM sub-partition take turns at its exponential unit: left
+                // alone they fall into step, both in exponentials or both between them (measured: 2240
+                // clocks per 64 keys of 256 rows).
+                if (tile == 1 || n > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_fast(&turn[4 * tile + q4], static_cast<uint32_t>((tile == 1 ? n : n - 1) & 1)));
+                    if (!ok) break;
+                }
+                uint64_t s2[4] = {0, 0, 0, 0};  // the row sum, two lanes and four chains
+                uint32_t pk[kCKeys / 2];
+#pragma unroll
+                for (int i = 0; i < kCKeys / 2; ++i) {
+                    float a, b;
+                    unpack_f32x2(fma_f32x2(pack_f32x2(sv[2 * i], sv[2 * i + 1]), scale2, base2), a, b);
+                    a = ex2_approx(a);
+                    b = ex2_approx(b);
+                    s2[i & 3] = add_f32x2(s2[i & 3], pack_f32x2(a, b));
+                    pk[i] = pack_bf16(a, b);
+                    // the other tile's turn; the (always true) condition on what has been summed keeps the
+                    // exponentials before it from being scheduled behind it
+                    if (i == kTurnAfter - 1) {
+                        float x, y;
+                        unpack_f32x2(add_f32x2(add_f32x2(s2[0], s2[1]), add_f32x2(s2[2], s2[3])), x, y);
+                        if (__any_sync(0xffffffffu, !(x + y < 0.f)) && lane == 0) mbar_arrive(&turn[4 * (tile ^ 1) + q4]);
                     }
-                };
-                if (tail) zero_rows(kv_end - k0, kCKeys);
-                if (za < zb) zero_rows(za, zb);
-                fence_proxy_async_smem();  // the zeros (generic writes) before the MMA reads them
+                }
+                float a, b;
+                unpack_f32x2(add_f32x2(add_f32x2(s2[0], s2[1]), add_f32x2(s2[2], s2[3])), a, b);
+                l = l * corr + (a + b);
+                m = mnew;
+                // P.V of the previous tile is done with P's columns (and with O, should it be rescaled)
+                if (!first) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_fast(&pvdone[tile], static_cast<uint32_t>((n - 1) & 1)));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                tmem_st32u(tP, pk);
+                if (!first && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+                    for (int c = 0; c < kDim / 32; ++c) {
+                        float o[32];
+                        tmem_ld32(tO + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] *= corr;
+                        tmem_st32(tO + c * 32, o);
+                    }
+                }
+                tmem_wait_st();
+                // V rows that no row of the pair sees - past the context in the last tile, or between the
+                // sinks and the first row's window - are zeroed so that P = 0 meets 0. Each query tile
+                // does it for its own product: the two are issued in either order.
+                const int za = max(0, p.sinks - k0), zb = min(kCKeys, sg.lo - k0);
+                const bool tail = k0 == last_tile * kCKeys && kv_end < k0 + kCKeys;
+                if (tail || za < zb) {
+                    const int s = n % kCStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait_fast(&vfull[s], ph(n)));
+                    if (!ok) break;
+                    uint8_t* vd = smem + kCOffV + s * kCKvTile;
+                    auto zero_rows = [&](int from, int end) {
+                        for (int x = threadIdx.x & 127; x < (end - from) * 16; x += 128) {
+                            const int key = from + x / 16;
+                            *reinterpret_cast<uint4*>(vd + ((x / 8) & 1) * (kCKeys * 128) + sw128(key, x & 7)) = make_uint4(0, 0, 0, 0);
+                        }
+                    };
+                    if (tail) zero_rows(kv_end - k0, kCKeys);
+                    if (za < zb) zero_rows(za, zb);
+                    fence_proxy_async_smem();  // the zeros (generic writes) before the MMA reads them
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[tile]);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[tile]);
-        }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait_fast(&pvdone[tile], static_cast<uint32_t>((nt - 1) & 1)));
-        if (ok) {
-            // ---- epilogue: O / l. Rows leave TMEM one per thread, 32 columns at a time, and go to
-            // global memory through 4 KB of the tile's Q buffer (its S MMAs are done), so that a store
-            // covers pieces of 4 rows; float4 slot i of staging row r sits at i ^ (r & 7): conflict-free.
+            if (ok) ok = __all_sync(0xffffffffu, mbar_wait_fast(&pvdone[tile], static_cast<uint32_t>((n - 1) & 1)));
+            if (!ok) break;
+            // ---- the segment's rows: O / l, or, where the pair's list is cut, O as it is with (m, l). They
+            // leave TMEM one per thread, 32 columns at a time, and go to global memory through the warp's
+            // staging area, so that a store covers pieces of 4 rows; float4 slot i of staging row r sits
+            // at i ^ (r & 7): conflict-free.
             tc_fence_after();
-            const float wo = live ? 1.f / l : 0.f;
-            if (p.ml != nullptr && item >= 0)
-                p.ml[(static_cast<size_t>(item) * p.kvh + head) * kRows + r] = live ? make_float2(m, wo) : make_float2(0.f, 0.f);
-            float* stg = reinterpret_cast<float*>(smem + kCOffQ + tile * kTile + q4 * 4096);
-            auto stg4 = [&](int row, int i) { return reinterpret_cast<float4*>(stg + row * 32 + 4 * (i ^ (row & 7))); };
+            const bool whole = sg.slot < 0;
+            const float wo = whole ? (live ? 1.f / l : 0.f) : 1.f;
+            const size_t prow = (static_cast<size_t>(whole ? 0 : sg.slot) * 2 + tile) * kRows;
+            if (!whole) {
+                p.part_ml[(prow + r) * 2] = m;
+                p.part_ml[(prow + r) * 2 + 1] = l;
+            } else if (p.ml != nullptr && item >= 0) {
+                p.ml[(static_cast<size_t>(item) * p.kvh + sg.kvhead) * kRows + r] = live ? make_float2(m, wo) : make_float2(0.f, 0.f);
+            }
             const int sub = lane >> 3, cq = lane & 7;  // transposed: row 4 * k + sub, 4 columns at 4 * cq
+            const unsigned rows_live = __ballot_sync(0xffffffffu, live);
+            uint32_t ridx[8];  // this lane's rows in the output, in units of 128 elements (row * H + head)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                ridx[k] = whole ? __shfl_sync(0xffffffffu, static_cast<uint32_t>(oidx), 4 * k + sub)
+                                : static_cast<uint32_t>(prow + 32 * q4 + 4 * k + sub);
 #pragma unroll 1
             for (int c = 0; c < kDim / 32; ++c) {
                 float o[32];
                 tmem_ld32(tO + c * 32, o);
                 tmem_wait_ld();
+                if (c == kDim / 32 - 1) {  // all of O is out
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&ofree[tile]);
+                }
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     *stg4(lane, i) = make_float4(o[4 * i] * wo, o[4 * i + 1] * wo, o[4 * i + 2] * wo, o[4 * i + 3] * wo);
@@ -412,12 +470,12 @@ __global__ void __launch_bounds__(kCThreads, 1)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const int row = 4 * k + sub;
-                    const unsigned long long oi = __shfl_sync(0xffffffffu, static_cast<unsigned long long>(oidx), row);
-                    const bool lv = __shfl_sync(0xffffffffu, live ? 1 : 0, row) != 0;
                     const float4 x = *stg4(row, cq);
-                    const size_t off = static_cast<size_t>(oi) * kDim + c * 32 + 4 * cq;
-                    if (!lv) continue;
-                    if constexpr (IO16)
+                    if (!(rows_live >> row & 1u)) continue;
+                    const size_t off = static_cast<size_t>(ridx[k]) * kDim + c * 32 + 4 * cq;
+                    if (!whole)
+                        *reinterpret_cast<float4*>(p.part_o + off) = x;
+                    else if constexpr (IO16)
                         *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) =
                             make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
                     else
@@ -425,17 +483,60 @@ __global__ void __launch_bounds__(kCThreads, 1)
                 }
                 __syncwarp();
             }
-        } else {
+        }
+        if (!ok) {
             *abort_flag = 1;
             if (lane == 0) atomicExch(p.err, kErrTimeout);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+}
+
+// Joins the partials of the (pair, KV head)s whose tile lists are cut between CTAs, in slot order: one
+// warp per row, lane = 4 dims. split = [nsplit][4] pair, KV head, first slot, slots.
+template <bool IO16>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, const int32_t* __restrict__ split, int nsplit) {
+    const int wid = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int e = wid / (2 * kRows), tile = (wid / kRows) & 1, r = wid % kRows;
+    if (e >= nsplit) return;
+    const int pair = split[4 * e], h = split[4 * e + 1], s0 = split[4 * e + 2], ns = split[4 * e + 3];
+    const int item = p.w_pair[2 * pair + tile];
+    if (item < 0) return;
+    const int t = r / p.g;
+    const bool live = t < p.w_ntok[item];
+    float2* ml = p.ml != nullptr ? p.ml + (static_cast<size_t>(item) * p.kvh + h) * kRows + r : nullptr;
+    if (!live) {
+        if (ml != nullptr && lane == 0) *ml = make_float2(0.f, 0.f);
+        return;
+    }
+    auto row = [&](int s) { return (static_cast<size_t>(s) * 2 + tile) * kRows + r; };
+    float mx = -INFINITY;
+    for (int s = s0; s < s0 + ns; ++s) mx = fmaxf(mx, p.part_ml[row(s) * 2]);
+    float den = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = s0; s < s0 + ns; ++s) {
+        const float ms = p.part_ml[row(s) * 2];
+        const float f = ms == -INFINITY ? 0.f : exp2f(ms - mx);
+        const float4 x = reinterpret_cast<const float4*>(p.part_o + row(s) * kDim)[lane];
+        den = fmaf(f, p.part_ml[row(s) * 2 + 1], den);
+        a.x = fmaf(f, x.x, a.x);
+        a.y = fmaf(f, x.y, a.y);
+        a.z = fmaf(f, x.z, a.z);
+        a.w = fmaf(f, x.w, a.w);
+    }
+    const float inv = 1.f / den;
+    if (ml != nullptr && lane == 0) *ml = make_float2(mx, inv);
+    const size_t off = (static_cast<size_t>(p.tok_row[p.w_tok0[item]] + t) * p.H + h * p.g + r % p.g) * kDim + 4 * lane;
+    if constexpr (IO16)
+        *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) =
+            make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+    else
+        *reinterpret_cast<float4*>(p.out + off) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
 }
 
 // ---------------------------------------------------------------- weights
@@ -648,12 +749,15 @@ __global__ void __launch_bounds__(256) weight_pieces_kernel(const WideParams p, 
 size_t chunk_smem_bytes() { return kCSmem; }
 
 cudaError_t launch_chunk_attention(const CUtensorMap* tmk2, const CUtensorMap* tmv2, const CUtensorMap* tmq,
-                                   const WideParams& p, int npairs, cudaStream_t st) {
-    if (npairs <= 0) return cudaSuccess;
+                                   const WideParams& p, const int32_t* split, int nsplit, cudaStream_t st) {
+    if (p.nctas <= 0) return cudaSuccess;
     auto kern = p.io16 ? chunk_attn_kernel<true> : chunk_attn_kernel<false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kCSmem);
     if (e != cudaSuccess) return e;
-    kern<<<npairs * p.kvh, kCThreads, kCSmem, st>>>(*tmk2, *tmv2, *tmq, p);
+    kern<<<p.nctas, kCThreads, kCSmem, st>>>(*tmk2, *tmv2, *tmq, p);
+    if ((e = cudaGetLastError()) != cudaSuccess || nsplit <= 0) return e;
+    auto merge = p.io16 ? chunk_merge_kernel<true> : chunk_merge_kernel<false>;
+    merge<<<nsplit * 2 * kRows / 8, 256, 0, st>>>(p, split, nsplit);
     return cudaGetLastError();
 }
 

@@ -188,6 +188,7 @@ struct WideParams {
     int sinks;
     float sscale;            // applied to the scores: 1 when the packed queries are scaled, else qscale
     int io16;                // q and out hold bf16
+    int bs_shift;            // log2 of bs (a power of two: it divides 128)
     float2* ml;              // [items][kvh][128] (max, 1 / sum) of each query row, log2 domain, or NULL
 };
 
@@ -387,11 +388,12 @@ cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const i
 cudaError_t launch_cc_attention(int dtype, bool io16, const CcParams& p, cudaStream_t st);
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
-// Chunk items of a bounded step: `npairs` pairs x KV heads. tmq: the tensor map of bf16 queries
+// Chunk items of a bounded step: p.nctas CTAs over the segments of p.cta_seg / p.seg, then the merge
+// of the `nsplit` (pair, KV head)s cut between CTAs. tmq: the tensor map of bf16 queries
 // (p.io16; unread otherwise); tmk2 / tmv2: boxes of min(block_size, kChunkKeys) slots.
 size_t chunk_smem_bytes();
 cudaError_t launch_chunk_attention(const CUtensorMap* tmk2, const CUtensorMap* tmv2, const CUtensorMap* tmq,
-                                   const WideParams& p, int npairs, cudaStream_t st);
+                                   const WideParams& p, const int32_t* split, int nsplit, cudaStream_t st);
 // Their weights: pieces {sequence, key tile, first and end query item} scored into
 // part[npieces][kvh][128], then added up into the touched blocks of `w` (t_piece: first piece of
 // each block's key tile and how many).
