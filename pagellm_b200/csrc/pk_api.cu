@@ -347,7 +347,7 @@ struct pk_batch {
     std::vector<int32_t> pieces;        // chunks' weights: sequence, key tile, first and end query item
     std::vector<int32_t> t_piece;       // per touched block of a chunk: first piece of its tile, pieces
     DevBuf wpieces;                     // [pieces][kvh][128] sums
-    DevBuf ml_items;                    // [chunk items][kvh][128] softmax statistics
+    DevBuf row_lse;                     // [chunk items][kvh][128] log-sum-exp of the rows
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
     std::vector<int32_t> t_meta;        // records of the first ntouch_tc touched blocks
@@ -1096,7 +1096,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
             B->t_seq.insert(B->t_seq.end(), ts[k].begin(), ts[k].end());
             B->t_blk.insert(B->t_blk.end(), tb[k].begin(), tb[k].end());
         }
-        PK_CUDA(B->ml_items.reserve(static_cast<size_t>(B->nwide) * P->kvh * 128 * sizeof(float2)));
+        PK_CUDA(B->row_lse.reserve(static_cast<size_t>(B->nwide) * P->kvh * 128 * sizeof(float)));
         PK_CUDA(B->wpieces.reserve(B->pieces.size() / 4 * P->kvh * pk::kWideKeys * sizeof(float)));
     }
     // Wide CTAs take two items each: neighbouring items of one sequence (chunk) or of one
@@ -1627,7 +1627,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         wide.sscale = io16 ? p.qscale : 1.f;
         wide.io16 = io16 ? 1 : 0;
         wide.bs_shift = log2_or_minus(P->block_size);
-        wide.ml = B->weights_mode != 0 ? static_cast<float2*>(B->ml_items.ptr) : nullptr;
+        wide.row_lse = B->weights_mode != 0 ? static_cast<float*>(B->row_lse.ptr) : nullptr;
         const int32_t* wrows = B->plan.at<int32_t>(10);
         const int64_t nw = fused ? static_cast<int64_t>(B->w_rows.size()) : 0;  // chunk rows still to append
         if (io16) {
@@ -2175,7 +2175,7 @@ int pk_batch_destroy(pk_batch* B) {
     B->score.release();
     B->cc_part.release();
     B->wpieces.release();
-    B->ml_items.release();
+    B->row_lse.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);

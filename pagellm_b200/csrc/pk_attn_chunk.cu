@@ -443,8 +443,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
             if (!whole) {
                 p.part_ml[(prow + r) * 2] = m;
                 p.part_ml[(prow + r) * 2 + 1] = l;
-            } else if (p.ml != nullptr && item >= 0) {
-                p.ml[(static_cast<size_t>(item) * p.kvh + sg.kvhead) * kRows + r] = live ? make_float2(m, wo) : make_float2(0.f, 0.f);
+            } else if (p.row_lse != nullptr && item >= 0) {
+                p.row_lse[(static_cast<size_t>(item) * p.kvh + sg.kvhead) * kRows + r] = live ? m + log2f(l) : INFINITY;
             }
             const int sub = lane >> 3, cq = lane & 7;  // transposed: row 4 * k + sub, 4 columns at 4 * cq
             const unsigned rows_live = __ballot_sync(0xffffffffu, live);
@@ -509,9 +509,9 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
     if (item < 0) return;
     const int t = r / p.g;
     const bool live = t < p.w_ntok[item];
-    float2* ml = p.ml != nullptr ? p.ml + (static_cast<size_t>(item) * p.kvh + h) * kRows + r : nullptr;
+    float* lse = p.row_lse != nullptr ? p.row_lse + (static_cast<size_t>(item) * p.kvh + h) * kRows + r : nullptr;
     if (!live) {
-        if (ml != nullptr && lane == 0) *ml = make_float2(0.f, 0.f);
+        if (lse != nullptr && lane == 0) *lse = INFINITY;
         return;
     }
     auto row = [&](int s) { return (static_cast<size_t>(s) * 2 + tile) * kRows + r; };
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
         a.w = fmaf(f, x.w, a.w);
     }
     const float inv = 1.f / den;
-    if (ml != nullptr && lane == 0) *ml = make_float2(mx, inv);
+    if (lse != nullptr && lane == 0) *lse = mx + log2f(den);
     const size_t off = (static_cast<size_t>(p.tok_row[p.w_tok0[item]] + t) * p.H + h * p.g + r % p.g) * kDim + 4 * lane;
     if constexpr (IO16)
         *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) =
@@ -541,7 +541,8 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
 
 // ---------------------------------------------------------------- weights
 // Attention weight of every key of a 128-key tile: a[j] = sum over query rows c of
-// 2^(s[j, c] - m[c]) / l[c], with the row statistics of chunk_attn_kernel. The score tile is computed
+// 2^(s[j, c] - lse[c]), with the rows' log-sum-exp of chunk_attn_kernel (one float per column: with
+// maximum and 1 / sum kept apart, reading them from shared memory took half of its bandwidth). The score tile is computed
 // transposed, S^T = K . Q^T with keys as the MMA rows, so that a thread owns one key and sums its
 // row alone: no reduction across threads, and a fixed order. A CTA takes one piece: a key tile of
 // one KV head against consecutive query items [i0, i1); the pieces of a tile are added in order by
@@ -553,8 +554,8 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
 constexpr int kGThreads = 192;  // producer, MMA issuer, 4 epilogue warps
 constexpr int kGOffK = 0;
 constexpr int kGOffQ = kGOffK + kTile;
-constexpr int kGOffStat = kGOffQ + 2 * kTile;               // [8][128] {m, 1/l}
-constexpr int kGOffBar = kGOffStat + 8 * kRows * 8;
+constexpr int kGOffStat = kGOffQ + 2 * kTile;               // [8][128] log-sum-exp
+constexpr int kGOffBar = kGOffStat + 8 * kRows * 4;
 constexpr int kGSmem = kGOffBar + 256 + 1024;
 
 template <bool IO16>
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kGThreads, 2)
                         const __grid_constant__ WideParams p, const int4* __restrict__ pieces, float* __restrict__ part) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const float2* stat = reinterpret_cast<const float2*>(smem + kGOffStat);
+    const float* stat = reinterpret_cast<const float*>(smem + kGOffStat);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + kGOffBar);
     uint64_t* qfull = kfull + 1;    // [2]
     uint64_t* qempty = qfull + 2;   // [2]
@@ -606,14 +607,14 @@ __global__ void __launch_bounds__(kGThreads, 2)
             load_key_tile(&tmk, smem + kGOffK, kfull, p, p.ids + p.indptr[seq], p.indptr[seq + 1] - p.indptr[seq], kt, head);
             int issued = 0;
             for (int x = 0; x < n; ++x) {
-                if (!mbar_wait_fast(&qempty[x & 1], ((x >> 1) & 1u) ^ 1u) || *abort_flag) {
+                if (!mbar_wait_bounded(&qempty[x & 1], ((x >> 1) & 1u) ^ 1u) || *abort_flag) {
                     *abort_flag = 1;
                     atomicExch(p.err, kErrTimeout);
                     break;
                 }
-                mbar_arrive_expect_tx(&stfull[x & 7], kRows * 8);
-                bulk_load(smem + kGOffStat + (x & 7) * kRows * 8, p.ml + (static_cast<size_t>(i0 + x) * p.kvh + head) * kRows,
-                          kRows * 8, &stfull[x & 7]);
+                mbar_arrive_expect_tx(&stfull[x & 7], kRows * 4);
+                bulk_load(smem + kGOffStat + (x & 7) * kRows * 4, p.row_lse + (static_cast<size_t>(i0 + x) * p.kvh + head) * kRows,
+                          kRows * 4, &stfull[x & 7]);
                 mbar_arrive_expect_tx(&qfull[x & 1], kTile);
                 load_query_tile<IO16>(&tmq, smem + kGOffQ + (x & 1) * kTile, &qfull[x & 1], p, i0 + x, head);
                 issued = x + 1;
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(kGThreads, 2)
         bool ok = __all_sync(0xffffffffu, mbar_wait_fast(kfull, 0u));
         for (int x = 0; x < n && ok; ++x) {
             const int b = x & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait_fast(&qfull[b], (x >> 1) & 1u, &sempty[b], ((x >> 1) & 1u) ^ 1u));
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&qfull[b], (x >> 1) & 1u) && mbar_wait_bounded(&sempty[b], ((x >> 1) & 1u) ^ 1u));
             if (!ok) break;
             tc_fence_after();
             const uint64_t qd = qd0 + b * (kTile >> 4);
@@ -661,10 +662,10 @@ __global__ void __launch_bounds__(kGThreads, 2)
         bool ok = true;
         for (int x = 0; x < n && ok; ++x) {
             const int b = x & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait_fast(&stfull[x & 7], (x >> 3) & 1u, &sfull[b], (x >> 1) & 1u));
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&stfull[x & 7], (x >> 3) & 1u) && mbar_wait_bounded(&sfull[b], (x >> 1) & 1u));
             if (!ok) break;
             tc_fence_after();
-            const float2* st = stat + (x & 7) * kRows;
+            const float* st = stat + (x & 7) * kRows;
             // token t of the item, at position pos0 + t, sees key j for t in [j - pos0, j - pos0 + window)
             // (without the upper limit when j is a sink); its columns are g * t .. g * t + g - 1
             const int pos0 = pos_i0 + x * tpt, ntok = x == n - 1 ? ntok_last : tpt;
@@ -687,20 +688,16 @@ __global__ void __launch_bounds__(kGThreads, 2)
                     if (lane == 0) mbar_arrive(&sempty[b]);
                 }
                 const float* v = sv[c & 1];
-                const float4* mlp = reinterpret_cast<const float4*>(st + 32 * c);
-                if (whole) {
+                const float4* lsep = reinterpret_cast<const float4*>(st + 32 * c);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float4 a = mlp[i];
-                        sum[(2 * i) & 3] = fmaf(ex2_approx(fmaf(v[2 * i], p.sscale, -a.x)), a.y, sum[(2 * i) & 3]);
-                        sum[(2 * i + 1) & 3] = fmaf(ex2_approx(fmaf(v[2 * i + 1], p.sscale, -a.z)), a.w, sum[(2 * i + 1) & 3]);
-                    }
-                } else {
+                for (int i = 0; i < 8; ++i) {
+                    const float4 a = lsep[i];
+                    const float ls[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float2 a = st[32 * c + i];
-                        const float e = 32 * c + i >= c_lo && 32 * c + i < c_hi ? ex2_approx(fmaf(v[i], p.sscale, -a.x)) : 0.f;
-                        sum[i & 3] = fmaf(e, a.y, sum[i & 3]);
+                    for (int k = 0; k < 4; ++k) {
+                        const int col = 32 * c + 4 * i + k;
+                        const float e = ex2_approx(fmaf(v[4 * i + k], p.sscale, -ls[k]));
+                        sum[k] += whole || (col >= c_lo && col < c_hi) ? e : 0.f;
                     }
                 }
             }
