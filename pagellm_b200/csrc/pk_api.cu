@@ -1238,7 +1238,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
         PK_CUDA(B->wpart.reserve(static_cast<size_t>(B->nslots) * 2 * 128 * (128 + 2) * sizeof(float)));
-    if (!B->w_seq.empty())
+    if (!B->w_seq.empty() && !B->bounded())  // (bounded steps pack only float queries: attend_bounded)
         PK_CUDA(B->qpk.reserve((B->w_seq.size() * P->kvh + 1) * static_cast<size_t>(pk::kWideQTileBytes)));
     if (B->nprefix > 0) PK_CUDA(B->lse.reserve(static_cast<size_t>(B->nrows) * H * sizeof(float)));
     rc = B->plan.commit(st);
@@ -1609,6 +1609,13 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     if (B->nwide > 0 && io16) {
         int rc = encode_query_map(P, q, B->nrows, H, &tmq);
         if (rc != PK_OK) return rc;
+    } else if (B->nwide > 0) {
+        const size_t bytes = (B->w_seq.size() * P->kvh + 1) * static_cast<size_t>(pk::kWideQTileBytes);
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+        if (bytes > B->qpk.cap && capturing != cudaStreamCaptureStatusNone)
+            return fail(PK_ERR_UNSUPPORTED, "the first call with float rows cannot be captured: call once before");
+        PK_CUDA(B->qpk.reserve(bytes));
     }
     if (B->nwide > 0) {
         cudaStream_t ws = st;
@@ -1728,6 +1735,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.t_blk = B->plan.at<int32_t>(27);
         w.ntouched = B->ntouch_tc;
         w.add = B->weights_mode == 1;
+        w.max_rows = *std::max_element(B->nnew.begin(), B->nnew.end());
         if (w.ntouched > 0) {
             pk::ScoreWeightParams sw{};
             sw.w = w;

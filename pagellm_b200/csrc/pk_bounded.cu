@@ -125,11 +125,16 @@ cudaError_t launch_rows_t(const BoundedParams& p, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ weights
-// One CTA per (touched block, KV head), warp = key: the key's row in registers, its score with
-// every row of the sequence that sees it recomputed, probability 2^(s - m) / l from the row's
-// statistics, summed in row order (one owner per key: no atomics, a fixed order).
-template <typename T, typename IO, int DPL>
-__global__ void __launch_bounds__(128) weight_rows_kernel(const BoundedParams p, const WeightParams w) {
+// Weights from K once more: a key's row in registers, its score with every row of the sequence that
+// sees it recomputed, probability 2^(s - m) / l from the row's statistics. One owner per key and a
+// fixed order of addition: no atomics. BY_ROW = false: one CTA per (touched block, KV head), a warp
+// takes every eighth key and all rows. BY_ROW = true (16 rows and more): one CTA per (touched block,
+// KV head, key), the rows dealt to its eight warps, whose sums are added in order; with a warp per key
+// a 191-row chunk of 48 (block, head)s kept 192 warps busy and took 0.9 ms.
+template <typename T, typename IO, int DPL, bool BY_ROW>
+__global__ void __launch_bounds__(256) weight_rows_kernel(const BoundedParams p, const WeightParams w) {
+    constexpr int NW = 8;
+    __shared__ float part[NW];
     const int e = blockIdx.x, kh = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int seq = w.t_seq[e], lb = w.t_blk[e];
@@ -139,47 +144,62 @@ __global__ void __launch_bounds__(128) weight_rows_kernel(const BoundedParams p,
     const int phys = p.ids[p.indptr[seq] + lb];
     const int g = p.H / p.kvh;
     const T* kpool = static_cast<const T*>(p.pool_k);
-    for (int t = warp; t < p.bs; t += 4) {
+    for (int t = BY_ROW ? static_cast<int>(blockIdx.z) : warp; t < p.bs; t += BY_ROW ? p.bs : NW) {
         const int j = lb * p.bs + t;
-        if (j >= ctx || (j >= p.sinks && j < lo)) continue;
+        if (j >= ctx || (j >= p.sinks && j < lo)) continue;  // (the same for all warps when BY_ROW)
         const size_t off = ((static_cast<size_t>(phys) * p.bs + t) * p.kvh + kh) * p.D;
         float kv[DPL];
 #pragma unroll
         for (int i = 0; i < DPL; ++i) kv[i] = lane + 32 * i < p.D ? to_f(kpool[off + lane + 32 * i]) : 0.f;
         float sum = 0.f;
-        for (int r = max(0, j - start); r < n; ++r) {
-            if (j >= p.sinks && j <= start + r - p.window) break;  // this and every later row is past it
+        // rows from the key's own on, until its window has passed it
+        const int r_end = j < p.sinks || j - start > INT32_MAX - p.window ? n : min(n, j - start + p.window);
+        for (int r = max(0, j - start) + (BY_ROW ? warp : 0); r < r_end; r += BY_ROW ? NW : 1) {
+            const size_t row = static_cast<size_t>(row0 + r) * p.H + kh * g;
+            const IO* qp = static_cast<const IO*>(p.q) + row * p.D;
+#pragma unroll 2
             for (int c = 0; c < g; ++c) {
-                const size_t row = static_cast<size_t>(row0 + r) * p.H + kh * g + c;
-                const IO* qp = static_cast<const IO*>(p.q) + row * p.D;
                 float dot = 0.f;
 #pragma unroll
                 for (int i = 0; i < DPL; ++i)
-                    if (lane + 32 * i < p.D) dot = fmaf(to_f(qp[lane + 32 * i]), kv[i], dot);
+                    if (lane + 32 * i < p.D) dot = fmaf(to_f(qp[static_cast<size_t>(c) * p.D + lane + 32 * i]), kv[i], dot);
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                const float2 ml = p.ml[row];
+                const float2 ml = p.ml[row + c];
                 sum += exp2f(dot * p.qscale - ml.x) * ml.y;
             }
         }
-        if (lane == 0) {
+        if (BY_ROW) {
+            if (lane == 0) part[warp] = sum;
+            __syncthreads();
+            sum = 0.f;
+            for (int x = 0; x < NW; ++x) sum += part[x];
+        }
+        if (lane == 0 && (!BY_ROW || warp == 0)) {
             float* dst = w.weights + (static_cast<size_t>(phys) * p.kvh + kh) * p.bs + t;
             *dst = w.add && j < start ? *dst + sum : sum;
         }
     }
 }
 
+template <typename T, typename IO, int DPL>
+cudaError_t launch_weight_rows_d(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
+    const dim3 grid(w.ntouched, p.kvh, w.max_rows >= 16 ? p.bs : 1);
+    if (grid.z > 1) weight_rows_kernel<T, IO, DPL, true><<<grid, 256, 0, st>>>(p, w);
+    else weight_rows_kernel<T, IO, DPL, false><<<grid, 256, 0, st>>>(p, w);
+    return cudaGetLastError();
+}
+
 template <typename T, typename IO>
 cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
-    const dim3 grid(w.ntouched, p.kvh);
+    if (p.kvh > 65535 || p.bs > 65535) return cudaErrorInvalidValue;
     const int dpl = (p.D + 31) / 32;
-    if (dpl <= 1) weight_rows_kernel<T, IO, 1><<<grid, 128, 0, st>>>(p, w);
-    else if (dpl <= 2) weight_rows_kernel<T, IO, 2><<<grid, 128, 0, st>>>(p, w);
-    else if (dpl <= 4) weight_rows_kernel<T, IO, 4><<<grid, 128, 0, st>>>(p, w);
-    else if (dpl <= 8) weight_rows_kernel<T, IO, 8><<<grid, 128, 0, st>>>(p, w);
-    else if (dpl <= 16) weight_rows_kernel<T, IO, 16><<<grid, 128, 0, st>>>(p, w);
-    else return cudaErrorInvalidValue;
-    return cudaGetLastError();
+    if (dpl <= 1) return launch_weight_rows_d<T, IO, 1>(p, w, st);
+    if (dpl <= 2) return launch_weight_rows_d<T, IO, 2>(p, w, st);
+    if (dpl <= 4) return launch_weight_rows_d<T, IO, 4>(p, w, st);
+    if (dpl <= 8) return launch_weight_rows_d<T, IO, 8>(p, w, st);
+    if (dpl <= 16) return launch_weight_rows_d<T, IO, 16>(p, w, st);
+    return cudaErrorInvalidValue;
 }
 
 // The scores of the touched blocks are still in L2 (8 to 64 bytes per key and KV head beside the

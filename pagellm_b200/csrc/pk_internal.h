@@ -254,6 +254,7 @@ struct WeightParams {
     const int32_t* t_blk;  // [ntouched] block of its table
     int ntouched;
     int add;  // add to the weights of tokens cached before the step (else store)
+    int max_rows;  // most new rows of a sequence
 };
 
 // Weights from the scores that a bounded split-KV launch kept, one warp per touched block.
