@@ -1751,6 +1751,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             sw.bs_shift = log2_or_minus(p.bs);
             sw.window = p.window;
             sw.sinks = p.sinks;
+            for (int i = 0; i < B->nseq; ++i) sw.max_units = std::max(sw.max_units, B->seq_u[i + 1] - B->seq_u[i]);
             PK_CUDA(pk::launch_weight_scores(sw, st));
             B->launches++;
         }

@@ -182,6 +182,91 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(const BoundedParams p,
     }
 }
 
+// The same for many rows, row lengths that are multiples of 4 * LK: LK lanes hold a key's row, R
+// elements each, so that a warp scores 32 / LK keys against a query row with R multiply-adds and
+// log2(LK) shuffles, the query read as 16-byte broadcasts; the (row, head) pairs are dealt to the
+// CTA's eight warps and their sums added in order. One CTA per (touched block, KV head, 32 / LK keys).
+__device__ __forceinline__ float4 vec4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
+__device__ __forceinline__ float4 vec4(const __nv_bfloat16* p) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    return make_float4(bf16_lo_f(w.x), bf16_hi_f(w.x), bf16_lo_f(w.y), bf16_hi_f(w.y));
+}
+template <typename T, typename IO, int R, int LK>
+__global__ void __launch_bounds__(256) weight_tile_kernel(const BoundedParams p, const WeightParams w) {
+    constexpr int NW = 8, KPW = 32 / LK;
+    __shared__ float part[NW][KPW];
+    const int e = blockIdx.x, kh = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = lane % LK, key = lane / LK;
+    const int seq = w.t_seq[e], lb = w.t_blk[e];
+    const int start = p.starts[seq], row0 = p.offsets[seq], n = p.offsets[seq + 1] - row0;
+    const int ctx = start + n;
+    const int lo = max(0, start - p.window + 1);
+    const int phys = p.ids[p.indptr[seq] + lb];
+    const int g = p.H / p.kvh;
+    const int t0 = blockIdx.z * KPW, t = t0 + key;
+    const int j = lb * p.bs + t;
+    const bool seen = t < p.bs && j < ctx && (j < p.sinks || j >= lo);
+    // the lane's part of its key: vectors sub, sub + LK, ...
+    float4 kv[R / 4];
+    const T* kp = static_cast<const T*>(p.pool_k) + ((static_cast<size_t>(phys) * p.bs + (t < p.bs ? t : 0)) * p.kvh + kh) * p.D;
+#pragma unroll
+    for (int v = 0; v < R / 4; ++v) {
+        const int d = 4 * (sub + LK * v);
+        kv[v] = seen && d < p.D ? vec4(kp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    // rows [r_lo, r_hi) see the lane's key; the CTA's rows: those that see any of its keys
+    const int r_lo = seen ? max(0, j - start) : INT32_MAX;
+    const int r_hi = !seen ? 0 : j < p.sinks || j - start > INT32_MAX - p.window ? n : min(n, j - start + p.window);
+    int a = r_lo, b = r_hi;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a = min(a, __shfl_xor_sync(0xffffffffu, a, o));
+        b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+    float sum = 0.f;
+    if (a < b) {
+        const IO* q = static_cast<const IO*>(p.q);
+        const int64_t x_end = static_cast<int64_t>(b) * g;
+        for (int64_t x = static_cast<int64_t>(a) * g + warp; x < x_end; x += NW) {
+            const int r = static_cast<int>(x / g), c = static_cast<int>(x - static_cast<int64_t>(r) * g);
+            const size_t row = static_cast<size_t>(row0 + r) * p.H + kh * g + c;
+            const IO* qp = q + row * p.D;
+            const float2 ml = __ldg(p.ml + row);
+            float d0 = 0.f, d1 = 0.f;
+#pragma unroll
+            for (int v = 0; v < R / 4; ++v) {
+                const int d = 4 * (sub + LK * v);
+                if (d >= p.D) continue;
+                const float4 y = vec4(qp + d);
+                d0 = fmaf(y.x, kv[v].x, d0);
+                d1 = fmaf(y.y, kv[v].y, d1);
+                d0 = fmaf(y.z, kv[v].z, d0);
+                d1 = fmaf(y.w, kv[v].w, d1);
+            }
+            float dot = d0 + d1;
+#pragma unroll
+            for (int o = LK / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+            if (r >= r_lo && r < r_hi) sum += exp2f(dot * p.qscale - ml.x) * ml.y;
+        }
+    }
+    if (sub == 0) part[warp][key] = sum;
+    __syncthreads();
+    if (warp == 0 && sub == 0 && seen) {
+        sum = 0.f;
+        for (int x = 0; x < NW; ++x) sum += part[x][key];
+        float* dst = w.weights + (static_cast<size_t>(phys) * p.kvh + kh) * p.bs + t;
+        *dst = w.add && j < start ? *dst + sum : sum;
+    }
+}
+
+template <typename T, typename IO, int R, int LK>
+cudaError_t launch_weight_tile(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
+    constexpr int KPW = 32 / LK;
+    weight_tile_kernel<T, IO, R, LK><<<dim3(w.ntouched, p.kvh, (p.bs + KPW - 1) / KPW), 256, 0, st>>>(p, w);
+    return cudaGetLastError();
+}
+
 template <typename T, typename IO, int DPL>
 cudaError_t launch_weight_rows_d(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
     const dim3 grid(w.ntouched, p.kvh, w.max_rows >= 16 ? p.bs : 1);
@@ -193,6 +278,14 @@ cudaError_t launch_weight_rows_d(const BoundedParams& p, const WeightParams& w, 
 template <typename T, typename IO>
 cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
     if (p.kvh > 65535 || p.bs > 65535) return cudaErrorInvalidValue;
+    // 16 rows and more (fewer do not fill the tile kernel's warps)
+    if (w.max_rows >= 16 && p.D % 4 == 0) {
+        if (p.D <= 32) return launch_weight_tile<T, IO, 16, 2>(p, w, st);
+        if (p.D <= 64) return launch_weight_tile<T, IO, 32, 2>(p, w, st);
+        if (p.D <= 128) return launch_weight_tile<T, IO, 64, 2>(p, w, st);
+        if (p.D <= 256) return launch_weight_tile<T, IO, 64, 4>(p, w, st);
+        if (p.D <= 512) return launch_weight_tile<T, IO, 64, 8>(p, w, st);
+    }
     const int dpl = (p.D + 31) / 32;
     if (dpl <= 1) return launch_weight_rows_d<T, IO, 1>(p, w, st);
     if (dpl <= 2) return launch_weight_rows_d<T, IO, 2>(p, w, st);
@@ -205,17 +298,20 @@ cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, 
 // The scores of the touched blocks are still in L2 (8 to 64 bytes per key and KV head beside the
 // 512 of its K and V), so summing them costs a fraction of reading K again. One warp per touched
 // block, its (KV head, token) pairs over the lanes, four of them in flight; records from the plan, so
-// that the chain is record -> unit -> scores. Units of a sequence in order, columns in order: the sum
-// does not depend on the schedule.
+// that the chain is record -> unit -> scores. MANY (a sequence of 16 units and more): one CTA per
+// (touched block, 32 pairs), the units dealt to its eight warps. Sums are added in a fixed order.
+template <bool MANY>
 __global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightParams p) {
-    const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    constexpr int NW = 8, kPer = MANY ? 1 : 4;
+    __shared__ float part[MANY ? NW : 1][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int e = MANY ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * NW + warp;
     if (e >= p.w.ntouched) return;
     const int4 r0 = __ldg(p.t_meta + 2 * e), r1 = __ldg(p.t_meta + 2 * e + 1);
     const int phys = r0.x, lb = r0.y, u0 = r0.z, u1 = r0.w, start = r1.x, ctx = r1.y;
     const int pairs = p.kvh * p.bs;
     float* wb = p.w.weights + static_cast<size_t>(phys) * pairs;
-    constexpr int kPer = 4;
-    for (int x0 = lane; x0 < pairs; x0 += 32 * kPer) {
+    for (int x0 = lane + (MANY ? 32 * static_cast<int>(blockIdx.y) : 0); MANY || x0 < pairs; x0 += 32 * kPer) {
         float sum[kPer], old[kPer];
         int h[kPer], t[kPer];
         bool live[kPer];
@@ -229,7 +325,7 @@ __global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightPar
             sum[k] = 0.f;
             old[k] = live[k] && p.w.add && j < start ? wb[x] : 0.f;
         }
-        for (int u = u0; u < u1; ++u) {
+        for (int u = u0 + (MANY ? warp : 0); u < u1; u += MANY ? NW : 1) {
             const int4 b = __ldg(p.u_bound + u);
             const int4 m0 = __ldg(p.u_meta + 2 * u), m1 = __ldg(p.u_meta + 2 * u + 1);
             const int nblk = m1.z - m1.y;
@@ -258,6 +354,16 @@ __global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightPar
                     if (c + 1 < ncol) sum[k] += exp2f(s[k].y - mb[k].x) * mb[k].y;
                 }
             }
+        }
+        if (MANY) {
+            part[warp][lane] = sum[0];
+            __syncthreads();
+            if (warp == 0 && live[0]) {
+                float total = old[0];
+                for (int x = 0; x < NW; ++x) total += part[x][lane];
+                wb[x0] = total;
+            }
+            return;
         }
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
@@ -557,7 +663,10 @@ cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, con
 
 cudaError_t launch_weight_scores(const ScoreWeightParams& p, cudaStream_t st) {
     if (p.w.ntouched <= 0) return cudaSuccess;
-    weight_scores_kernel<<<(p.w.ntouched + 7) / 8, 256, 0, st>>>(p);
+    if (p.max_units >= 16)
+        weight_scores_kernel<true><<<dim3(p.w.ntouched, (p.kvh * p.bs + 31) / 32), 256, 0, st>>>(p);
+    else
+        weight_scores_kernel<false><<<(p.w.ntouched + 7) / 8, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 

@@ -273,6 +273,7 @@ struct ScoreWeightParams {
     int bs_shift;           // log2 of bs, or -1
     int window;
     int sinks;
+    int max_units;          // most units of a sequence
 };
 
 struct EvictParams {
