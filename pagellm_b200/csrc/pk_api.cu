@@ -358,6 +358,12 @@ struct pk_batch {
     int cc_nsplit = 1, cc_max_vis = 0;
     std::vector<int32_t> cc_meta, cc_zero;
     DevBuf cc_part;
+    // sequences in tiles on the CUDA cores (tile_attn_kernel): units, key splits; the tiles of keys
+    // whose weights tile_weight_kernel sums, CTAs of each; counters of both
+    std::vector<uint8_t> seq_tile;
+    std::vector<int32_t> tile_meta, wtile_meta, tile_zero;
+    int ntiles = 0, tile_nsplit = 1, nwtiles = 0, wtile_parts = 1, ntouch_tile = 0;
+    DevBuf tile_part, wtile_part;
     DevBuf score;                       // raw scores of a split-KV launch with weights
     bool use_scores = false;
     DevBuf ml;  // [rows][H] softmax statistics of a step with weights
@@ -943,15 +949,16 @@ constexpr int64_t kCcCtasPerSm = 4, kCcMinKeys = 128, kCcScoreBytes = 64 * 1024;
 int plan_cc(pk_batch* B, int H) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
-    B->use_cc = B->bounded() && B->ngeneric > 0 && P->d % 4 == 0 && P->d <= 512;
+    B->use_cc = false;
     B->cc_meta.clear();
     B->cc_zero.clear();
     B->cc_weights = false;
-    if (!B->use_cc) return PK_OK;
+    if (!B->bounded() || P->d % 4 != 0 || P->d > 512) return PK_OK;
     int64_t vis = 0, most = 0;
     bool single = true;
     for (int r : B->gen_rows) {
         const int i = B->row_seq[r];
+        if (B->seq_tile[i]) continue;
         const int64_t pos = static_cast<int64_t>(B->starts[i]) + (r - B->offsets[i]);
         const int64_t lo = B->window > 0 ? std::max<int64_t>(0, pos - B->window + 1) : 0;
         const int64_t n = std::min(B->sinks, lo) + pos - lo + 1;
@@ -960,12 +967,15 @@ int plan_cc(pk_batch* B, int H) {
         single = single && B->nnew[i] == 1;
         B->cc_meta.insert(B->cc_meta.end(), {r, B->indptr[i], static_cast<int32_t>(pos), B->starts[i], B->offsets[i], 0, 0, 0});
     }
+    const int64_t nrows = static_cast<int64_t>(B->cc_meta.size() / 8);
+    if (nrows == 0) return PK_OK;
+    B->use_cc = true;
     const int G = pk::cc_group(g);
     const int64_t groups = static_cast<int64_t>(P->kvh) * ceil_div(g, G);
-    const int64_t ctas = static_cast<int64_t>(B->ngeneric) * groups;
+    const int64_t ctas = nrows * groups;
     if (groups > 65535) return fail(PK_ERR_UNSUPPORTED, "n_heads %d too large", H);
     const int64_t want = (kCcCtasPerSm * P->num_sms + ctas - 1) / ctas;
-    const int64_t room = std::max<int64_t>(1, vis / B->ngeneric / kCcMinKeys);
+    const int64_t room = std::max<int64_t>(1, vis / nrows / kCcMinKeys);
     B->cc_nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, room, 256})));
     B->cc_max_vis = static_cast<int>(most);
     B->cc_weights = B->weights_mode != 0 && single && g <= G && most * G * 4 <= kCcScoreBytes;
@@ -974,6 +984,70 @@ int plan_cc(pk_batch* B, int H) {
         PK_CUDA(B->cc_part.reserve(static_cast<size_t>(ctas) * B->cc_nsplit * G * (P->d + 2) * sizeof(float)));
         B->cc_zero.assign(static_cast<size_t>(ctas), 0);
     }
+    return PK_OK;
+}
+
+// Sequences in tiles on the CUDA cores. Units with the most visible keys go first. Splits of the keys,
+// as long as one keeps kTileMinKeyTiles tiles of the average unit, and parts of the columns for the
+// weights, of kTileMinKeyTiles column tiles of the longest sequence, until two CTAs per SM have work.
+constexpr int64_t kTileMinKeyTiles = 4;
+int plan_tiles(pk_batch* B, int H) {
+    pk_pool* P = B->pool;
+    const int g = H / P->kvh, bs = P->block_size;
+    B->tile_meta.clear();
+    B->wtile_meta.clear();
+    B->tile_zero.clear();
+    B->ntiles = B->nwtiles = 0;
+    B->tile_nsplit = B->wtile_parts = 1;
+    if (!B->bounded()) return PK_OK;
+    struct Unit { int64_t vis; int32_t m[4]; };
+    std::vector<Unit> units;
+    int64_t tiles = 0, most_new = 0;
+    const int tpt = std::max(1, pk::kTileCols / g);
+    for (size_t x = 0; x < B->gen_rows.size();) {  // (the rows of a sequence stand together)
+        const int i = B->row_seq[B->gen_rows[x]], n = B->nnew[i];
+        x += n;
+        if (!B->seq_tile[i]) continue;
+        for (int t0 = 0; t0 < n; t0 += tpt) {
+            const int nt = std::min(tpt, n - t0);
+            const int64_t pos = static_cast<int64_t>(B->starts[i]) + t0;
+            const int64_t lo = B->window > 0 ? std::max<int64_t>(0, pos - B->window + 1) : 0;
+            const int64_t vis = std::min(B->sinks, lo) + pos + nt - lo;
+            tiles += ceil_div(vis, pk::kTileKeys);
+            units.push_back({vis, {B->offsets[i] + t0, B->indptr[i], static_cast<int32_t>(pos), nt}});
+        }
+    }
+    std::stable_sort(units.begin(), units.end(), [](const Unit& a, const Unit& b) { return a.vis > b.vis; });
+    for (const Unit& u : units) B->tile_meta.insert(B->tile_meta.end(), u.m, u.m + 4);
+    B->ntiles = static_cast<int>(units.size());
+    if (B->ntiles > 0) {
+        const int64_t ctas = static_cast<int64_t>(B->ntiles) * P->kvh;
+        const int64_t want = (2 * P->num_sms + ctas - 1) / ctas;
+        B->tile_nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, tiles / B->ntiles / kTileMinKeyTiles)));
+        if (B->tile_nsplit > 1)
+            PK_CUDA(B->tile_part.reserve(static_cast<size_t>(ctas) * B->tile_nsplit * pk::kTileCols * (P->d + 4) * sizeof(float)));
+    }
+    const int e0 = B->ntouch_tc + B->ntouch_wide;
+    for (int x = e0; x < e0 + B->ntouch_tile;) {
+        const int i = B->t_seq[x];
+        int nb = 1;
+        while (x + nb < e0 + B->ntouch_tile && B->t_seq[x + nb] == i) ++nb;
+        for (int64_t s = 0; s < static_cast<int64_t>(nb) * bs; s += pk::kTileKeys)
+            B->wtile_meta.insert(B->wtile_meta.end(), {B->offsets[i], B->indptr[i], B->starts[i], B->nnew[i], x, nb,
+                                                       static_cast<int32_t>(s), 0});
+        most_new = std::max<int64_t>(most_new, B->nnew[i]);
+        x += nb;
+    }
+    B->nwtiles = static_cast<int>(B->wtile_meta.size() / 8);
+    if (B->nwtiles > 0) {
+        const int64_t ctas = static_cast<int64_t>(B->nwtiles) * P->kvh;
+        const int64_t want = (4 * P->num_sms + ctas - 1) / ctas;
+        B->wtile_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, most_new / tpt / kTileMinKeyTiles)));
+        if (B->wtile_parts > 1)
+            PK_CUDA(B->wtile_part.reserve(static_cast<size_t>(ctas) * B->wtile_parts * pk::kTileKeys * sizeof(float)));
+    }
+    if (B->tile_nsplit > 1 || B->wtile_parts > 1)
+        B->tile_zero.assign(static_cast<size_t>(B->ntiles + B->nwtiles) * P->kvh, 0);
     return PK_OK;
 }
 
@@ -1003,10 +1077,13 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->seq_kb0.assign(B->nseq, 0);
     const bool wide_ok = P->wide_ok && g <= 128 && 128 % g == 0;
     const int tpt = wide_ok ? 128 / g : 0;  // query tokens per wide item
+    const bool tile_ok = B->bounded() && P->d % 4 == 0 && P->d <= pk::kTileMaxDim && g <= pk::kTileCols && P->kvh <= 65535;
+    B->seq_tile.assign(B->nseq, 0);
     std::vector<int> tc_seqs;
     for (int i = 0; i < B->nseq; ++i) {
         const int n = B->nnew[i];
         if (n <= 0) continue;
+        B->seq_tile[i] = tile_ok && static_cast<int64_t>(n) * g >= pk::kTileMinCols;
         if (wide_ok && static_cast<int64_t>(n) * g >= kWideMinRows) {
             // chunk items: 128 query rows (128/g consecutive tokens) each
             for (int t0 = 0; t0 < n; t0 += tpt) {
@@ -1073,17 +1150,17 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->use_scores = B->weights_mode != 0 && score_floats > 0 &&
                     score_floats * static_cast<int64_t>(sizeof(float)) <= kMaxScoreBytes;
     if (B->use_scores) PK_CUDA(B->score.reserve(static_cast<size_t>(score_floats) * sizeof(float)));
-    B->ntouch_tc = B->ntouch_wide = 0;
+    B->ntouch_tc = B->ntouch_wide = B->ntouch_tile = 0;
     B->pieces.clear();
     B->t_piece.clear();
     if (B->weights_mode != 0) {
-        // touched blocks by the kernel that sums them: kept scores, chunks, K once more
-        std::vector<int32_t> ts[3], tb[3];
+        // touched blocks by the kernel that sums them: kept scores, chunks, K once more in tiles, by rows
+        std::vector<int32_t> ts[4], tb[4];
         std::vector<uint8_t> wide_seq(B->nseq, 0);
         for (int i : B->w_seq) wide_seq[i] = 1;
         for (size_t x = 0; x < B->t_seq.size(); ++x) {
             const int i = B->t_seq[x];
-            const int k = wide_seq[i] ? 1 : B->use_scores && B->seq_tc[i] ? 0 : 2;
+            const int k = wide_seq[i] ? 1 : B->use_scores && B->seq_tc[i] ? 0 : B->seq_tile[i] ? 2 : 3;
             ts[k].push_back(i);
             tb[k].push_back(B->t_blk[x]);
         }
@@ -1092,7 +1169,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         plan_weight_pieces(B, ts[1], tb[1]);
         B->t_seq.clear();
         B->t_blk.clear();
-        for (int k = 0; k < 3; ++k) {
+        B->ntouch_tile = static_cast<int>(ts[2].size());
+        for (int k = 0; k < 4; ++k) {
             B->t_seq.insert(B->t_seq.end(), ts[k].begin(), ts[k].end());
             B->t_blk.insert(B->t_blk.end(), tb[k].begin(), tb[k].end());
         }
@@ -1234,6 +1312,11 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (rc != PK_OK) return rc;
     B->plan.add(B->cc_meta.data(), B->cc_meta.size() * 4);  // 33
     B->plan.add(B->cc_zero.data(), B->cc_zero.size() * 4);  // 34
+    rc = plan_tiles(B, H);
+    if (rc != PK_OK) return rc;
+    B->plan.add(B->tile_meta.data(), B->tile_meta.size() * 4);  // 35
+    B->plan.add(B->wtile_meta.data(), B->wtile_meta.size() * 4);  // 36
+    B->plan.add(B->tile_zero.data(), B->tile_zero.size() * 4);  // 37
     if (B->weights_mode != 0)
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
@@ -1562,7 +1645,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     const bool fused_tc = k_new != nullptr && (B->use_tc || B->nwide > 0) && B->ngeneric == 0 && B->fuse_append_ok &&
                           B->tc_max_new <= kFuseMaxNew;
     // (a step wholly on cc_attn_kernel appends there)
-    const bool fused_cc = k_new != nullptr && B->use_cc && !B->use_tc && B->nwide == 0 && B->fuse_append_ok;
+    const bool fused_cc = k_new != nullptr && B->use_cc && B->ntiles == 0 && !B->use_tc && B->nwide == 0 && B->fuse_append_ok;
     const bool fused = fused_tc || fused_cc;
     if (k_new != nullptr && !fused) {
         const bool listed = !B->app_rows.empty();
@@ -1688,6 +1771,34 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         PK_CUDA(prof_end(B, kProfTc, st));
         B->launches++;
     }
+    pk::TileParams tile{};
+    if (B->ntiles > 0 || B->nwtiles > 0) {
+        tile.q = q;
+        tile.out = out;
+        tile.pool_k = p.pool_k;
+        tile.pool_v = p.pool_v;
+        tile.ids = p.ids;
+        tile.meta = B->plan.at<int4>(35);
+        tile.ml = p.ml;
+        tile.part = static_cast<float*>(B->tile_part.ptr);
+        tile.counters = B->plan.at<int>(37);
+        tile.nunits = B->ntiles;
+        tile.nsplit = B->tile_nsplit;
+        tile.H = H;
+        tile.kvh = p.kvh;
+        tile.D = p.D;
+        tile.bs = p.bs;
+        tile.bs_shift = log2_or_minus(p.bs);
+        tile.window = p.window;
+        tile.sinks = p.sinks;
+        tile.qscale = p.qscale;
+    }
+    if (B->ntiles > 0) {
+        PK_CUDA(prof_begin(B, st));
+        PK_CUDA(pk::launch_tile_attention(P->dtype, io16, tile, st));
+        PK_CUDA(prof_end(B, kProfGeneric, st));
+        B->launches++;
+    }
     if (B->use_cc) {
         pk::CcParams c{};
         c.q = q;
@@ -1702,7 +1813,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         c.weights = B->cc_weights ? P->weights + static_cast<int64_t>(layer) * P->layer_weights() : nullptr;
         c.part = static_cast<float*>(B->cc_part.ptr);
         c.counters = B->plan.at<int>(34);
-        c.nrows = B->ngeneric;
+        c.nrows = static_cast<int>(B->cc_meta.size() / 8);
         c.nsplit = B->cc_nsplit;
         c.max_vis = B->cc_max_vis;
         c.H = H;
@@ -1718,7 +1829,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         PK_CUDA(pk::launch_cc_attention(P->dtype, io16, c, st));
         PK_CUDA(prof_end(B, kProfGeneric, st));
         B->launches++;
-    } else if (B->ngeneric > 0) {
+    } else if (B->ngeneric > 0 && B->ntiles == 0) {
         PK_CUDA(prof_begin(B, st));
         PK_CUDA(pk::launch_bounded_rows(P->dtype, io16, p, st));
         PK_CUDA(prof_end(B, kProfGeneric, st));
@@ -1766,7 +1877,22 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         }
         w.t_seq += B->ntouch_wide;
         w.t_blk += B->ntouch_wide;
-        w.ntouched = B->cc_weights ? 0 : static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide;
+        if (B->nwtiles > 0) {
+            pk::TileWeightParams tw{};
+            tw.weights = w.weights;
+            tw.meta = B->plan.at<int4>(36);
+            tw.t_blk = B->plan.at<int32_t>(27);
+            tw.part = static_cast<float*>(B->wtile_part.ptr);
+            tw.counters = tile.counters + static_cast<size_t>(B->ntiles) * P->kvh;
+            tw.ntiles = B->nwtiles;
+            tw.nparts = B->wtile_parts;
+            tw.add = w.add;
+            PK_CUDA(pk::launch_tile_weights(P->dtype, io16, tile, tw, st));
+            B->launches++;
+        }
+        w.t_seq += B->ntouch_tile;
+        w.t_blk += B->ntouch_tile;
+        w.ntouched = B->cc_weights ? 0 : static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide - B->ntouch_tile;
         if (w.ntouched > 0) {
             PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
             B->launches++;

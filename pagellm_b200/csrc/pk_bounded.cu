@@ -182,91 +182,6 @@ __global__ void __launch_bounds__(256) weight_rows_kernel(const BoundedParams p,
     }
 }
 
-// The same for many rows, row lengths that are multiples of 4 * LK: LK lanes hold a key's row, R
-// elements each, so that a warp scores 32 / LK keys against a query row with R multiply-adds and
-// log2(LK) shuffles, the query read as 16-byte broadcasts; the (row, head) pairs are dealt to the
-// CTA's eight warps and their sums added in order. One CTA per (touched block, KV head, 32 / LK keys).
-__device__ __forceinline__ float4 vec4(const float* p) { return __ldg(reinterpret_cast<const float4*>(p)); }
-__device__ __forceinline__ float4 vec4(const __nv_bfloat16* p) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-    return make_float4(bf16_lo_f(w.x), bf16_hi_f(w.x), bf16_lo_f(w.y), bf16_hi_f(w.y));
-}
-template <typename T, typename IO, int R, int LK>
-__global__ void __launch_bounds__(256) weight_tile_kernel(const BoundedParams p, const WeightParams w) {
-    constexpr int NW = 8, KPW = 32 / LK;
-    __shared__ float part[NW][KPW];
-    const int e = blockIdx.x, kh = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane % LK, key = lane / LK;
-    const int seq = w.t_seq[e], lb = w.t_blk[e];
-    const int start = p.starts[seq], row0 = p.offsets[seq], n = p.offsets[seq + 1] - row0;
-    const int ctx = start + n;
-    const int lo = max(0, start - p.window + 1);
-    const int phys = p.ids[p.indptr[seq] + lb];
-    const int g = p.H / p.kvh;
-    const int t0 = blockIdx.z * KPW, t = t0 + key;
-    const int j = lb * p.bs + t;
-    const bool seen = t < p.bs && j < ctx && (j < p.sinks || j >= lo);
-    // the lane's part of its key: vectors sub, sub + LK, ...
-    float4 kv[R / 4];
-    const T* kp = static_cast<const T*>(p.pool_k) + ((static_cast<size_t>(phys) * p.bs + (t < p.bs ? t : 0)) * p.kvh + kh) * p.D;
-#pragma unroll
-    for (int v = 0; v < R / 4; ++v) {
-        const int d = 4 * (sub + LK * v);
-        kv[v] = seen && d < p.D ? vec4(kp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    // rows [r_lo, r_hi) see the lane's key; the CTA's rows: those that see any of its keys
-    const int r_lo = seen ? max(0, j - start) : INT32_MAX;
-    const int r_hi = !seen ? 0 : j < p.sinks || j - start > INT32_MAX - p.window ? n : min(n, j - start + p.window);
-    int a = r_lo, b = r_hi;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a = min(a, __shfl_xor_sync(0xffffffffu, a, o));
-        b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-    }
-    float sum = 0.f;
-    if (a < b) {
-        const IO* q = static_cast<const IO*>(p.q);
-        const int64_t x_end = static_cast<int64_t>(b) * g;
-        for (int64_t x = static_cast<int64_t>(a) * g + warp; x < x_end; x += NW) {
-            const int r = static_cast<int>(x / g), c = static_cast<int>(x - static_cast<int64_t>(r) * g);
-            const size_t row = static_cast<size_t>(row0 + r) * p.H + kh * g + c;
-            const IO* qp = q + row * p.D;
-            const float2 ml = __ldg(p.ml + row);
-            float d0 = 0.f, d1 = 0.f;
-#pragma unroll
-            for (int v = 0; v < R / 4; ++v) {
-                const int d = 4 * (sub + LK * v);
-                if (d >= p.D) continue;
-                const float4 y = vec4(qp + d);
-                d0 = fmaf(y.x, kv[v].x, d0);
-                d1 = fmaf(y.y, kv[v].y, d1);
-                d0 = fmaf(y.z, kv[v].z, d0);
-                d1 = fmaf(y.w, kv[v].w, d1);
-            }
-            float dot = d0 + d1;
-#pragma unroll
-            for (int o = LK / 2; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            if (r >= r_lo && r < r_hi) sum += exp2f(dot * p.qscale - ml.x) * ml.y;
-        }
-    }
-    if (sub == 0) part[warp][key] = sum;
-    __syncthreads();
-    if (warp == 0 && sub == 0 && seen) {
-        sum = 0.f;
-        for (int x = 0; x < NW; ++x) sum += part[x][key];
-        float* dst = w.weights + (static_cast<size_t>(phys) * p.kvh + kh) * p.bs + t;
-        *dst = w.add && j < start ? *dst + sum : sum;
-    }
-}
-
-template <typename T, typename IO, int R, int LK>
-cudaError_t launch_weight_tile(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
-    constexpr int KPW = 32 / LK;
-    weight_tile_kernel<T, IO, R, LK><<<dim3(w.ntouched, p.kvh, (p.bs + KPW - 1) / KPW), 256, 0, st>>>(p, w);
-    return cudaGetLastError();
-}
-
 template <typename T, typename IO, int DPL>
 cudaError_t launch_weight_rows_d(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
     const dim3 grid(w.ntouched, p.kvh, w.max_rows >= 16 ? p.bs : 1);
@@ -278,14 +193,6 @@ cudaError_t launch_weight_rows_d(const BoundedParams& p, const WeightParams& w, 
 template <typename T, typename IO>
 cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, cudaStream_t st) {
     if (p.kvh > 65535 || p.bs > 65535) return cudaErrorInvalidValue;
-    // 16 rows and more (fewer do not fill the tile kernel's warps)
-    if (w.max_rows >= 16 && p.D % 4 == 0) {
-        if (p.D <= 32) return launch_weight_tile<T, IO, 16, 2>(p, w, st);
-        if (p.D <= 64) return launch_weight_tile<T, IO, 32, 2>(p, w, st);
-        if (p.D <= 128) return launch_weight_tile<T, IO, 64, 2>(p, w, st);
-        if (p.D <= 256) return launch_weight_tile<T, IO, 64, 4>(p, w, st);
-        if (p.D <= 512) return launch_weight_tile<T, IO, 64, 8>(p, w, st);
-    }
     const int dpl = (p.D + 31) / 32;
     if (dpl <= 1) return launch_weight_rows_d<T, IO, 1>(p, w, st);
     if (dpl <= 2) return launch_weight_rows_d<T, IO, 2>(p, w, st);

@@ -246,6 +246,43 @@ struct CcParams {
 // Query heads of a KV head that a CTA of cc_attn_kernel takes together.
 inline int cc_group(int g) { return g == 1 ? 1 : g == 2 ? 2 : 4; }
 
+// Windowed attention on the CUDA cores in tiles of kTileCols columns - (token, head) pairs of a sequence
+// and KV head - by kTileKeys keys (tile_attn_kernel), for sequences with kTileMinCols columns and more.
+constexpr int kTileCols = 64, kTileKeys = 64, kTileMinCols = 32, kTileMaxDim = 256;
+struct TileParams {
+    const void* q;       // [rows][H][D], float or bf16
+    void* out;
+    const void* pool_k;  // layer base
+    const void* pool_v;
+    const int32_t* ids;
+    const int4* meta;    // [nunits] {first row, first table entry, its position, tokens}
+    float2* ml;          // [rows][H] (max, 1 / sum), log2 domain, or NULL
+    float* part;         // [nunits][kvh][nsplit][kTileCols][D + 4] partials (nsplit > 1)
+    int* counters;       // [nunits][kvh], zero between launches
+    int nunits;
+    int nsplit;
+    int H;
+    int kvh;
+    int D;
+    int bs;
+    int bs_shift;        // log2 of bs, or -1
+    int window;          // >= 1; INT32_MAX without a window
+    int sinks;
+    float qscale;        // log2(e) / sqrt(D)
+};
+// Their weights (tile_weight_kernel): tiles of kTileKeys consecutive slots of a sequence's touched blocks.
+struct TileWeightParams {
+    float* weights;
+    const int4* meta;      // [ntiles][2] {first row, first table entry, start, rows} of the sequence,
+                           // {its first touched block, their number, first slot of the tile, 0}
+    const int32_t* t_blk;  // touched blocks: table index
+    float* part;           // [ntiles][kvh][nparts][kTileKeys] (nparts > 1)
+    int* counters;         // [ntiles][kvh], zero between launches
+    int ntiles;
+    int nparts;            // CTAs of a tile and KV head
+    int add;
+};
+
 // The touched blocks of a step - those with a key that some row sees - and the layer's
 // accumulated weights [num_blocks][kvh][bs].
 struct WeightParams {
@@ -388,6 +425,8 @@ cudaError_t launch_slot_mapping(const int32_t* table, int64_t table_len, const i
                                 int64_t n, int bs, int64_t* slots, int32_t* err, cudaStream_t st);
 
 cudaError_t launch_cc_attention(int dtype, bool io16, const CcParams& p, cudaStream_t st);
+cudaError_t launch_tile_attention(int dtype, bool io16, const TileParams& p, cudaStream_t st);
+cudaError_t launch_tile_weights(int dtype, bool io16, const TileParams& p, const TileWeightParams& w, cudaStream_t st);
 cudaError_t launch_bounded_rows(int dtype, bool io16, const BoundedParams& p, cudaStream_t st);
 cudaError_t launch_weight_rows(int dtype, bool io16, const BoundedParams& p, const WeightParams& w, cudaStream_t st);
 // Chunk items of a bounded step: p.nctas CTAs over the segments of p.cta_seg / p.seg, then the merge
