@@ -1,0 +1,177 @@
+"""The forms that a bounded step takes besides the ordinary ones: register tiles on the CUDA cores,
+split keys, long contexts with few KV heads, weights summed from many units, steps on several streams
+and in captured graphs. Same oracle, same tolerances as the steps of test_gpu_bounded."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from gpu_util import Shape, torch_cuda
+from test_gpu_bounded import Case
+
+pytestmark = pytest.mark.gpu
+
+
+def _shape(s):
+    return "-".join(map(str, s))
+
+
+TILES = [("fp32", 16, 8, 128, 16), ("fp32", 64, 1, 32, 8), ("fp32", 33, 1, 64, 16), ("fp32", 6, 2, 96, 5),
+         ("fp32", 4, 4, 256, 16), ("fp32", 8, 2, 100, 48), ("fp32", 4, 2, 4, 1), ("bf16", 8, 2, 48, 16),
+         ("bf16", 9, 3, 132, 7), ("bf16", 16, 1, 252, 200)]
+
+
+@pytest.mark.parametrize("bounds", [(None, 0), (50, 3), (64, 70), (1, 1)])
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("shape", TILES, ids=_shape)
+def test_chunks_in_register_tiles(shape, weights, bounds):
+    """Sequences on both sides of the tiles' smallest size, beside rows alone and none."""
+    c = Case(*shape, [0, 200, 77, 5, 64, 129], [100, 33, 0, 1, 64, 7], window=bounds[0], sinks=bounds[1], weights=weights)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("weights", [None, "replace"])
+@pytest.mark.parametrize("shape", [("fp32", 65, 1, 64, 16), ("fp32", 4, 2, 260, 16), ("fp32", 3, 1, 17, 5),
+                                   ("fp32", 2, 1, 512, 16), ("bf16", 5, 1, 33, 16)], ids=_shape)
+def test_chunks_that_tiles_do_not_take(shape, weights):
+    c = Case(*shape, [0, 90], [40, 21], window=60, sinks=3, weights=weights)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("rows_io", ["bf16", "fp32"])
+def test_tiles_read_both_types_of_rows(rows_io):
+    c = Case("bf16", 8, 2, 48, 16, [30, 300], [70, 20], window=90, sinks=2, weights="add", io=rows_io)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("bounds", [(None, 0), (5000, 4)])
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("shape, starts, new", [
+    (("fp32", 4, 1, 64, 16), [9000], [16]),            # tiles, keys split
+    (("fp32", 4, 1, 64, 16), [0, 20], [700, 9]),       # the weights' columns dealt to several CTAs
+    (("fp32", 4, 1, 64, 16), [9000, 3], [1, 1]),       # rows, keys split
+    (("fp32", 16, 1, 128, 16), [9000], [1]),
+    (("fp32", 4, 1, 64, 16), [9000, 4000], [16, 2]),   # both in one step
+    (("bf16", 4, 2, 48, 16), [9000, 8000], [1, 30])], ids=str)
+def test_long_contexts_on_the_cuda_cores(shape, starts, new, weights, bounds):
+    c = Case(*shape, starts, new, window=bounds[0], sinks=bounds[1], weights=weights)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("bounds", [(None, 0), (20000, 4)])
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("H, new", [(8, 33), (16, 129), (4, 300)])
+def test_chunks_of_few_kv_heads_behind_long_contexts(H, new, weights, bounds):
+    c = Case("bf16", H, 1, 128, 16, [30000], [new], window=bounds[0], sinks=bounds[1], weights=weights, poison=False)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("shape", [("bf16", 8, 2, 128, 128), ("bf16", 32, 1, 128, 16), ("bf16", 8, 8, 128, 32),
+                                   ("bf16", 64, 2, 128, 64)], ids=_shape)
+@pytest.mark.parametrize("bounds", [(None, 0), (130, 3), (1, 129)])
+def test_chunks_beside_decodes(shape, weights, bounds):
+    c = Case(*shape, [0, 500, 127, 128, 0, 3], [200, 1, 1, 300, 0, 5], window=bounds[0], sinks=bounds[1], weights=weights)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("mode", ["add", "replace"])
+@pytest.mark.parametrize("shape", [("bf16", 16, 4, 64, 16), ("bf16", 24, 8, 128, 16), ("bf16", 10, 2, 128, 32)], ids=_shape)
+def test_weights_of_sequences_in_many_units(shape, mode):
+    c = Case(*shape, [0, 100, 7], [300, 40, 1], window=150, sinks=2, weights=mode)
+    c.check(c.run())
+
+
+def test_rows_of_every_magnitude():
+    """Scores up to some hundreds either way: the softmax ends on few keys, and earlier maxima fade."""
+    for dtype in ("fp32", "bf16"):
+        c = Case(dtype, 8, 2, 128, 16, [40, 300], [80, 1], window=70, sinks=2, q_scale=30.0)
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("shape", [("fp32", 4, 1, 64, 16), ("bf16", 8, 1, 128, 16)], ids=_shape)
+def test_split_steps_captured_and_repeated(shape):
+    """Counters and partials of split keys are ready again after each replay."""
+    torch = torch_cuda()
+    c = Case(*shape, [9000, 40], [40, 1], window=8000, sinks=4, weights="replace")
+    b = c.batch()
+    eager, weights = c.run(b).clone(), c.pool.weights.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b.write_and_attend(0, c.q, c.k, c.v)
+    for _ in range(3):
+        got.zero_()
+        c.pool.weights.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager)
+        touched = c.pool.weights != 0
+        assert torch.equal(c.pool.weights[touched], weights[touched])
+        assert bool((~touched | (weights != 0)).all())
+    b.check()
+    # and the handle runs eagerly again
+    c.pool.weights.copy_(c.before)
+    c.check(c.run(b))
+
+
+@pytest.mark.parametrize("shape", [("fp32", 8, 2, 128, 16), ("bf16", 8, 2, 128, 16)], ids=_shape)
+def test_two_steps_of_one_pool_at_once(shape):
+    """Two handles with sequences of their own, on two streams: as one after the other."""
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case(*shape, [3000, 1000, 40, 600], [1, 90, 60, 1], window=800, sinks=4, weights="add")
+    c.check(c.run())
+    halves = []
+    for ids in ((0, 1), (2, 3)):
+        rows = torch.cat([torch.arange(c.rows(i).start, c.rows(i).stop) for i in ids]).cuda()
+        halves.append((PagedBatch(c.pool, [c.tables[i] for i in ids], c.starts[list(ids)], c.new[list(ids)], window=800,
+                                  sinks=4, weights="add"), rows, [x[rows].contiguous() for x in (c.q, c.k, c.v)]))
+    one, weights = [], []
+    for turn in range(4):
+        c.pool.weights.copy_(c.before)
+        torch.cuda.synchronize()
+        outs, streams = [], []
+        for b, _, (q, k, v) in halves:
+            s = torch.cuda.Stream() if turn else torch.cuda.current_stream()
+            with torch.cuda.stream(s):
+                outs.append(b.write_and_attend(0, q, k, v))
+            streams.append(s)
+        torch.cuda.synchronize()
+        one.append(torch.cat(outs))
+        weights.append(c.pool.weights.clone())
+    for x in range(1, 4):
+        assert torch.equal(one[x], one[0]) and torch.equal(weights[x], weights[0])
+    order = torch.argsort(torch.cat([r for _, r, _ in halves]))
+    c.pool.weights.copy_(weights[0])
+    c.check(one[0][order])
+
+
+def test_many_layers_share_a_plan():
+    """One plan, a call per layer, each with its own weights."""
+    torch = torch_cuda()
+    c = Case("fp32", 8, 2, 64, 16, [700, 30], [40, 1], window=300, sinks=2, weights="add", layers=3, layer=1)
+    b = c.batch()
+    before = c.pool.weights.clone()
+    c.check(c.run(b))
+    assert torch.equal(c.pool.weights[0], before[0]) and torch.equal(c.pool.weights[2], before[2])
+    for layer in (0, 2):
+        c.layer, c.before = layer, c.pool.weights.clone()
+        c.check(c.run(b))
+
+
+def test_a_pool_of_numpy_rows_in_tiles():
+    """Host rows go the same way."""
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch, PagedKVPool
+
+    rng = np.random.default_rng(3)
+    q = rng.standard_normal((50, 4, 32)).astype(np.float32)
+    k, v = (rng.standard_normal((50, 2, 32)).astype(np.float32) for _ in range(2))
+    pools = [PagedKVPool(Shape(1, 2, 32), 8, 8, track_weights=True) for _ in range(2)]
+    outs = []
+    for pool, rows in zip(pools, ((q, k, v), [torch.as_tensor(x).cuda() for x in (q, k, v)])):
+        outs.append(PagedBatch(pool, [list(range(7))], [0], [50], window=20, sinks=1, weights="add").write_and_attend(0, *rows))
+    assert isinstance(outs[0], np.ndarray) and np.array_equal(outs[0], outs[1].cpu().numpy())
+    assert torch.equal(pools[0].weights, pools[1].weights)
