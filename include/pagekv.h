@@ -89,8 +89,9 @@ PK_API int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const fl
 /* Accumulated attention weights (no counterpart in pagellm): float32
  * [layers][num_blocks][n_kv_heads][block_size], zero-filled, one value per layer, token slot
  * and KV head, owned by the pool from the first call on (later calls return the same
- * memory). They belong to the block: sequences that share a block share its weights. pk_pool_copy_blocks copies a block's weights with it; pk_batch_set_bounds makes
- * steps keep them up and pk_pool_evict goes by them. */
+ * memory). They belong to the block: sequences that share a block share its weights.
+ * pk_pool_copy_blocks copies a block's weights with it; pk_batch_set_bounds makes steps keep
+ * them up and pk_pool_evict goes by them. */
 PK_API int pk_pool_track_weights(pk_pool* pool, float** weights_dev);
 /* Shortens cached sequences to the tokens worth keeping (no counterpart in pagellm, whose
  * caches only grow). For every layer, sequence i and KV head, a sequence of lengths[i] > budget
@@ -130,6 +131,8 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
  * it to the token's accumulated weight or puts it in its place. Tokens of the step itself
  * always start anew; tokens that no row sees keep their weight. With weights, a block that is
  * read must appear only once in the step (PK_ERR_INVALID_ARG from pk_batch_plan otherwise).
+ * A K or V that is not finite in a place that one row of a sequence's step sees may reach the
+ * sequence's other rows of the step; places that none sees are not read.
  * After a change the batch has to be planned again before it attends. A bounded step's first
  * call with some n_heads cannot be captured (PK_ERR_UNSUPPORTED); later ones can, and graphs
  * that were captured from one batch share its scratch: replay them one after another. */

@@ -107,7 +107,7 @@ struct Uploader {
     }
     // by_kernel: small uploads are fetched from the page-locked buffer by a kernel instead of the copy
     // engine, which a stream of short kernels waits for on both sides (an eviction of 8 short
-    // sequences: 36 us with the engine's copy, 25 us without).
+    // sequences: 38 us with the engine's copy, 34 without).
     static constexpr size_t kKernelBytes = size_t(1) << 20;
     int commit(cudaStream_t st, bool by_kernel = false) {
         size_t total = parts.empty() ? 0 : offs.back() + parts.back().second;
@@ -255,6 +255,7 @@ struct pk_pool {
     float* weights = nullptr;
     // evict: its tables and items, the kept positions when the caller wants none, and the end
     // of the last call (the next one may come on another stream)
+    std::mutex evict_mutex;
     EvictPlan evict_plan;
     Uploader evict_up[3];  // in turn: a call need not wait until the last one's copy has run
     unsigned evict_turn = 0;
@@ -541,6 +542,9 @@ void setup_tc(pk_pool* P) {
 
 // log2 of a power of two, else -1
 int log2_or_minus(int x) { return x > 0 && (x & (x - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(x)) : -1; }
+
+// The bounded steps' and the eviction's kernels step through 32-bit positions by up to this much.
+constexpr int kIndexRoom = 1 << 16;
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
@@ -1945,7 +1949,7 @@ int plan_evict(int64_t num_blocks, int bs, int nseq, const int64_t* table_indptr
     for (int i = 0; i < nseq; ++i) {
         const int64_t n = lengths[i], have = table_indptr[i + 1] - table_indptr[i], nhave = new_indptr[i + 1] - new_indptr[i];
         if (n < 0) return fail(PK_ERR_INVALID_ARG, "seq %d: length %lld negative", i, (long long)n);
-        if (n >= (int64_t(1) << 31) - bs) return fail(PK_ERR_UNSUPPORTED, "seq %d: length %lld too long", i, (long long)n);
+        if (n >= (int64_t(1) << 31) - std::max(bs, kIndexRoom)) return fail(PK_ERR_UNSUPPORTED, "seq %d: length %lld too long", i, (long long)n);
         if (have < 0 || nhave < 0) return fail(PK_ERR_INVALID_ARG, "a table's indptr decreases at seq %d", i);
         const int64_t need = (n + bs - 1) / bs, nneed = (std::min(n, budget) + bs - 1) / bs;
         if (need > have || nneed > nhave)
@@ -2183,6 +2187,7 @@ int pk_pool_track_weights(pk_pool* pool, float** weights_dev) {
         float* w = nullptr;
         cudaError_t e = cudaMalloc(&w, bytes);
         if (e == cudaSuccess) e = cudaMemset(w, 0, bytes);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);  // streams that do not wait for the default one
         if (e != cudaSuccess) {
             if (w) cudaFree(w);
             return fail(PK_ERR_CUDA, "attention weights of %zu bytes: %s", bytes, cudaGetErrorString(e));
@@ -2199,6 +2204,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     if (!P) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
     if (!P->weights) return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
     const int bs = P->block_size;
+    std::lock_guard<std::mutex> lock(P->evict_mutex);  // plan, uploads and scratch are the pool's
     EvictPlan& plan = P->evict_plan;
     int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
                         &plan);
@@ -2215,6 +2221,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     else PK_CUDA(cudaEventCreateWithFlags(&P->evict_done, cudaEventDisableTiming));
     pk::EvictParams p{};
     if (kept_dev == nullptr) {
+        budget = std::min<int64_t>(budget, std::max(plan.max_len, 1));  // the scratch needs no more places
         PK_CUDA(P->evict_kept.reserve(static_cast<size_t>(P->n_layers) * nseq * P->kvh * budget * sizeof(int32_t)));
         kept_dev = static_cast<int32_t*>(P->evict_kept.ptr);
     }
@@ -2346,7 +2353,8 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
         if (s < 0 || n < 0) return fail(PK_ERR_INVALID_ARG, "seq %d: start %lld / n_new %lld negative", i, (long long)s, (long long)n);
         if (te < tb) return fail(PK_ERR_INVALID_ARG, "table_indptr not non-decreasing at seq %d", i);
         const int64_t ctx = s + n;
-        if (ctx >= (int64_t(1) << 31)) return fail(PK_ERR_UNSUPPORTED, "seq %d: context %lld too long", i, (long long)ctx);
+        if (ctx >= (int64_t(1) << 31) - (B->bounded() ? std::max(bs, kIndexRoom) : 0))
+            return fail(PK_ERR_UNSUPPORTED, "seq %d: context %lld too long", i, (long long)ctx);
         const int64_t need = (ctx + bs - 1) / bs;
         if (need > te - tb)
             return fail(PK_ERR_OUT_OF_RANGE, "seq %d: positions up to %lld need %lld blocks, table has %lld",
@@ -2621,6 +2629,7 @@ int pk_peer_gather_write_and_attend(pk_peer_gather* g, pk_batch* B, int layer, i
     if (B->nrows > 0 && (!q_dev || !k_dev || !v_dev)) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
     if ((rc = check_aligned(q_dev, "q")) || (rc = check_aligned(k_dev, "k")) || (rc = check_aligned(v_dev, "v")))
         return rc;
+    if ((rc = check_bounds(B)) != PK_OK) return rc;
     DeviceScope ds(P->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (B->plan_H != n_heads) {

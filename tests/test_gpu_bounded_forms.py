@@ -175,3 +175,68 @@ def test_a_pool_of_numpy_rows_in_tiles():
         outs.append(PagedBatch(pool, [list(range(7))], [0], [50], window=20, sinks=1, weights="add").write_and_attend(0, *rows))
     assert isinstance(outs[0], np.ndarray) and np.array_equal(outs[0], outs[1].cpu().numpy())
     assert torch.equal(pools[0].weights, pools[1].weights)
+
+
+def test_positions_near_the_end_of_32_bits_are_refused():
+    """Kernels step through positions in 32 bits; the last 65536 of them are not given out."""
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import PagedBatch, PagedKVPool
+
+    pool = PagedKVPool(Shape(1, 1, 4), 1, 16, track_weights=True)
+    for n in (2 ** 31 - 2, 2 ** 31 - 65536):
+        with pytest.raises(_lib.PagedKVError, match="too long"):
+            PagedBatch(pool, [[0]], [n - 1], [1], window=4)
+        with pytest.raises(_lib.PagedKVError, match="too long"):
+            pool.evict([[0]], [n], 4)
+
+
+def _evictable(n=8, length=700, bs=16):
+    from pagellm_b200.cache import PagedKVPool
+
+    torch = torch_cuda()
+    nb = -(-length // bs)
+    pool = PagedKVPool(Shape(2, 2, 64), n * nb, bs, track_weights=True)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for x in (pool.k, pool.v, pool.weights):
+        x.normal_(generator=g)
+    pool.weights.abs_()
+    return pool, [list(range(i * nb, (i + 1) * nb)) for i in range(n)]
+
+
+def test_evict_with_a_budget_beyond_every_sequence():
+    torch = torch_cuda()
+    pool, tables = _evictable()
+    k, w = pool.k.clone(), pool.weights.clone()
+    for budget in (700, 2 ** 31 - 1):
+        assert pool.evict(tables, [700, 0, 1, 16, 333, 700, 699, 2], budget, sinks=4, recent=100).tolist() \
+            == [700, 0, 1, 16, 333, 700, 699, 2]
+        assert torch.equal(pool.k, k) and torch.equal(pool.weights, w)
+
+
+def test_evictions_from_several_threads():
+    """Each thread shortens its own sequences on its own stream, as one call after the other."""
+    import threading
+
+    torch = torch_cuda()
+    pool, tables = _evictable(16)
+    before = [x.clone() for x in (pool.k, pool.v, pool.weights)]
+    for t in tables:
+        pool.evict([t], [700], 100, sinks=2, recent=10)
+    want = [x.clone() for x in (pool.k, pool.v, pool.weights)]
+    for x, y in zip((pool.k, pool.v, pool.weights), before):
+        x.copy_(y)
+    torch.cuda.synchronize()
+
+    def work(mine):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for t in mine:
+                pool.evict([t], [700], 100, sinks=2, recent=10)
+
+    threads = [threading.Thread(target=work, args=(tables[i::4],)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for x, y in zip((pool.k, pool.v, pool.weights), want):
+        assert torch.equal(x, y)
