@@ -566,6 +566,10 @@ int64_t split_kv_ctas(int64_t T, int64_t nu, int64_t max_ctas) {
 // Sequences with at least this many new query rows (tokens x heads per KV head) go to the
 // wide-tile tensor-core kernel; fewer rows stay on the split-KV kernel's units.
 constexpr int64_t kWideMinRows = 64;
+// Bounded steps: more rows than two units hold, which then read the context three times (32 verify steps
+// of 12 tokens x 4 heads: 281 us in units, 225 on chunk_attn_kernel); two units are faster there than one
+// 128-row tile with most rows dead (5 tokens x 4 heads: 64 us against 90).
+constexpr int64_t kBoundedWideMinRows = 2 * pk::kMaxCols + 1;
 
 // Time a split-KV CTA loses per unit boundary inside its block range (B200, C2 decode
 // shape): it reloads queries, publishes a partial for the unit it leaves, and the unit it
@@ -1088,7 +1092,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         const int n = B->nnew[i];
         if (n <= 0) continue;
         B->seq_tile[i] = tile_ok && static_cast<int64_t>(n) * g >= pk::kTileMinCols;
-        if (wide_ok && static_cast<int64_t>(n) * g >= kWideMinRows) {
+        if (wide_ok && static_cast<int64_t>(n) * g >= (B->bounded() ? kBoundedWideMinRows : kWideMinRows)) {
             // chunk items: 128 query rows (128/g consecutive tokens) each
             for (int t0 = 0; t0 < n; t0 += tpt) {
                 const int nt = std::min(tpt, n - t0);
