@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kCThreads, 1)
                 p.part_ml[(prow + r) * 2] = m;
                 p.part_ml[(prow + r) * 2 + 1] = l;
             } else if (p.row_lse != nullptr && item >= 0) {
-                p.row_lse[(static_cast<size_t>(item) * p.kvh + sg.kvhead) * kRows + r] = live ? m + log2f(l) : INFINITY;
+                p.row_lse[(static_cast<size_t>(item) * p.kvh + sg.kvhead) * kRows + r] = live ? -(m + log2f(l)) : -INFINITY;
             }
             const int sub = lane >> 3, cq = lane & 7;  // transposed: row 4 * k + sub, 4 columns at 4 * cq
             const unsigned rows_live = __ballot_sync(0xffffffffu, live);
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
     const bool live = t < p.w_ntok[item];
     float* lse = p.row_lse != nullptr ? p.row_lse + (static_cast<size_t>(item) * p.kvh + h) * kRows + r : nullptr;
     if (!live) {
-        if (lse != nullptr && lane == 0) *lse = INFINITY;
+        if (lse != nullptr && lane == 0) *lse = -INFINITY;
         return;
     }
     auto row = [&](int s) { return (static_cast<size_t>(s) * 2 + tile) * kRows + r; };
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
         a.w = fmaf(f, x.w, a.w);
     }
     const float inv = 1.f / den;
-    if (lse != nullptr && lane == 0) *lse = mx + log2f(den);
+    if (lse != nullptr && lane == 0) *lse = -(mx + log2f(den));
     const size_t off = (static_cast<size_t>(p.tok_row[p.w_tok0[item]] + t) * p.H + h * p.g + r % p.g) * kDim + 4 * lane;
     if constexpr (IO16)
         *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + off) =
@@ -541,8 +541,9 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
 
 // ---------------------------------------------------------------- weights
 // Attention weight of every key of a 128-key tile: a[j] = sum over query rows c of
-// 2^(s[j, c] - lse[c]), with the rows' log-sum-exp of chunk_attn_kernel (one float per column: with
-// maximum and 1 / sum kept apart, reading them from shared memory took half of its bandwidth). The score tile is computed
+// 2^(s[j, c] - lse[c]), with the rows' log-sum-exp of chunk_attn_kernel, stored negated (one float per
+// column: with maximum and 1 / sum kept apart, reading them from shared memory took half of its
+// bandwidth). The score tile is computed
 // transposed, S^T = K . Q^T with keys as the MMA rows, so that a thread owns one key and sums its
 // row alone: no reduction across threads, and a fixed order. A CTA takes one piece: a key tile of
 // one KV head against consecutive query items [i0, i1); the pieces of a tile are added in order by
@@ -550,8 +551,10 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
 // (slot x + 8 is filled after the MMA of x + 6, which waited until the epilogue had taken S^T of
 // x + 4, so it was done with x), and S^T through two TMEM buffers; at 106 KB of shared memory and 256
 // TMEM columns two CTAs share an SM, so that one's exponentials run beside the other's loads and
-// MMAs. Bound: one exponential per score, 16 per clock and SM, twice the MMA's time.
-constexpr int kGThreads = 192;  // producer, MMA issuer, 4 epilogue warps
+// MMAs. Bound: one exponential per score, 16 per clock and SM, twice the MMA's time; 63 % of that rate
+// (85 us for 1024 rows of 32 heads over 5120 keys; with the column masks in every tile and four epilogue
+// warps 108, the integer pipe busier than the exponentials).
+constexpr int kGThreads = 320;  // producer, MMA issuer, 8 epilogue warps: two per 32 keys, 64 columns each
 constexpr int kGOffK = 0;
 constexpr int kGOffQ = kGOffK + kTile;
 constexpr int kGOffStat = kGOffQ + 2 * kTile;               // [8][128] log-sum-exp
@@ -564,6 +567,7 @@ __global__ void __launch_bounds__(kGThreads, 2)
                         const __grid_constant__ WideParams p, const int4* __restrict__ pieces, float* __restrict__ part) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ float halves[2][kKeys];
     const float* stat = reinterpret_cast<const float*>(smem + kGOffStat);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + kGOffBar);
     uint64_t* qfull = kfull + 1;    // [2]
@@ -585,7 +589,7 @@ __global__ void __launch_bounds__(kGThreads, 2)
             mbar_init(&qfull[b], 1);
             mbar_init(&qempty[b], 1);
             mbar_init(&sfull[b], 1);
-            mbar_init(&sempty[b], 4);
+            mbar_init(&sempty[b], 8);
         }
         for (int b = 0; b < 8; ++b) mbar_init(&stfull[b], 1);
         *abort_flag = 0;
@@ -651,66 +655,79 @@ __global__ void __launch_bounds__(kGThreads, 2)
         }
     } else {
         const int q4 = warp & 3;  // TMEM lanes 32 * q4 .. + 31
+        const int half = (warp - 2) >> 2;  // of the columns
         const int key = 32 * q4 + lane;
         const int j = kt * kKeys + key;
-        const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16);
+        const uint32_t trow = tmem + (static_cast<uint32_t>(32 * q4) << 16) + half * (kRows / 2);
         // items hold tpt = 128 / g consecutive tokens, all but a sequence's last one exactly
         const int tpt = kRows / p.g;
         const int pos_i0 = p.tok_pos[p.w_tok0[i0]];
         const int ntok_last = p.w_ntok[i0 + n - 1];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum2[2] = {0, 0};
+        const uint64_t scale2 = pack_f32x2(p.sscale, p.sscale);
         bool ok = true;
         for (int x = 0; x < n && ok; ++x) {
             const int b = x & 1;
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&stfull[x & 7], (x >> 3) & 1u) && mbar_wait_bounded(&sfull[b], (x >> 1) & 1u));
             if (!ok) break;
             tc_fence_after();
-            const float* st = stat + (x & 7) * kRows;
+            const float* st = stat + (x & 7) * kRows + half * (kRows / 2);
             // token t of the item, at position pos0 + t, sees key j for t in [j - pos0, j - pos0 + window)
             // (without the upper limit when j is a sink); its columns are g * t .. g * t + g - 1
             const int pos0 = pos_i0 + x * tpt, ntok = x == n - 1 ? ntok_last : tpt;
             const int rel = j - pos0;
             const int t_lo = max(0, rel);
             const int t_hi = j < p.sinks || rel > INT32_MAX - p.window ? ntok : min(ntok, rel + p.window);
-            const int c_lo = t_lo * p.g, c_hi = t_hi * p.g;
-            const bool whole = __all_sync(0xffffffffu, c_lo == 0 && c_hi == kRows);
-            // 32 columns at a time, the next ones on their way while these are summed
+            // (columns of this warp's half)
+            const int c_lo = t_lo * p.g - half * (kRows / 2), c_hi = t_hi * p.g - half * (kRows / 2);
+            const bool whole = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= kRows / 2);
             float sv[2][32];
             tmem_ld32(trow + b * kKeys, sv[0]);
+            tmem_ld32(trow + b * kKeys + 32, sv[1]);
+            tmem_wait_ld();
+            tc_fence_before();  // S^T is in registers
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sempty[b]);
 #pragma unroll
-            for (int c = 0; c < kRows / 32; ++c) {
-                tmem_wait_ld();
-                if (c + 1 < kRows / 32) {
-                    tmem_ld32(trow + b * kKeys + 32 * (c + 1), sv[(c + 1) & 1]);
-                } else {  // all of S^T is in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sempty[b]);
-                }
-                const float* v = sv[c & 1];
-                const float4* lsep = reinterpret_cast<const float4*>(st + 32 * c);
+            for (int c = 0; c < 2; ++c) {
+                const float* v = sv[c];
+                const ulonglong2* lsep = reinterpret_cast<const ulonglong2*>(st + 32 * c);
+                // two columns at a time; masks only where some key does not see all of the rows
+                auto add_columns = [&](auto masked) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 a = lsep[i];
-                    const float ls[4] = {a.x, a.y, a.z, a.w};
+                    for (int i = 0; i < 8; ++i) {
+                        const ulonglong2 nl = lsep[i];
+                        float e[4];
+                        unpack_f32x2(fma_f32x2(pack_f32x2(v[4 * i], v[4 * i + 1]), scale2, nl.x), e[0], e[1]);
+                        unpack_f32x2(fma_f32x2(pack_f32x2(v[4 * i + 2], v[4 * i + 3]), scale2, nl.y), e[2], e[3]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int col = 32 * c + 4 * i + k;
-                        const float e = ex2_approx(fmaf(v[4 * i + k], p.sscale, -ls[k]));
-                        sum[k] += whole || (col >= c_lo && col < c_hi) ? e : 0.f;
+                        for (int k = 0; k < 4; ++k) {
+                            e[k] = ex2_approx(e[k]);
+                            if constexpr (decltype(masked)::value) {
+                                const int col = 32 * c + 4 * i + k;
+                                e[k] = col >= c_lo && col < c_hi ? e[k] : 0.f;
+                            }
+                        }
+                        sum2[0] = add_f32x2(sum2[0], pack_f32x2(e[0], e[1]));
+                        sum2[1] = add_f32x2(sum2[1], pack_f32x2(e[2], e[3]));
                     }
-                }
+                };
+                if (whole) add_columns(std::false_type{});
+                else add_columns(std::true_type{});
             }
         }
-        if (ok) {
-            part[(static_cast<size_t>(blockIdx.x) * p.kvh + head) * kKeys + key] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        } else {
+        if (!ok) {
             *abort_flag = 1;
             if (lane == 0) atomicExch(p.err, kErrTimeout);
         }
+        float a, c;
+        unpack_f32x2(add_f32x2(sum2[0], sum2[1]), a, c);
+        halves[half][key] = a + c;
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x < kKeys && !*abort_flag)
+        part[(static_cast<size_t>(blockIdx.x) * p.kvh + head) * kKeys + threadIdx.x] = halves[0][threadIdx.x] + halves[1][threadIdx.x];
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 2 * kKeys);

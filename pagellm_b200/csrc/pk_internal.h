@@ -189,7 +189,7 @@ struct WideParams {
     float sscale;            // applied to the scores: 1 when the packed queries are scaled, else qscale
     int io16;                // q and out hold bf16
     int bs_shift;            // log2 of bs (a power of two: it divides 128)
-    float* row_lse;          // [items][kvh][128] log-sum-exp of each query row, log2 domain (dead rows: inf), or NULL
+    float* row_lse;          // [items][kvh][128] minus the log-sum-exp of each query row, log2 domain (dead rows: -inf), or NULL
 };
 
 // Windowed attention on the CUDA cores: any pool, rows of `q` / `out` in the pool's input type.
