@@ -212,8 +212,17 @@ class PagedKVPool:
         a new block is read by the call (other than the same block of the same sequence)."""
         torch = _torch()
         lens = np.ascontiguousarray(np.asarray(lengths, dtype=np.int64).reshape(-1))
-        indptr, ids = _csr(block_tables)
-        nindptr, nids = (indptr, ids) if new_tables is None else _csr(new_tables)
+        if type(block_tables) is list and type(new_tables) is list and block_tables and new_tables \
+                and type(block_tables[0]) is type(new_tables[0]):
+            # both in one pass (an eviction of a few short sequences is bound by this host work)
+            n = len(block_tables)
+            indptr, ids = _csr(block_tables + new_tables)
+            m = int(indptr[n])
+            nindptr, nids = indptr[n:] - m, ids[m:]
+            indptr, ids = indptr[: n + 1], ids[:m]
+        else:
+            indptr, ids = _csr(block_tables)
+            nindptr, nids = (indptr, ids) if new_tables is None else _csr(new_tables)
         if len(indptr) - 1 != len(lens) or len(nindptr) - 1 != len(lens):
             raise ValueError("block_tables, new_tables and lengths differ in length")
         kept = None
@@ -497,18 +506,19 @@ class PagedBatch:
 
     def _run(self, layer, q, k, v, append):
         P = self.pool
-        if q.ndim != 3 or q.shape[0] != self.num_rows or q.shape[2] != P.head_dim:
-            raise ValueError(f"q must be (rows={self.num_rows}, H, {P.head_dim}), got {tuple(q.shape)}")
-        H = int(q.shape[1])
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != self.num_rows or shape[2] != P.head_dim:
+            raise ValueError(f"q must be (rows={self.num_rows}, H, {P.head_dim}), got {tuple(shape)}")
+        H = int(shape[1])
         if append:
             want = (self.num_rows, P.n_kv_heads, P.head_dim)
-            if tuple(k.shape) != want or tuple(v.shape) != want:
+            if k.shape != want or v.shape != want:
                 raise ValueError(f"k, v must be {want}")
         st = _stream(P.device)
         if self._bounded and hasattr(q, "is_cuda"):
             torch = _torch()
             # bf16 rows on a bf16 pool as they are, anything else as float32
-            io16 = q.dtype == torch.bfloat16 and P.dtype_name == "bfloat16"
+            io16 = q.dtype is torch.bfloat16 and P.dtype_name == "bfloat16"
             dt = torch.bfloat16 if io16 else torch.float32
             qd = _rows(q, P.device, dt)
             out = torch.empty_like(qd)
@@ -524,7 +534,7 @@ class PagedBatch:
                 rc = self._lib.pk_batch_attend(self._b, layer, H, qd.data_ptr(), out.data_ptr(), st)
             if rc:
                 _lib.check(rc)
-            return out if io16 or q.dtype == torch.float32 else out.to(q.dtype)
+            return out if io16 or q.dtype is dt else out.to(q.dtype)
         if hasattr(q, "is_cuda"):
             torch = _torch()
             qd = _aligned(q.to(P.device, torch.float32).contiguous())
