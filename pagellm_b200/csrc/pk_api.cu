@@ -364,6 +364,7 @@ struct pk_batch {
     std::vector<uint8_t> seq_tile;
     std::vector<int32_t> tile_meta, wtile_meta, tile_zero;
     int ntiles = 0, tile_nsplit = 1, nwtiles = 0, wtile_parts = 1, ntouch_tile = 0;
+    int rest_max_rows = 0;  // most new rows of the sequences whose weights come by rows
     DevBuf tile_part, wtile_part;
     DevBuf score;                       // raw scores of a split-KV launch with weights
     bool use_scores = false;
@@ -966,7 +967,7 @@ int plan_cc(pk_batch* B, int H) {
     bool single = true;
     for (int r : B->gen_rows) {
         const int i = B->row_seq[r];
-        if (B->seq_tile[i]) continue;
+        if (B->seq_tile[i] & 1) continue;
         const int64_t pos = static_cast<int64_t>(B->starts[i]) + (r - B->offsets[i]);
         const int64_t lo = B->window > 0 ? std::max<int64_t>(0, pos - B->window + 1) : 0;
         const int64_t n = std::min(B->sinks, lo) + pos - lo + 1;
@@ -1015,7 +1016,7 @@ int plan_tiles(pk_batch* B, int H) {
     for (size_t x = 0; x < B->gen_rows.size();) {  // (the rows of a sequence stand together)
         const int i = B->row_seq[B->gen_rows[x]], n = B->nnew[i];
         x += n;
-        if (!B->seq_tile[i]) continue;
+        if (!(B->seq_tile[i] & 1)) continue;
         for (int t0 = 0; t0 < n; t0 += tpt) {
             const int nt = std::min(tpt, n - t0);
             const int64_t pos = static_cast<int64_t>(B->starts[i]) + t0;
@@ -1091,7 +1092,9 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     for (int i = 0; i < B->nseq; ++i) {
         const int n = B->nnew[i];
         if (n <= 0) continue;
-        B->seq_tile[i] = tile_ok && static_cast<int64_t>(n) * g >= pk::kTileMinCols;
+        // bit 0: rows in tiles, bit 1: weights in tiles
+        B->seq_tile[i] = !tile_ok ? 0 : (static_cast<int64_t>(n) * g >= pk::kTileMinCols ? 1 : 0) |
+                                            (static_cast<int64_t>(n) * g >= pk::kTileMinWeightCols ? 2 : 0);
         if (wide_ok && static_cast<int64_t>(n) * g >= (B->bounded() ? kBoundedWideMinRows : kWideMinRows)) {
             // chunk items: 128 query rows (128/g consecutive tokens) each
             for (int t0 = 0; t0 < n; t0 += tpt) {
@@ -1168,7 +1171,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         for (int i : B->w_seq) wide_seq[i] = 1;
         for (size_t x = 0; x < B->t_seq.size(); ++x) {
             const int i = B->t_seq[x];
-            const int k = wide_seq[i] ? 1 : B->use_scores && B->seq_tc[i] ? 0 : B->seq_tile[i] ? 2 : 3;
+            const int k = wide_seq[i] ? 1 : B->use_scores && B->seq_tc[i] ? 0 : (B->seq_tile[i] & 2) != 0 ? 2 : 3;
             ts[k].push_back(i);
             tb[k].push_back(B->t_blk[x]);
         }
@@ -1178,6 +1181,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         B->t_seq.clear();
         B->t_blk.clear();
         B->ntouch_tile = static_cast<int>(ts[2].size());
+        B->rest_max_rows = 0;
+        for (int i : ts[3]) B->rest_max_rows = std::max(B->rest_max_rows, B->nnew[i]);
         for (int k = 0; k < 4; ++k) {
             B->t_seq.insert(B->t_seq.end(), ts[k].begin(), ts[k].end());
             B->t_blk.insert(B->t_blk.end(), tb[k].begin(), tb[k].end());
@@ -1854,7 +1859,6 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.t_blk = B->plan.at<int32_t>(27);
         w.ntouched = B->ntouch_tc;
         w.add = B->weights_mode == 1;
-        w.max_rows = *std::max_element(B->nnew.begin(), B->nnew.end());
         if (w.ntouched > 0) {
             pk::ScoreWeightParams sw{};
             sw.w = w;
@@ -1901,6 +1905,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.t_seq += B->ntouch_tile;
         w.t_blk += B->ntouch_tile;
         w.ntouched = B->cc_weights ? 0 : static_cast<int>(B->t_seq.size()) - B->ntouch_tc - B->ntouch_wide - B->ntouch_tile;
+        w.max_rows = B->rest_max_rows;
         if (w.ntouched > 0) {
             PK_CUDA(pk::launch_weight_rows(P->dtype, io16, p, w, st));
             B->launches++;

@@ -249,6 +249,11 @@ inline int cc_group(int g) { return g == 1 ? 1 : g == 2 ? 2 : 4; }
 // Windowed attention on the CUDA cores in tiles of kTileCols columns - (token, head) pairs of a sequence
 // and KV head - by kTileKeys keys (tile_attn_kernel), for sequences with kTileMinCols columns and more.
 constexpr int kTileCols = 64, kTileKeys = 64, kTileMinCols = 32, kTileMaxDim = 256;
+// Columns from which tile_weight_kernel sums a sequence's weights; more than the 4 heads of a KV head up
+// to which a decode row's are summed inside cc_attn_kernel. Weights of 7 verify rows of 2 heads, 15
+// contexts up to 1886: 306 us with the attention by rows, 218 here; decode rows of 8 heads 214 and 220,
+// of 5 heads 597 and 702.
+constexpr int kTileMinWeightCols = 8;
 struct TileParams {
     const void* q;       // [rows][H][D], float or bf16
     void* out;
@@ -291,7 +296,7 @@ struct WeightParams {
     const int32_t* t_blk;  // [ntouched] block of its table
     int ntouched;
     int add;  // add to the weights of tokens cached before the step (else store)
-    int max_rows;  // most new rows of a sequence
+    int max_rows;  // most new rows of a touched sequence
 };
 
 // Weights from the scores that a bounded split-KV launch kept, one warp per touched block.

@@ -240,3 +240,12 @@ def test_evictions_from_several_threads():
     torch.cuda.synchronize()
     for x, y in zip((pool.k, pool.v, pool.weights), want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("mode", ["add", "replace"])
+@pytest.mark.parametrize("shape", [("fp32", 16, 8, 64, 8), ("fp32", 8, 1, 128, 16), ("fp32", 10, 2, 64, 16),
+                                   ("bf16", 40, 8, 128, 64)], ids=_shape)
+def test_weights_of_few_columns(shape, mode):
+    """Rows on one kernel, their weights on another: by rows or in tiles, side by side in one step."""
+    c = Case(*shape, [150, 90, 333, 0, 64], [7, 1, 1, 19, 4], window=120, sinks=2, weights=mode)
+    c.check(c.run())
