@@ -207,8 +207,10 @@ cudaError_t launch_weight_rows_t(const BoundedParams& p, const WeightParams& w, 
 // block, its (KV head, token) pairs over the lanes, four of them in flight; records from the plan, so
 // that the chain is record -> unit -> scores. MANY (a sequence of 16 units and more): one CTA per
 // (touched block, 32 pairs), the units dealt to its eight warps. Sums are added in a fixed order.
+// Bound by its chain of loads: 64 decodes over 148k tokens 20 us of the step's 124 (128 where the
+// compiler is not told that one CTA per SM will do, 140 held to 40 registers).
 template <bool MANY>
-__global__ void __launch_bounds__(256) weight_scores_kernel(const ScoreWeightParams p) {
+__global__ void __launch_bounds__(256, 1) weight_scores_kernel(const ScoreWeightParams p) {
     constexpr int NW = 8, kPer = MANY ? 1 : 4;
     __shared__ float part[MANY ? NW : 1][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
