@@ -106,7 +106,7 @@ PK_API int pk_pool_track_weights(pk_pool* pool, float** weights_dev);
  * (eviction in place); and no block may appear twice in the new tables.
  * kept_dev: NULL, or int32 [layers][nseq][n_kv_heads][budget] that receives the kept positions
  * in ascending order, -1 behind the last. Uploads its tables from host memory of the call:
- * a capturing stream gets PK_ERR_UNSUPPORTED. */
+ * a capturing stream gets PK_ERR_UNSUPPORTED, and so does a head_dim above 512. */
 PK_API int pk_pool_evict(pk_pool* pool, int nseq, const int64_t* table_indptr, const int32_t* table_ids,
                   const int64_t* lengths, const int64_t* new_indptr, const int32_t* new_ids, int64_t budget,
                   int64_t sinks, int64_t recent, int32_t* kept_dev, void* stream);

@@ -1637,7 +1637,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     pk_pool* P = B->pool;
     if (g_inject_launch_failure.exchange(0) != 0)
         return fail(PK_ERR_CUDA, "injected launch failure (pk_test_inject_launch_failure)");
-    if (P->d > 512) return fail(PK_ERR_UNSUPPORTED, "head_dim %d > 512", P->d);
+    if (P->d > pk::kMaxBoundedDim) return fail(PK_ERR_UNSUPPORTED, "head_dim %d > %d", P->d, pk::kMaxBoundedDim);
     if (B->plan_H != H) {
         int rc = build_attention_plan(B, H, st);
         if (rc != PK_OK) return rc;
@@ -2218,6 +2218,7 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
                         &plan);
     if (rc != PK_OK || nseq == 0) return rc;
+    if (P->d > pk::kMaxBoundedDim) return fail(PK_ERR_UNSUPPORTED, "head_dim %d > %d", P->d, pk::kMaxBoundedDim);
     if (static_cast<int64_t>(P->kvh) * P->n_layers > 65535)
         return fail(PK_ERR_UNSUPPORTED, "n_layers * n_kv_heads above 65535");
     DeviceScope ds(P->device);

@@ -127,10 +127,12 @@ cudaError_t launch_rows_t(const BoundedParams& p, cudaStream_t st) {
 // ------------------------------------------------------------------ weights
 // Weights from K once more: a key's row in registers, its score with every row of the sequence that
 // sees it recomputed, probability 2^(s - m) / l from the row's statistics. One owner per key and a
-// fixed order of addition: no atomics. BY_ROW = false: one CTA per (touched block, KV head), a warp
-// takes every eighth key and all rows. BY_ROW = true (16 rows and more): one CTA per (touched block,
-// KV head, key), the rows dealt to its eight warps, whose sums are added in order; with a warp per key
-// a 191-row chunk of 48 (block, head)s kept 192 warps busy and took 0.9 ms.
+// fixed order of addition: no atomics. For what neither cc_attn_kernel nor tile_weight_kernel sums: few
+// columns in several rows or groups, head sizes above 256 or no multiples of 4. BY_ROW = false: one CTA
+// per (touched block, KV head), a warp takes every eighth key and all rows. BY_ROW = true (16 rows and
+// more): one CTA per (touched block, KV head, key), the rows dealt to its eight warps, whose sums are
+// added in order; with a warp per key a 191-row chunk of 48 (block, head)s kept 192 warps busy and took
+// 0.9 ms.
 template <typename T, typename IO, int DPL, bool BY_ROW>
 __global__ void __launch_bounds__(256) weight_rows_kernel(const BoundedParams p, const WeightParams w) {
     constexpr int NW = 8;
@@ -508,6 +510,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
 // whose new table names some of its old blocks is one item, so that its tiles run in order (see
 // evict_select_kernel). HBM bound: every kept row is read and written once.
 constexpr int kMoveThreads = 256, kMovePer = 8, kMoveWords = kMoveThreads * kMovePer;
+static_assert(kMoveWords >= kMaxBoundedDim, "a tile holds a row of any word size");
 template <typename W>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
     __shared__ int64_t src[kMoveThreads], dst[kMoveThreads];  // first word of each row of the tile

@@ -12,6 +12,8 @@ namespace pk {
 constexpr int kMaxCols = 16;
 // Largest number of KV heads the tensor-core kernel maps to warps of one CTA.
 constexpr int kTcMaxKvHeads = 8;
+// Largest head_dim of bounded steps and evictions (a row of 16-, 4- or 2-byte words).
+constexpr int kMaxBoundedDim = 512;
 constexpr int kChunkKeys = 64;  // keys per tile of the bounded chunk kernel
 constexpr int kWideKeys = 128;  // keys per tile of the wide-tile kernel (a multiple of block_size)
 

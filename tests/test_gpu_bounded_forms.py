@@ -249,3 +249,18 @@ def test_weights_of_few_columns(shape, mode):
     """Rows on one kernel, their weights on another: by rows or in tiles, side by side in one step."""
     c = Case(*shape, [150, 90, 333, 0, 64], [7, 1, 1, 19, 4], window=120, sinks=2, weights=mode)
     c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype, D", [("bfloat16", 513), ("bfloat16", 2051), (np.float32, 1024), (np.float32, 2050)])
+def test_head_sizes_beyond_the_kernels_are_refused(dtype, D):
+    torch = torch_cuda()
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import PagedBatch, PagedKVPool
+
+    pool = PagedKVPool(Shape(1, 1, D), 2, 16, dtype, track_weights=True)
+    with pytest.raises(_lib.PagedKVError, match="head_dim"):
+        pool.evict([[0]], [9], 4)
+    x = torch.zeros((1, 1, D), device="cuda")
+    with pytest.raises(_lib.PagedKVError, match="head_dim"):
+        PagedBatch(pool, [[0]], [3], [1], window=2).write_and_attend(0, x, x, x)
+    assert not bool(pool.k.any())
