@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const WideParams p, co
 // x + 4, so it was done with x), and S^T through two TMEM buffers; at 106 KB of shared memory and 256
 // TMEM columns two CTAs share an SM, so that one's exponentials run beside the other's loads and
 // MMAs. Bound: one exponential per score, 16 per clock and SM, twice the MMA's time; 63 % of that rate
-// (85 us for 1024 rows of 32 heads over 5120 keys; with the column masks in every tile and four epilogue
+// (85 us for 2048 rows of 32 heads behind 2048 tokens; with the column masks in every tile and four epilogue
 // warps 108, the integer pipe busier than the exponentials).
 constexpr int kGThreads = 320;  // producer, MMA issuer, 8 epilogue warps: two per 32 keys, 64 columns each
 constexpr int kGOffK = 0;

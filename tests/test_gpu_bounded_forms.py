@@ -264,3 +264,12 @@ def test_head_sizes_beyond_the_kernels_are_refused(dtype, D):
     with pytest.raises(_lib.PagedKVError, match="head_dim"):
         PagedBatch(pool, [[0]], [3], [1], window=2).write_and_attend(0, x, x, x)
     assert not bool(pool.k.any())
+
+
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("shape, new", [(("bf16", 8, 8, 128, 16), 33), (("bf16", 1, 1, 128, 128), 40),
+                                        (("bf16", 128, 1, 128, 16), 1), (("bf16", 128, 1, 128, 32), 3)], ids=str)
+def test_chunks_smaller_than_a_query_tile(shape, new, weights):
+    """A step of fewer rows than one query tile has tokens, and one token that fills it."""
+    c = Case(*shape, [100], [new], window=77, sinks=2, weights=weights)
+    c.check(c.run())
