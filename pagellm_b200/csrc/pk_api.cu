@@ -237,6 +237,7 @@ struct pk_pool {
     bool tc_ok = false;
     int tc_per_head = 0;
     int tc_stages = 0;
+    int tc_part_stages = 0;  // of bounded steps (tc_bs slots each)
     size_t tc_smem = 0;
     int tc_virt = 1;  // virtual split-KV CTAs per CTA (8 / kvh for pools of few KV heads)
     int smem_optin = 0;  // largest dynamic shared memory a CTA may opt in to
@@ -245,6 +246,10 @@ struct pk_pool {
     CUtensorMap tmv{};
     // wide-tile (tcgen05) kernel: one (block, head, 64-dim chunk) per TMA box
     bool wide_ok = false;
+    // bounded steps: slots of a split-KV stage (the block, or a part of it where the block is too large for
+    // two stages; 0: no tensor-core path), and whether chunk_attn_kernel takes their chunks
+    int tc_bs = 0;
+    bool chunk_ok = false;
     CUtensorMap tmk1{};
     CUtensorMap tmv1{};
     // bounded chunk kernel: the same with at most kChunkKeys slots of a block per box
@@ -349,6 +354,7 @@ struct pk_batch {
     std::vector<int32_t> t_piece;       // per touched block of a chunk: first piece of its tile, pieces
     DevBuf wpieces;                     // [pieces][kvh][128] sums
     DevBuf row_lse;                     // [chunk items][kvh][128] log-sum-exp of the rows
+    std::vector<int32_t> part_ids;      // table entries of parts of blocks (tc_parts > 1)
     std::vector<int32_t> u_bound;       // per unit: table entries in front of the jump, the jump, score place
     std::vector<int32_t> seq_u;         // [nseq + 1] first unit of each sequence
     std::vector<int32_t> t_meta;        // records of the first ntouch_tc touched blocks
@@ -469,13 +475,13 @@ bool encode_pool_maps(pk_pool* P, int layout, std::string* why) {
         strides[0] = static_cast<cuuint64_t>(P->kvh) * P->d * 2;
         strides[1] = static_cast<cuuint64_t>(P->d) * 2;
         strides[2] = 128;
-        box[0] = 64; box[1] = P->block_size; box[2] = P->kvh; box[3] = chunks;
+        box[0] = 64; box[1] = P->tc_bs; box[2] = P->kvh; box[3] = chunks;
     } else {
         dims[0] = 64; dims[1] = chunks; dims[2] = P->kvh; dims[3] = slots;
         strides[0] = 128;
         strides[1] = static_cast<cuuint64_t>(P->d) * 2;
         strides[2] = static_cast<cuuint64_t>(P->kvh) * P->d * 2;
-        box[0] = 64; box[1] = chunks; box[2] = 1; box[3] = P->block_size;
+        box[0] = 64; box[1] = chunks; box[2] = 1; box[3] = P->tc_bs;
     }
     for (int t = 0; t < 2; ++t) {
         CUresult r = enc(t == 0 ? &P->tmk : &P->tmv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
@@ -505,22 +511,45 @@ void setup_tc(pk_pool* P) {
     int optin = 0;
     cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, P->device);
     P->smem_optin = optin;
-    const size_t stage = static_cast<size_t>(2) * P->block_size * P->kvh * P->d * 2;
     // A CTA has one consumer warp per KV head of each of its V virtual CTAs. With few KV heads
     // (the head-sharded layout gives 1-4 per GPU) V = 8 / kvh virtual CTAs - each its own block
     // range, stage ring and barriers - keep 8 consumer warps per SM under one producer warp
     // (several 2-warp CTAs per SM would spend half the register file on producers). Stages: as
     // many as fit (at most 8); V is lowered while fewer than 3 fit.
-    int stages = 0;
-    for (int v = std::max(1, pk::kTcMaxKvHeads / P->kvh); v >= 1; --v) {
-        const size_t budget = std::min<size_t>(static_cast<size_t>(optin), size_t(200) << 10);
-        stages = 8;
-        while (stages >= 2 && pk::tc_smem_bytes(P->d, P->block_size, P->kvh, stages, v) > budget) --stages;
-        P->tc_virt = v;
-        if (stages >= 3 || v == 1) break;
+    auto stages_for = [&](int slots_per_stage) {
+        int stages = 0;
+        for (int v = std::max(1, pk::kTcMaxKvHeads / P->kvh); v >= 1; --v) {
+            const size_t budget = std::min<size_t>(static_cast<size_t>(optin), size_t(200) << 10);
+            stages = 8;
+            while (stages >= 2 && pk::tc_smem_bytes(P->d, slots_per_stage, P->kvh, stages, v) > budget) --stages;
+            P->tc_virt = v;
+            if (stages >= 3 || v == 1) break;
+        }
+        return stages;
+    };
+    P->tc_bs = P->block_size;
+    int stages = stages_for(P->tc_bs);
+    std::string why2;
+    auto chunk_fits = [&]() {
+        return P->d == 128 && pk::kWideKeys % P->block_size == 0 &&
+               static_cast<size_t>(optin) >= std::max(pk::wide_smem_bytes(), pk::chunk_smem_bytes()) && encode_chunk_maps(P, &why2);
+    };
+    if (stages < 2) {
+        // Bounded steps stream the largest part of a block that leaves three stages (8 KV heads of 128 with
+        // 32-slot blocks: 16 slots), under table entries of their own (build_attention_plan): 64 decodes 52 us,
+        // 323 on the CUDA cores.
+        do P->tc_bs -= 16;
+        while (P->tc_bs >= 16 && (P->block_size % P->tc_bs != 0 || stages_for(P->tc_bs) < 3));
+        std::string why;
+        if (P->tc_bs >= 16 && encode_pool_maps(P, 0, &why)) {
+            P->tc_part_stages = stages_for(P->tc_bs);
+            P->tc_smem = pk::tc_smem_bytes(P->d, P->tc_bs, P->kvh, P->tc_part_stages, P->tc_virt);
+            P->chunk_ok = chunk_fits();
+        } else {
+            P->tc_bs = 0;
+        }
+        return no("K/V block too large for two shared-memory stages");
     }
-    (void)stage;
-    if (stages < 2) return no("K/V block too large for two shared-memory stages");
     std::string why;
     if (encode_pool_maps(P, 0, &why)) {
         P->tc_per_head = 0;
@@ -528,17 +557,15 @@ void setup_tc(pk_pool* P) {
         P->tc_per_head = 1;
     } else {
         P->tc_why = why;
+        P->tc_bs = 0;
         return;
     }
-    P->tc_stages = stages;
+    P->tc_stages = P->tc_part_stages = stages;
     P->tc_smem = pk::tc_smem_bytes(P->d, P->block_size, P->kvh, stages, P->tc_virt);
     P->tc_ok = true;
     P->tc_why.clear();
     // wide tiles: head_dim 128, 128-key tiles made of whole blocks, the layout-0 view
-    std::string why2;
-    P->wide_ok = P->d == 128 && pk::kWideKeys % P->block_size == 0 && P->tc_per_head == 0 &&
-                 static_cast<size_t>(optin) >= std::max(pk::wide_smem_bytes(), pk::chunk_smem_bytes()) &&
-                 encode_chunk_maps(P, &why2);
+    P->wide_ok = P->chunk_ok = P->tc_per_head == 0 && chunk_fits();
 }
 
 // log2 of a power of two, else -1
@@ -663,7 +690,7 @@ constexpr double kSplitKvBytesPerUs = 6.0e6;  // split-KV streaming rate (HBM / 
 // over the K+V bytes of one block.
 int64_t unit_switch_blocks(const pk_pool* P, int64_t ctas) {
     const double cta_rate = kSplitKvBytesPerUs / static_cast<double>(std::max<int64_t>(1, ctas));
-    const double blk = static_cast<double>(P->block_bytes()) * 2.0;
+    const double blk = static_cast<double>(P->block_bytes()) * 2.0 * P->tc_bs / P->block_size;
     const double us = P->tc_virt > 1 ? kUnitSwitchUsVirtual : kUnitSwitchUs;
     return std::max<int64_t>(0, std::llround(us * cta_rate / blk));
 }
@@ -1060,6 +1087,11 @@ int plan_tiles(pk_batch* B, int H) {
     return PK_OK;
 }
 
+// Parts of a block that the split-KV kernel of a bounded step takes one by one (1: whole blocks).
+int tc_parts(const pk_batch* B) {
+    return B->bounded() && B->pool->tc_bs > 0 ? B->pool->block_size / B->pool->tc_bs : 1;
+}
+
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
@@ -1075,7 +1107,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nt = 1;
     int qmax = 0;
     // (bounded modes know only the layout that one box brings per block)
-    if (P->tc_ok && g <= pk::kMaxCols && !(B->bounded() && P->tc_per_head)) {
+    if ((B->bounded() ? P->tc_bs > 0 && !P->tc_per_head : P->tc_ok) && g <= pk::kMaxCols) {
         qmax = std::max(1, pk::kMaxCols / g);
         if (P->d == 256) qmax = g <= 8 ? std::max(1, 8 / g) : 0;  // one n8 tile only at D=256
     }
@@ -1084,7 +1116,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->nwide = B->nprefix = B->nprefix_groups = 0;
     B->prefix_keys = B->prefix_token_keys = 0;
     B->seq_kb0.assign(B->nseq, 0);
-    const bool wide_ok = P->wide_ok && g <= 128 && 128 % g == 0;
+    const bool wide_ok = (B->bounded() ? P->chunk_ok : P->wide_ok) && g <= 128 && 128 % g == 0;
     const int tpt = wide_ok ? 128 / g : 0;  // query tokens per wide item
     const bool tile_ok = B->bounded() && P->d % 4 == 0 && P->d <= pk::kTileMaxDim && g <= pk::kTileCols && P->kvh <= 65535;
     B->seq_tile.assign(B->nseq, 0);
@@ -1136,11 +1168,11 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
             const int64_t ctx = static_cast<int64_t>(B->starts[i]) + t0 + nu;
             if (B->bounded()) {
                 const VisibleBlocks vb = visible_blocks(static_cast<int64_t>(B->starts[i]) + t0, ctx, B->window, B->sinks,
-                                                        P->block_size);
+                                                        P->tc_bs);
                 T += vb.count;
                 B->u_bound.insert(B->u_bound.end(), {vb.head, vb.skip, static_cast<int32_t>(static_cast<uint32_t>(score_floats)),
                                                      static_cast<int32_t>(score_floats >> 32)});
-                score_floats += vb.count * P->block_size * ((nu * g + 1) & ~1) * P->kvh;
+                score_floats += vb.count * P->tc_bs * ((nu * g + 1) & ~1) * P->kvh;
                 B->seq_u[i + 1]++;
             } else {
                 T += ceil_div(ctx, P->block_size) - kb0;
@@ -1284,6 +1316,8 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (!B->use_tc) B->u_cta.clear();
     B->plan.add(B->u_cta.data(), B->u_cta.size() * 4);  // 23
     // packed unit records: {t0, n, kb0, row0}, {qpos0, blk0, blk1, tbase}
+    // (a step in parts of blocks: tbase counts entries of part_ids)
+    const int parts = tc_parts(B);
     B->u_meta.resize(8 * static_cast<size_t>(B->nu));
     for (int u = 0; u < B->nu; ++u) {
         const int i = B->u_seq[u];
@@ -1295,7 +1329,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
         r[4] = B->starts[i] + B->u_t0[u];
         r[5] = B->u_blk[u];
         r[6] = B->u_blk[u + 1];
-        r[7] = B->indptr[i] + B->u_kb0[u] - B->u_blk[u];
+        r[7] = B->indptr[i] * parts + B->u_kb0[u] - B->u_blk[u];
     }
     B->plan.add(B->u_meta.data(), B->u_meta.size() * 4);  // 24
     // pool slots of the wide-item rows, for their append
@@ -1314,8 +1348,10 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->t_meta.clear();
     for (int x = 0; x < B->ntouch_tc; ++x) {
         const int i = B->t_seq[x];
-        B->t_meta.insert(B->t_meta.end(), {B->ids[B->indptr[i] + B->t_blk[x]], B->t_blk[x], B->seq_u[i], B->seq_u[i + 1],
-                                           B->starts[i], B->starts[i] + B->nnew[i], 0, 0});
+        for (int y = 0; y < parts; ++y)
+            B->t_meta.insert(B->t_meta.end(), {B->ids[B->indptr[i] + B->t_blk[x]], B->t_blk[x] * parts + y, B->seq_u[i],
+                                               B->seq_u[i + 1], B->starts[i], B->starts[i] + B->nnew[i],
+                                               y * P->tc_bs, 0});
     }
     B->plan.add(B->t_meta.data(), B->t_meta.size() * 4);  // 29
     B->plan.add(B->pair_bound.data(), B->pair_bound.size() * 4);  // 30
@@ -1330,6 +1366,11 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan.add(B->tile_meta.data(), B->tile_meta.size() * 4);  // 35
     B->plan.add(B->wtile_meta.data(), B->wtile_meta.size() * 4);  // 36
     B->plan.add(B->tile_zero.data(), B->tile_zero.size() * 4);  // 37
+    B->part_ids.clear();
+    if (parts > 1 && B->use_tc)
+        for (int32_t b : B->ids)
+            for (int y = 0; y < parts; ++y) B->part_ids.push_back(b * parts + y);
+    B->plan.add(B->part_ids.data(), B->part_ids.size() * 4);  // 38
     if (B->weights_mode != 0)
         PK_CUDA(B->ml.reserve(static_cast<size_t>(std::max<int64_t>(B->nrows, 1)) * H * sizeof(float2)));
     if (B->nslots > 0)
@@ -1434,7 +1475,7 @@ pk::TcParams tc_params(pk_batch* B, int layer, int H, const float* q, float* out
     p.part_ml = static_cast<float*>(B->ws.ptr) + B->ws_part_o_floats;
     p.err = static_cast<int*>(B->err.ptr);
     p.indptr = B->meta.at<int32_t>(0);
-    p.ids = B->meta.at<int32_t>(1);
+    p.ids = tc_parts(B) > 1 ? B->plan.at<int32_t>(38) : B->meta.at<int32_t>(1);
     p.starts = B->meta.at<int32_t>(2);
     p.offsets = B->meta.at<int32_t>(3);
     p.u_seq = B->plan.at<int32_t>(0);
@@ -1452,8 +1493,8 @@ pk::TcParams tc_params(pk_batch* B, int layer, int H, const float* q, float* out
     p.kvh = P->kvh;
     p.g = H / P->kvh;
     p.H = H;
-    p.bs = P->block_size;
-    p.stages = P->tc_stages;
+    p.bs = P->tc_bs;
+    p.stages = P->tc_part_stages;
     p.virt = P->tc_virt;
     p.per_head_layout = P->tc_per_head;
     p.layer_slot0 = static_cast<int64_t>(layer) * P->num_blocks * P->block_size;
@@ -1857,7 +1898,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         w.weights = P->weights + static_cast<int64_t>(layer) * P->layer_weights();
         w.t_seq = B->plan.at<int32_t>(26);
         w.t_blk = B->plan.at<int32_t>(27);
-        w.ntouched = B->ntouch_tc;
+        w.ntouched = B->ntouch_tc * tc_parts(B);
         w.add = B->weights_mode == 1;
         if (w.ntouched > 0) {
             pk::ScoreWeightParams sw{};
@@ -1870,8 +1911,9 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             sw.kvh = p.kvh;
             sw.g = H / p.kvh;
             sw.H = H;
-            sw.bs = p.bs;
-            sw.bs_shift = log2_or_minus(p.bs);
+            sw.bs = P->tc_bs;
+            sw.bs_shift = log2_or_minus(P->tc_bs);
+            sw.block = p.bs;
             sw.window = p.window;
             sw.sinks = p.sinks;
             for (int i = 0; i < B->nseq; ++i) sw.max_units = std::max(sw.max_units, B->seq_u[i + 1] - B->seq_u[i]);

@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(256, 1) weight_scores_kernel(const ScoreWeight
     const int4 r0 = __ldg(p.t_meta + 2 * e), r1 = __ldg(p.t_meta + 2 * e + 1);
     const int phys = r0.x, lb = r0.y, u0 = r0.z, u1 = r0.w, start = r1.x, ctx = r1.y;
     const int pairs = p.kvh * p.bs;
-    float* wb = p.w.weights + static_cast<size_t>(phys) * pairs;
+    float* wb = p.w.weights + static_cast<size_t>(phys) * p.kvh * p.block + r1.z;
+    auto place = [&](int h, int t) { return wb + h * p.block + t; };
     for (int x0 = lane + (MANY ? 32 * static_cast<int>(blockIdx.y) : 0); MANY || x0 < pairs; x0 += 32 * kPer) {
         float sum[kPer], old[kPer];
         int h[kPer], t[kPer];
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(256, 1) weight_scores_kernel(const ScoreWeight
             const int j = lb * p.bs + t[k];
             live[k] = x < pairs && j < ctx && (j < p.sinks || j > start - p.window);
             sum[k] = 0.f;
-            old[k] = live[k] && p.w.add && j < start ? wb[x] : 0.f;
+            old[k] = live[k] && p.w.add && j < start ? *place(h[k], t[k]) : 0.f;
         }
         for (int u = u0 + (MANY ? warp : 0); u < u1; u += MANY ? NW : 1) {
             const int4 b = __ldg(p.u_bound + u);
@@ -272,13 +273,13 @@ __global__ void __launch_bounds__(256, 1) weight_scores_kernel(const ScoreWeight
             if (warp == 0 && live[0]) {
                 float total = old[0];
                 for (int x = 0; x < NW; ++x) total += part[x][lane];
-                wb[x0] = total;
+                *place(h[0], t[0]) = total;
             }
             return;
         }
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
-            if (live[k]) wb[x0 + 32 * k] = old[k] + sum[k];
+            if (live[k]) *place(h[k], t[k]) = old[k] + sum[k];
     }
 }
 

@@ -305,7 +305,7 @@ struct WeightParams {
 struct ScoreWeightParams {
     WeightParams w;
     const int4* t_meta;     // [ntouched][2] {block id, table index, first and end unit of the sequence},
-                            // {first new position, context, 0, 0}
+                            // {first new position, context, first slot of the part, 0}
     const float* score;
     const float2* ml;
     const int4* u_meta;     // units as in TcParams
@@ -315,6 +315,7 @@ struct ScoreWeightParams {
     int H;
     int bs;
     int bs_shift;           // log2 of bs, or -1
+    int block;              // slots of a block (bs, or more: entries are parts of blocks)
     int window;
     int sinks;
     int max_units;          // most units of a sequence

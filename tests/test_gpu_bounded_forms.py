@@ -273,3 +273,19 @@ def test_chunks_smaller_than_a_query_tile(shape, new, weights):
     """A step of fewer rows than one query tile has tokens, and one token that fills it."""
     c = Case(*shape, [100], [new], window=77, sinks=2, weights=weights)
     c.check(c.run())
+
+
+@pytest.mark.parametrize("bounds", [(None, 0), (70, 3), (1, 40), (33, 100)])
+@pytest.mark.parametrize("weights", [None, "add"])
+@pytest.mark.parametrize("shape", [("bf16", 32, 8, 128, 32), ("bf16", 40, 8, 128, 64), ("bf16", 16, 4, 256, 32),
+                                   ("bf16", 8, 8, 128, 128), ("bf16", 6, 2, 256, 64), ("bf16", 16, 8, 128, 256),
+                                   ("bf16", 8, 8, 64, 96)], ids=_shape)
+def test_blocks_too_large_for_two_stages(shape, weights, bounds):
+    """The split-KV kernel takes such blocks in parts."""
+    c = Case(*shape, [0, 31, 300, 129, 64, 500], [1, 3, 1, 60, 0, 9], window=bounds[0], sinks=bounds[1], weights=weights)
+    c.check(c.run())
+    d = Case(*shape, [0, 31, 300, 64, 255, 256, 700], [1] * 7, window=bounds[0], sinks=bounds[1], weights=weights, seed=1)
+    b = d.batch()
+    d.check(d.run(b))
+    if bounds[0] or weights:  # (a plain step has them on the CUDA cores)
+        assert b.stats()["generic_rows"] == 0
