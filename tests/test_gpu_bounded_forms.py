@@ -289,3 +289,22 @@ def test_blocks_too_large_for_two_stages(shape, weights, bounds):
     d.check(d.run(b))
     if bounds[0] or weights:  # (a plain step has them on the CUDA cores)
         assert b.stats()["generic_rows"] == 0
+
+
+@pytest.mark.parametrize("shape", [("bf16", 32, 8, 128, 32), ("bf16", 16, 8, 128, 64), ("bf16", 16, 4, 256, 32)], ids=_shape)
+def test_parts_of_blocks_with_float_rows_layers_and_graphs(shape):
+    torch = torch_cuda()
+    for new in ([1, 1, 1, 1], [1, 70, 2, 0]):
+        c = Case(*shape, [300, 31, 64, 5], new, window=90, sinks=3, weights="add", io="fp32", layers=2, layer=1)
+        b = c.batch()
+        # q at bf16 where the kernel has no room for its low half
+        c.check(c.run(b), q_step=2.0 ** -8)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = b.write_and_attend(1, c.q, c.k, c.v)
+        for _ in range(2):
+            c.pool.weights.copy_(c.before)
+            graph.replay()
+            torch.cuda.synchronize()
+            c.check(got, q_step=2.0 ** -8)
+        b.check()
