@@ -133,6 +133,7 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
  * read must appear only once in the step (PK_ERR_INVALID_ARG from pk_batch_plan otherwise).
  * A K or V that is not finite in a place that one row of a sequence's step sees may reach the
  * sequence's other rows of the step; places that none sees are not read.
+ * Contexts within 65536 of 2^31 tokens and a head_dim above 512 are refused (PK_ERR_UNSUPPORTED).
  * After a change the batch has to be planned again before it attends. A bounded step's first
  * call with some n_heads cannot be captured (PK_ERR_UNSUPPORTED); later ones can, and graphs
  * that were captured from one batch share its scratch: replay them one after another. */

@@ -980,8 +980,11 @@ void plan_weight_pieces(pk_batch* B, const std::vector<int32_t>& ts, const std::
 // Bounded rows on the CUDA cores. Splits: enough CTAs for kCcCtasPerSm per SM, as long as a split
 // keeps kCcMinKeys visible keys of the average row. Weights are summed in the same launch when every
 // such sequence has one row, a CTA has all of its KV head's query heads and all keys, and the scores
-// fit kCcScoreBytes of shared memory.
+// fit kCcScoreBytes of shared memory - unless few CTAs would then walk long contexts alone: 16 x 8 KV
+// heads over 2000 tokens 135 us fused, 208 split and summed by rows; 8 x 4 heads 71 and 56, one
+// sequence of 8 heads 92 and 39; 8 x 2 heads over 512 tokens 19 and 21.
 constexpr int64_t kCcCtasPerSm = 4, kCcMinKeys = 128, kCcScoreBytes = 64 * 1024;
+constexpr int64_t kCcFuseKeys = 256;
 int plan_cc(pk_batch* B, int H) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
@@ -1014,7 +1017,8 @@ int plan_cc(pk_batch* B, int H) {
     const int64_t room = std::max<int64_t>(1, vis / nrows / kCcMinKeys);
     B->cc_nsplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, room, 256})));
     B->cc_max_vis = static_cast<int>(most);
-    B->cc_weights = B->weights_mode != 0 && single && g <= G && most * G * 4 <= kCcScoreBytes;
+    B->cc_weights = B->weights_mode != 0 && single && g <= G && most * G * 4 <= kCcScoreBytes &&
+                    (2 * ctas >= P->num_sms || most <= kCcFuseKeys);
     if (B->cc_weights) B->cc_nsplit = 1;
     if (B->cc_nsplit > 1) {
         PK_CUDA(B->cc_part.reserve(static_cast<size_t>(ctas) * B->cc_nsplit * G * (P->d + 2) * sizeof(float)));
