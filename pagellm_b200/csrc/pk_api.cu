@@ -375,7 +375,9 @@ struct pk_batch {
     DevBuf score;                       // raw scores of a split-KV launch with weights
     bool use_scores = false;
     DevBuf ml;  // [rows][H] softmax statistics of a step with weights
-    cudaStream_t plan_stream = nullptr;  // stream of the last uploads
+    // streams of the last uploads: the tables (pk_batch_plan) and the attention plan, which the first
+    // call makes on its own stream
+    cudaStream_t meta_stream = nullptr, plan_stream = nullptr;
     cudaEvent_t ev_bounded = nullptr;    // end of the last bounded call
     bool used = false;
     bool bounded() const { return window > 0 || weights_mode != 0; }
@@ -1688,14 +1690,14 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         if (rc != PK_OK) return rc;
     }
     if (B->nrows == 0) return PK_OK;
-    if (st != B->plan_stream) {
-        // the plan came over on another stream; a capture cannot wait for it, and follows a
-        // call that did (build_attention_plan)
+    if (st != B->meta_stream || st != B->plan_stream) {
+        // the tables or the plan came over on another stream; a capture cannot wait for them, and
+        // follows a call that did (build_attention_plan)
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
         PK_CUDA(cudaStreamIsCapturing(st, &capturing));
         if (capturing == cudaStreamCaptureStatusNone) {
-            PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
-            PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
+            if (st != B->meta_stream) PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
+            if (st != B->plan_stream) PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
         }
     }
     // decode steps append inside the split-KV kernel and chunk rows with the packing of their
@@ -2542,7 +2544,7 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     DeviceScope ds(P->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     PK_CUDA(wait_used(B, st));
-    B->plan_stream = st;
+    B->meta_stream = st;
     B->meta.begin();
     B->meta.add(B->indptr.data(), B->indptr.size() * 4);
     B->meta.add(B->ids.data(), B->ids.size() * 4);
