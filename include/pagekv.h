@@ -135,8 +135,11 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
  * sequence's other rows of the step; places that none sees are not read.
  * Contexts within 65536 of 2^31 tokens and a head_dim above 512 are refused (PK_ERR_UNSUPPORTED).
  * After a change the batch has to be planned again before it attends. A bounded step's first
- * call with some n_heads cannot be captured (PK_ERR_UNSUPPORTED); later ones can, and graphs
- * that were captured from one batch share its scratch: replay them one after another. */
+ * call with some n_heads cannot be captured (PK_ERR_UNSUPPORTED); later ones can.
+ * All calls of a batch share its scratch. Bounded calls on different streams therefore run in the
+ * order of the calls, behind the plan's uploads (what they read and write beyond the batch - rows,
+ * the pool - is the caller's to order); graphs that were captured from one batch are the caller's to
+ * replay one after another, and not while other calls of the batch run. */
 PK_API int pk_batch_set_bounds(pk_batch* batch, int64_t window, int64_t sinks, int weights_mode);
 PK_API int pk_batch_destroy(pk_batch* batch);
 /* PagedBatch.__init__ (:397-439). Host arrays: block tables in CSR form

@@ -378,7 +378,10 @@ struct pk_batch {
     // streams of the last uploads: the tables (pk_batch_plan) and the attention plan, which the first
     // call makes on its own stream
     cudaStream_t meta_stream = nullptr, plan_stream = nullptr;
-    cudaEvent_t ev_bounded = nullptr;    // end of the last bounded call
+    // End of the last bounded call, and its stream. Later calls and plans on another stream wait for it
+    // (wait_last), so that one event stands for all calls before it.
+    cudaEvent_t ev_bounded = nullptr;
+    cudaStream_t last_stream = nullptr;
     bool used = false;
     bool bounded() const { return window > 0 || weights_mode != 0; }
     int launches = 0;
@@ -1098,13 +1101,25 @@ int tc_parts(const pk_batch* B) {
     return B->bounded() && B->pool->tc_bs > 0 ? B->pool->block_size / B->pool->tc_bs : 1;
 }
 
+// Before uploads and kernels on `st`, which is not being captured: those of the last bounded call, where it
+// came on another stream, still read the tables and the plan and use the scratch (scores, statistics,
+// partials and their counters).
+cudaError_t wait_last(pk_batch* B, cudaStream_t st) {
+    return B->used && st != B->last_stream ? cudaStreamWaitEvent(st, B->ev_bounded, 0) : cudaSuccess;
+}
+
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
     B->plan_H = -1;
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (B->bounded() && cudaStreamIsCapturing(st, &capturing) == cudaSuccess && capturing != cudaStreamCaptureStatusNone)
-        return fail(PK_ERR_UNSUPPORTED, "plan the step before a stream capture (call once with the same n_heads)");
+    if (B->bounded() || B->used) {
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+        if (capturing == cudaStreamCaptureStatusNone)
+            PK_CUDA(wait_last(B, st));
+        else if (B->bounded())
+            return fail(PK_ERR_UNSUPPORTED, "plan the step before a stream capture (call once with the same n_heads)");
+    }
     B->u_seq.clear(); B->u_t0.clear(); B->u_n.clear(); B->u_blk.assign(1, 0);
     B->sp_u.clear(); B->sp_c0.clear(); B->sp_c1.clear(); B->gen_rows.clear();
     B->cta_blk.assign(1, 0);
@@ -1389,14 +1404,6 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     B->plan_stream = st;
     B->plan_H = H;
     return PK_OK;
-}
-
-// Before the uploads of a bounded step's plan: kernels of the last bounded call, perhaps on
-// another stream, still read what they replace.
-cudaError_t wait_used(pk_batch* B, cudaStream_t st) {
-    if (!B->used) return cudaSuccess;
-    B->used = false;
-    return cudaStreamWaitEvent(st, B->ev_bounded, 0);
 }
 
 // Kinds reported by pk_batch_profile_read.
@@ -1690,15 +1697,15 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         if (rc != PK_OK) return rc;
     }
     if (B->nrows == 0) return PK_OK;
-    if (st != B->meta_stream || st != B->plan_stream) {
-        // the tables or the plan came over on another stream; a capture cannot wait for them, and
-        // follows a call that did (build_attention_plan)
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
-        if (capturing == cudaStreamCaptureStatusNone) {
-            if (st != B->meta_stream) PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
-            if (st != B->plan_stream) PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
-        }
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+    const bool captured = capturing != cudaStreamCaptureStatusNone;
+    if (!captured) {
+        // The last call, and uploads of the tables and the plan, on other streams. A capture cannot wait
+        // for them: it follows a call that did (build_attention_plan).
+        PK_CUDA(wait_last(B, st));
+        if (st != B->meta_stream) PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
+        if (st != B->plan_stream) PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
     }
     // decode steps append inside the split-KV kernel and chunk rows with the packing of their
     // queries, as in plain steps
@@ -1754,9 +1761,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
         if (rc != PK_OK) return rc;
     } else if (B->nwide > 0) {
         const size_t bytes = (B->w_seq.size() * P->kvh + 1) * static_cast<size_t>(pk::kWideQTileBytes);
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
-        if (bytes > B->qpk.cap && capturing != cudaStreamCaptureStatusNone)
+        if (bytes > B->qpk.cap && captured)
             return fail(PK_ERR_UNSUPPORTED, "the first call with float rows cannot be captured: call once before");
         PK_CUDA(B->qpk.reserve(bytes));
     }
@@ -1959,11 +1964,10 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             B->launches++;
         }
     }
-    if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    PK_CUDA(cudaStreamIsCapturing(st, &capturing));
-    if (capturing == cudaStreamCaptureStatusNone) {
+    if (!captured) {
+        if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
         PK_CUDA(cudaEventRecord(B->ev_bounded, st));
+        B->last_stream = st;
         B->used = true;
     }
     return PK_OK;
@@ -2543,7 +2547,7 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     if (n_rows) *n_rows = rows;
     DeviceScope ds(P->device);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    PK_CUDA(wait_used(B, st));
+    PK_CUDA(wait_last(B, st));
     B->meta_stream = st;
     B->meta.begin();
     B->meta.add(B->indptr.data(), B->indptr.size() * 4);

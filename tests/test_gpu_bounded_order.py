@@ -44,3 +44,71 @@ def test_the_first_call_on_another_stream_follows_the_tables(shape, weights):
     torch.cuda.synchronize()
     b.check()
     c.check(out)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=_shape)
+def test_calls_of_one_batch_on_several_streams(shape):
+    """They share scores, statistics, partials and counters: as one after the other, here with split keys,
+    chunks and weights, the last call's in the end."""
+    torch = torch_cuda()
+    c = Case(*shape, [9000, 40, 700, 90], [1, 60, 5, 300], window=5000, sinks=4, weights="replace")
+    b = c.batch()
+    qs = [c.q] + [torch.randn_like(c.q) for _ in range(3)]
+    want = []
+    for q in qs:
+        want.append(b.write_and_attend(0, q, c.k, c.v))
+    weights = c.pool.weights.clone()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    _busy(streams[0])
+    got = []
+    for q, s in zip(qs, streams):
+        with torch.cuda.stream(s):
+            got.append(b.write_and_attend(0, q, c.k, c.v))
+    torch.cuda.synchronize()
+    b.check()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert torch.equal(c.pool.weights, weights)
+    c.q = qs[-1]
+    c.check(got[-1])
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=_shape)
+def test_a_new_plan_follows_the_calls_before_it(shape):
+    """Other n_heads, and a recycled handle that is planned on a second stream and called on a third:
+    calls that wait on the first stream still have their own tables, plan and scratch."""
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case(*shape, [9000, 40, 700], [1, 60, 5], window=5000, sinks=4, poison=False)
+    q2 = torch.randn((c.q.shape[0], 2 * c.H, c.D), device="cuda", dtype=c.q.dtype)
+    other = dict(starts=[300, 20], n_new=[3, 70], window=90, sinks=1)
+    tables = [c.tables[0][-30:], c.tables[2]]
+    q3 = torch.randn((73, c.H, c.D), device="cuda", dtype=c.q.dtype)
+
+    def steps(streams):
+        b = c.batch()
+        b.attend(0, c.q)
+        torch.cuda.synchronize()
+        if streams[0] is not streams[1]:
+            _busy(streams[0])
+        outs = []
+        for q, s in ((c.q, streams[0]), (q2, streams[1])):
+            with torch.cuda.stream(s):
+                outs.append(b.attend(0, q))
+        del b  # its handle goes to the next batch
+        with torch.cuda.stream(streams[2]):
+            n = PagedBatch(c.pool, tables, **other)
+        with torch.cuda.stream(streams[3]):
+            outs.append(n.attend(0, q3))
+        torch.cuda.synchronize()
+        n.check()
+        return outs
+
+    c.run()
+    now = torch.cuda.current_stream()
+    want = steps([now] * 4)
+    got = steps([torch.cuda.Stream() for _ in range(4)])
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
