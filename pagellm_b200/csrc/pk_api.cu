@@ -58,10 +58,14 @@ struct DeviceScope {
     }
 };
 
-// Grow-only device allocation.
+// Grow-only device allocation, freed with its owner (on the owner's device: pk_*_destroy).
 struct DevBuf {
     void* ptr = nullptr;
     size_t cap = 0;
+    DevBuf() = default;
+    DevBuf(const DevBuf&) = delete;
+    DevBuf& operator=(const DevBuf&) = delete;
+    ~DevBuf() { release(); }
     cudaError_t reserve(size_t bytes) {
         if (bytes <= cap) return cudaSuccess;
         if (ptr) {
@@ -2147,7 +2151,6 @@ int pk_pool_destroy(pk_pool* pool) {
     DeviceScope ds(pool->device);
     pool->pairs_up.release();
     for (Uploader& u : pool->evict_up) u.release();
-    pool->evict_kept.release();
     if (pool->evict_done) cudaEventDestroy(pool->evict_done);
     if (pool->weights) cudaFree(pool->weights);
     if (pool->k) cudaFree(pool->k);
@@ -2368,18 +2371,6 @@ int pk_batch_destroy(pk_batch* B) {
     DeviceScope ds(B->pool->device);
     B->meta.release();
     B->plan.release();
-    B->rows.release();
-    B->err.release();
-    B->ws.release();
-    B->io.release();
-    B->lse.release();
-    B->wpart.release();
-    B->qpk.release();
-    B->ml.release();
-    B->score.release();
-    B->cc_part.release();
-    B->wpieces.release();
-    B->row_lse.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);
     for (cudaEvent_t e : B->ev_pool) cudaEventDestroy(e);
     if (B->ev_fork) cudaEventDestroy(B->ev_fork);

@@ -308,3 +308,37 @@ def test_parts_of_blocks_with_float_rows_layers_and_graphs(shape):
             torch.cuda.synchronize()
             c.check(got, q_step=2.0 ** -8)
         b.check()
+
+
+def test_batches_give_their_memory_back():
+    """Every scratch of a batch goes with it: here split keys of tiles, weights in parts, kept scores and chunks."""
+    torch = torch_cuda()
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import PagedBatch, PagedKVPool
+
+    lib = _lib.load()
+    bf16 = PagedKVPool(Shape(1, 8, 128), 1100, 16, "bfloat16", track_weights=True)
+    fp32 = PagedKVPool(Shape(1, 8, 128), 550, 16, track_weights=True)
+
+    def round_trip():
+        for pool, H, starts, new in ((fp32, 32, [8000], [64]), (fp32, 8, [8000], [1]), (bf16, 32, [8000, 8000], [64, 1])):
+            nb = 550
+            b = PagedBatch(pool, [list(range(i * nb, (i + 1) * nb)) for i in range(len(starts))], starts, new, weights="add")
+            rows = sum(new)
+            q, k = (torch.randn((rows, h, 128), device="cuda") for h in (H, 8))
+            b.write_and_attend(0, q, k, k)
+            b.check()
+            del b
+            for h in pool._idle_batches:
+                assert lib.pk_batch_destroy(h) == 0
+            pool._idle_batches.clear()
+            pool._batch_bounds.clear()
+
+    round_trip()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(6):
+        round_trip()
+    torch.cuda.synchronize()
+    # the device allocates 2 MB at a time; one split-key scratch alone is more than 8
+    assert free - torch.cuda.mem_get_info()[0] <= 4 << 20
