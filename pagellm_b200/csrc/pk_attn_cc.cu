@@ -53,7 +53,7 @@ template <typename T, typename IO, int G, int NV, int LPK>
 __global__ void __launch_bounds__(kWarps * 32) cc_attn_kernel(const CcParams p) {
     constexpr int KPW = 32 / LPK;                            // keys a warp takes side by side
     constexpr int KB = NV >= 4 ? 2 : 4;                      // keys of a lane group in flight
-    extern __shared__ float sm[];                            // [kWarps][G][D] outputs, then the scores (weights)
+    extern __shared__ __align__(16) float sm[];              // [kWarps][G][D] outputs (16-byte words), then the scores (weights)
     __shared__ float sm_m[kWarps][G], sm_l[kWarps][G];
     __shared__ int sh_last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

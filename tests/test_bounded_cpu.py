@@ -248,3 +248,19 @@ def test_evict_keep_orders_ties_and_nan():
     assert bo.evict_keep(w, 2, 1, 1).tolist() == [0, 7]
     assert bo.evict_keep(w, 8, 1, 1).tolist() == list(range(8))
     assert bo.evict_keep([1.0, 0.0, -0.0, 0.0], 2, 0, 0).tolist() == [0, 1]
+
+
+# ------------------------------------------------------------------ the sources
+def test_shared_memory_of_wide_words_is_declared_aligned():
+    """Dynamic shared memory lies behind a kernel's static arrays: where it is read and written in 16-byte
+    words as `sm`, its declaration has to ask for that alignment."""
+    import re
+    from pathlib import Path
+
+    csrc = Path(__file__).resolve().parents[1] / "pagellm_b200" / "csrc"
+    found = 0
+    for path in sorted(csrc.glob("*.cu")):
+        for line in re.findall(r"extern __shared__[^;]*\bsm\[\]", path.read_text()):
+            found += 1
+            assert "__align__(16)" in line, f"{path.name}: {line}"
+    assert found >= 3
