@@ -344,8 +344,9 @@ PK_API int pk_bm_can_append(pk_block_manager* m, int64_t seq, int64_t n_tokens, 
 PK_API int pk_bm_ensure_capacity(pk_block_manager* m, int64_t seq, int64_t n_tokens,
                                  int64_t write_from, int64_t* pairs_out, int64_t cap,
                                  int64_t* npairs);
-/* A sequence's hash chain (BlockTable.hashes, paged.py:142-144): length and last digest,
- * or the digest at position i. */
+/* A sequence's hash chain (BlockTable.hashes, paged.py:142-144): length and last digest (*last_len:
+ * its bytes, -1 for an empty chain, -2 for that of a sequence that pk_bm_compact has shortened, which
+ * stays empty), or the digest at position i. */
 PK_API int pk_bm_seq_hashes(pk_block_manager* m, int64_t seq, int64_t* n, uint8_t* last,
                             int64_t cap, int64_t* last_len);
 PK_API int pk_bm_seq_hash_at(pk_block_manager* m, int64_t seq, int64_t i, uint8_t* out,

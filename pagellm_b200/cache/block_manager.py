@@ -301,7 +301,7 @@ class BlockManager:
         _ck(_L().pk_bm_seq_hashes(self._n.ptr, int(seq_id), C.byref(n), buf, 64, C.byref(ln)))
         have = n.value
         full = num_computed // self.block_size
-        if full <= have:
+        if full <= have or ln.value == -2:  # -2: compacted, publishes nothing
             return
         if ln.value > 64:
             buf = C.create_string_buffer(ln.value)

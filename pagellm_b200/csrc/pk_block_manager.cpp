@@ -387,7 +387,8 @@ PK_API int pk_bm_seq_hashes(pk_block_manager* m, int64_t seq, int64_t* n, uint8_
     int rc = get_table(m, seq, &t);
     if (rc) return rc;
     *n = static_cast<int64_t>(t->hashes.size());
-    if (last_len) *last_len = t->hashes.empty() ? -1 : static_cast<int64_t>(t->hashes.back().size());
+    if (last_len)
+        *last_len = t->compacted ? -2 : t->hashes.empty() ? -1 : static_cast<int64_t>(t->hashes.back().size());
     if (last && !t->hashes.empty() && cap >= static_cast<int64_t>(t->hashes.back().size()))
         std::memcpy(last, t->hashes.back().data(), t->hashes.back().size());
     return PK_OK;

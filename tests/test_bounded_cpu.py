@@ -164,6 +164,31 @@ def test_compact_exchanges_published_blocks_and_publishes_nothing_afterwards():
     assert len(bm.alloc.cached) > len(cached)
 
 
+def test_compacted_sequences_are_not_hashed_again(monkeypatch):
+    from pagellm_b200.cache import block_manager
+
+    calls = []
+    real = block_manager.block_hash
+    monkeypatch.setattr(block_manager, "block_hash", lambda *a: calls.append(a) or real(*a))
+    bm = BlockManager(16, 4)
+    toks = list(range(24))
+    bm.allocate(1, toks)
+    bm.mark_computed(1, toks, 24)
+    assert len(calls) >= 6
+    bm.compact(1, 12)
+    bm.fork(1, 2)
+    del calls[:]
+    for n in (12, 16, 20):
+        bm.ensure_capacity(1, n, n - 4)
+        bm.mark_computed(1, toks, n)
+        bm.mark_computed(2, toks, 12)
+    assert not calls and bm.tables[1].hashes == []
+    bm.free(1)
+    bm.allocate(1, [7] * 8)  # the old id's next sequence is hashed
+    bm.mark_computed(1, [7] * 8, 8)
+    assert calls and len(bm.tables[1].hashes) == 2
+
+
 def test_compact_refusals_change_nothing():
     bm = BlockManager(6, 4, enable_prefix_caching=False)
     bm.allocate(1, list(range(16)))
