@@ -577,7 +577,9 @@ def evict_sequences(pool: PagedKVPool, manager: BlockManager, seq_ids, lengths, 
 
     A block that one sequence gives up may become another's, and the last holder of a shared
     block thins it out in place; sequences whose new blocks an earlier one still reads go into
-    a later launch."""
+    a later launch. What the pool's eviction refuses (a capturing stream, a head size beyond
+    its kernels) is refused before any table changes; an error of the device leaves the
+    sequences of its call without valid caches."""
     seq_ids = [int(s) for s in seq_ids]
     lens = np.asarray(lengths, dtype=np.int64).reshape(-1)
     if len(seq_ids) != len(lens):
@@ -589,18 +591,24 @@ def evict_sequences(pool: PagedKVPool, manager: BlockManager, seq_ids, lengths, 
         raise ValueError("budget must be at least 1 and hold sinks + recent")
     if pool.weights is None:
         raise ValueError("eviction needs a pool made with track_weights=True")
+    if getattr(pool, "block_size", manager.block_size) != manager.block_size \
+            or getattr(pool, "num_blocks", manager.alloc.num_blocks) < manager.alloc.num_blocks:
+        raise ValueError("the block manager's blocks are not the pool's")
     for s, n in zip(seq_ids, lens):
         if n < 0 or n > len(manager.block_table(s)) * manager.block_size:
             raise ValueError(f"sequence {s} does not hold {n} tokens")
+    if isinstance(pool, PagedKVPool):
+        pool.evict([], [], budget, sinks=sinks, recent=recent)  # the refusals that need no sequence
     group: list = []
     reads: set = set()
 
     def flush():
         if group:
-            pool.evict([g[0] for g in group], [g[2] for g in group], budget, sinks=sinks, recent=recent,
-                       new_tables=[g[1] for g in group])
-            group.clear()
+            todo = group.copy()
+            group.clear()  # first: a call that fails is not made again on the way out
             reads.clear()
+            pool.evict([g[0] for g in todo], [g[2] for g in todo], budget, sinks=sinks, recent=recent,
+                       new_tables=[g[1] for g in todo])
 
     try:
         for s, n in zip(seq_ids, lens.tolist()):

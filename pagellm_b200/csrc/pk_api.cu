@@ -2267,12 +2267,8 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
                   int32_t* kept_dev, void* stream) try {
     if (!P) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
     if (!P->weights) return fail(PK_ERR_INVALID_ARG, "the pool does not track attention weights (pk_pool_track_weights)");
-    const int bs = P->block_size;
-    std::lock_guard<std::mutex> lock(P->evict_mutex);  // plan, uploads and scratch are the pool's
-    EvictPlan& plan = P->evict_plan;
-    int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
-                        &plan);
-    if (rc != PK_OK || nseq == 0) return rc;
+    // what no eviction of this pool or on this stream may be, before anything that a call without
+    // sequences does not have (evict_sequences asks with one)
     if (P->d > pk::kMaxBoundedDim) return fail(PK_ERR_UNSUPPORTED, "head_dim %d > %d", P->d, pk::kMaxBoundedDim);
     if (static_cast<int64_t>(P->kvh) * P->n_layers > 65535)
         return fail(PK_ERR_UNSUPPORTED, "n_layers * n_kv_heads above 65535");
@@ -2282,6 +2278,12 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     PK_CUDA(cudaStreamIsCapturing(st, &capturing));
     if (capturing != cudaStreamCaptureStatusNone)
         return fail(PK_ERR_UNSUPPORTED, "pk_pool_evict uploads from host memory and cannot be captured");
+    const int bs = P->block_size;
+    std::lock_guard<std::mutex> lock(P->evict_mutex);  // plan, uploads and scratch are the pool's
+    EvictPlan& plan = P->evict_plan;
+    int rc = plan_evict(P->num_blocks, bs, nseq, table_indptr, table_ids, lengths, new_indptr, new_ids, budget, sinks, recent,
+                        &plan);
+    if (rc != PK_OK || nseq == 0) return rc;
     if (P->evict_done) PK_CUDA(cudaStreamWaitEvent(st, P->evict_done, 0));
     else PK_CUDA(cudaEventCreateWithFlags(&P->evict_done, cudaEventDisableTiming));
     pk::EvictParams p{};

@@ -257,6 +257,31 @@ def test_evict_sequences_refuses(ids, lens, kw):
     assert not pool.calls and len(bm.block_table(1)) == 2
 
 
+def test_evict_sequences_checks_the_pool_before_it_compacts():
+    bm = BlockManager(8, 4, enable_prefix_caching=False)
+    bm.allocate(1, list(range(16)))
+    for wrong in (dict(block_size=8, num_blocks=8), dict(block_size=4, num_blocks=7)):
+        pool = _FakePool()
+        pool.__dict__.update(wrong)
+        with pytest.raises(ValueError, match="pool's"):
+            evict_sequences(pool, bm, [1], [16], 4)
+        assert not pool.calls and len(bm.block_table(1)) == 4
+
+
+def test_evict_sequences_does_not_repeat_a_failed_call():
+    class Broken(_FakePool):
+        def evict(self, tables, lengths, budget, **kw):
+            self.calls.append(lengths)
+            raise RuntimeError("device")
+
+    bm = BlockManager(8, 4, enable_prefix_caching=False)
+    bm.allocate(1, list(range(16)))
+    pool = Broken()
+    with pytest.raises(RuntimeError, match="device"):
+        evict_sequences(pool, bm, [1], [16], 4)
+    assert pool.calls == [[16]]
+
+
 @pytest.mark.parametrize("kw", [dict(window=0), dict(window=-3), dict(sinks=1), dict(window=4, sinks=-1),
                                 dict(weights="sum"), dict(weights="add")])
 def test_paged_batch_refuses_bad_bounds(kw):

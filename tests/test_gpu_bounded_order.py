@@ -112,3 +112,29 @@ def test_a_new_plan_follows_the_calls_before_it(shape):
     got = steps([torch.cuda.Stream() for _ in range(4)])
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("what", ["capture", "head_dim"])
+def test_refused_evictions_leave_the_tables_alone(what):
+    """What pool.evict refuses for good, evict_sequences refuses before the manager's tables change."""
+    torch = torch_cuda()
+    from gpu_util import Shape
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import BlockManager, PagedKVPool, evict_sequences
+
+    pool = PagedKVPool(Shape(1, 1, 32 if what == "capture" else 513), 8, 16, track_weights=True)
+    bm = BlockManager(8, 16, enable_prefix_caching=False)
+    bm.allocate(1, list(range(100)))
+    bm.fork(1, 2)
+    before = bm.block_table(1), bm.block_table(2), bm.alloc.num_free
+    with pytest.raises(_lib.PagedKVError, match="captured" if what == "capture" else "head_dim"):
+        if what == "capture":
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                evict_sequences(pool, bm, [1, 2], [100, 100], 10)
+        else:
+            evict_sequences(pool, bm, [1, 2], [100, 100], 10)
+    torch.cuda.synchronize()
+    assert (bm.block_table(1), bm.block_table(2), bm.alloc.num_free) == before
+    if what == "capture":
+        bm.free(2)
+        assert evict_sequences(pool, bm, [1], [100], 10).tolist() == [10]
