@@ -89,7 +89,8 @@ PK_API int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const fl
 /* Accumulated attention weights (no counterpart in pagellm): float32
  * [layers][num_blocks][n_kv_heads][block_size], zero-filled, one value per layer, token slot
  * and KV head, owned by the pool from the first call on (later calls return the same
- * memory). They belong to the block: sequences that share a block share its weights.
+ * memory). They belong to the block: sequences that share a block share its weights. A token that is
+ * stored by a call which keeps no weights (a plain or windowed step, pk_pool_append) starts at zero.
  * pk_pool_copy_blocks copies a block's weights with it; pk_batch_set_bounds makes steps keep
  * them up and pk_pool_evict goes by them. */
 PK_API int pk_pool_track_weights(pk_pool* pool, float** weights_dev);

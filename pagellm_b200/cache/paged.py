@@ -134,7 +134,8 @@ class PagedKVPool:
     ``track_weights``: the pool also holds ``weights``, float32 ``(layers, num_blocks,
     kv_heads, block_size)``, zero at first: the attention weight that every cached token has
     got, kept up by ``PagedBatch(..., weights=)``, moved by ``copy_blocks`` and ``evict``
-    (sequences that share a block share its weights).
+    (sequences that share a block share its weights). A token that a step without ``weights``
+    stores starts at zero.
     """
 
     def __init__(self, cfg, num_blocks: int, block_size: int, dtype=np.float32, device=None,

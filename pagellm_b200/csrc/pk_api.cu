@@ -1523,6 +1523,18 @@ pk::TcParams tc_params(pk_batch* B, int layer, int H, const float* q, float* out
     return p;
 }
 
+// After a call that stored the step's rows without keeping weights, on a pool that tracks them: the rows'
+// tokens start at zero.
+int clear_new_weights(pk_batch* B, int layer, cudaStream_t st) {
+    pk_pool* P = B->pool;
+    if (P->weights == nullptr || B->weights_mode != 0 || B->nrows == 0) return PK_OK;
+    PK_CUDA(pk::launch_clear_weights(P->weights + static_cast<int64_t>(layer) * P->layer_weights(), nullptr,
+                                     B->meta.at<int32_t>(4), B->meta.at<int32_t>(3), B->meta.at<int32_t>(2),
+                                     B->meta.at<int32_t>(0), B->meta.at<int32_t>(1), P->block_size, P->kvh, B->nrows, st));
+    B->launches++;
+    return PK_OK;
+}
+
 // Host-side fault injection for tests: the next attention call of any batch fails as a
 // launch error would, before it launches anything.
 std::atomic<int> g_inject_launch_failure{0};
@@ -1968,6 +1980,10 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
             B->launches++;
         }
     }
+    if (k_new != nullptr) {
+        int rc = clear_new_weights(B, layer, st);
+        if (rc != PK_OK) return rc;
+    }
     if (!captured) {
         if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
         PK_CUDA(cudaEventRecord(B->ev_bounded, st));
@@ -2339,6 +2355,10 @@ int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const float* v_
     DeviceScope ds(pool->device);
     PK_CUDA(pk::launch_append(pool->dtype, pool->k_layer(layer), pool->v_layer(layer), k_dev, v_dev,
                               slots_dev, nullptr, n, pool->kvh * pool->d, static_cast<cudaStream_t>(stream)));
+    if (pool->weights)
+        PK_CUDA(pk::launch_clear_weights(pool->weights + static_cast<int64_t>(layer) * pool->layer_weights(), slots_dev,
+                                         nullptr, nullptr, nullptr, nullptr, nullptr, pool->block_size, pool->kvh, n,
+                                         static_cast<cudaStream_t>(stream)));
     return PK_OK;
 }
 
@@ -2650,13 +2670,12 @@ int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* 
     // Fused append (rows patched into the attention kernels' shared memory) pays off for
     // decode steps; with several new tokens per sequence one scatter kernel first is faster
     // than each unit fetching its rows on its critical path.
-    if (B->ngeneric == 0 && B->fuse_append_ok && (B->use_tc || B->nwide > 0) && B->tc_max_new <= kFuseMaxNew)
-        return attend_impl(B, layer, n_heads, q_dev, out_dev, st, k_dev, v_dev);
+    const bool fused_tc = B->ngeneric == 0 && B->fuse_append_ok && (B->use_tc || B->nwide > 0) && B->tc_max_new <= kFuseMaxNew;
     // A step wholly on the CUDA-core kernel appends inside it as well: its CTAs read the
     // step's rows from the inputs and one CTA per (row, KV head) stores each to the pool.
-    if (B->ngeneric > 0 && !B->use_tc && B->nwide == 0 && B->fuse_append_ok)
-        return attend_impl(B, layer, n_heads, q_dev, out_dev, st, k_dev, v_dev);
-    if (B->nrows > 0) {
+    const bool fused_generic = B->ngeneric > 0 && !B->use_tc && B->nwide == 0 && B->fuse_append_ok;
+    const bool fused = fused_tc || fused_generic;
+    if (B->nrows > 0 && !fused) {
         const bool listed = !B->app_rows.empty();
         PK_CUDA(prof_begin(B, st));
         PK_CUDA(pk::launch_append_table(P->dtype, P->k_layer(layer), P->v_layer(layer), k_dev, v_dev,
@@ -2668,7 +2687,8 @@ int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* 
         PK_CUDA(prof_end(B, kProfAppend, st));
         B->launches++;
     }
-    return attend_impl(B, layer, n_heads, q_dev, out_dev, st);
+    rc = attend_impl(B, layer, n_heads, q_dev, out_dev, st, fused ? k_dev : nullptr, fused ? v_dev : nullptr);
+    return rc == PK_OK ? clear_new_weights(B, layer, st) : rc;
 } catch (const std::exception& e) {
     return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }

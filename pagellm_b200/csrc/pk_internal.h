@@ -420,6 +420,10 @@ cudaError_t launch_copy_blocks(void* k, void* v, const int64_t* pairs, int64_t n
 // The accumulated weights of copied blocks: pairs as in launch_copy_blocks, `block` floats each.
 cudaError_t launch_copy_weights(float* weights, const int64_t* pairs, int64_t npairs, int layers, int64_t layer_floats,
                                 int block, cudaStream_t st);
+// Zeroes one layer's accumulated weights of n tokens: at `slots`, or (NULL) of the step's rows by the block table.
+cudaError_t launch_clear_weights(float* weights, const int64_t* slots, const int32_t* row_seq, const int32_t* offsets,
+                                 const int32_t* starts, const int32_t* indptr, const int32_t* ids, int bs, int kvh,
+                                 int64_t n, cudaStream_t st);
 cudaError_t launch_bounded_wait_selftest(int* err, unsigned long long limit_ns, cudaStream_t st);
 // Three device-addressable host arrays (float counts multiples of 4, 16-byte aligned) into
 // device buffers, one launch.
