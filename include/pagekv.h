@@ -140,8 +140,11 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
  * All calls of a batch share its scratch. Bounded calls on different streams therefore run in the
  * order of the calls, behind the plan's uploads (what they read and write beyond the batch - rows,
  * the pool - is the caller's to order); graphs that were captured from one batch are the caller's to
- * replay one after another, and not while other calls of the batch run. */
+ * replay one after another, and not while other calls of the batch run. While such a graph exists the
+ * batch is not planned again, by pk_batch_plan or by a call with another n_heads (PK_ERR_UNSUPPORTED),
+ * and must not be destroyed; pk_batch_graphs counts them (a graph's end may show a moment later). */
 PK_API int pk_batch_set_bounds(pk_batch* batch, int64_t window, int64_t sinks, int weights_mode);
+PK_API int pk_batch_graphs(const pk_batch* batch, int64_t* graphs);
 PK_API int pk_batch_destroy(pk_batch* batch);
 /* PagedBatch.__init__ (:397-439). Host arrays: block tables in CSR form
  * (table_indptr[nseq+1] int64, table_ids int32), starts[nseq], n_new[nseq] (int64).

@@ -178,6 +178,7 @@ class PagedKVPool:
             wshape = (self.n_layers, self.num_blocks, self.n_kv_heads, self.block_size)
             self.weights = torch.as_tensor(_CudaArray(wp.value, wshape, "<f4", self._h), device=self.device)
         self._idle_batches: list[int] = []
+        self._held_batches: list[int] = []  # idle, but a CUDA graph captured from them still exists
         self._batch_prefix_mode: dict[int, int] = {}  # handle -> prefix-sharing mode it holds
         self._batch_bounds: dict[int, tuple] = {}  # handle -> (window, sinks, weights mode) it holds
 
@@ -254,28 +255,40 @@ class PagedKVPool:
         return self._h.ptr
 
     def _acquire_batch(self) -> int:
+        if self._held_batches:
+            held = self._held_batches
+            self._held_batches = [h for h in held if self._graphs_of(h)]
+            self._idle_batches += [h for h in held if h not in self._held_batches]
         if self._idle_batches:
             return self._idle_batches.pop()
         h = C.c_void_p()
         _lib.check(_lib.load().pk_batch_create(self._h.ptr, C.byref(h)))
         return h.value
 
-    def _release_batch(self, h: int) -> None:
-        self._idle_batches.append(h)
+    def _release_batch(self, h: int, bounded: bool) -> None:
+        # (only bounded calls count the graphs they are captured into)
+        (self._held_batches if bounded and self._graphs_of(h) else self._idle_batches).append(h)
+
+    @staticmethod
+    def _graphs_of(h: int) -> int:
+        n = C.c_int64()
+        _lib.check(_lib.load().pk_batch_graphs(h, C.byref(n)))
+        return n.value
+
+    def _destroy_batches(self) -> None:
+        lib = _lib.load()
+        for handles in (self._idle_batches, self._held_batches):
+            for h in handles:
+                lib.pk_batch_destroy(h)
+            handles.clear()
 
     def close(self) -> None:
-        lib = _lib.load()
-        for h in self._idle_batches:
-            lib.pk_batch_destroy(h)
-        self._idle_batches.clear()
+        self._destroy_batches()
         self._h.close()
 
     def __del__(self):
         try:
-            lib = _lib.load()
-            for h in self._idle_batches:
-                lib.pk_batch_destroy(h)
-            self._idle_batches.clear()
+            self._destroy_batches()
         except Exception:
             pass
 
@@ -366,7 +379,9 @@ class PagedBatch:
     adds it to the pool's ``weights`` (``"add"``) or stores it there (``"replace"``). The
     step's own tokens start anew; tokens that no row sees keep their weight. Such a step reads
     every block through one table entry only (``ValueError`` otherwise). In bounded steps of a
-    bf16 pool, bf16 CUDA tensors are read and written as they are.
+    bf16 pool, bf16 CUDA tensors are read and written as they are. Calls on different streams run
+    one after another (they share the batch's scratch); a CUDA graph of them keeps the batch's
+    tables and scratch for as long as it exists, and goes with the pool at the latest.
     """
 
     _WEIGHT_MODES = {None: 0, "add": 1, "replace": 2}
@@ -420,7 +435,7 @@ class PagedBatch:
         b = getattr(self, "_b", None)
         if b is not None:
             try:
-                self.pool._release_batch(b)
+                self.pool._release_batch(b, self._bounded)
             except Exception:
                 pass
             self._b = None

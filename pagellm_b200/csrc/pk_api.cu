@@ -11,6 +11,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <memory>
 #include <mutex>
 #include <queue>
 #include <array>
@@ -387,6 +388,10 @@ struct pk_batch {
     cudaEvent_t ev_bounded = nullptr;
     cudaStream_t last_stream = nullptr;
     bool used = false;
+    // CUDA graphs that bounded calls of this batch were captured into and that still exist (keep_for_graph),
+    // and the last such capture
+    std::shared_ptr<std::atomic<int64_t>> graphs = std::make_shared<std::atomic<int64_t>>(0);
+    unsigned long long capture_id = 0;
     bool bounded() const { return window > 0 || weights_mode != 0; }
     int launches = 0;
     // bytes the last pk_batch_write_and_attend_host moved: host to device, device to host
@@ -1112,9 +1117,47 @@ cudaError_t wait_last(pk_batch* B, cudaStream_t st) {
     return B->used && st != B->last_stream ? cudaStreamWaitEvent(st, B->ev_bounded, 0) : cudaSuccess;
 }
 
+// A captured call's kernels hold the addresses and sizes of the batch's tables, plan and scratch: while the
+// graph (or one instantiated from it) exists, it counts in B->graphs, and the batch is not planned again.
+int keep_for_graph(pk_batch* B, cudaStream_t st) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    PK_CUDA(cudaStreamGetCaptureInfo(st, &status, &id, &graph));
+    if (status != cudaStreamCaptureStatusActive || id == B->capture_id) return PK_OK;  // once per capture
+    using Count = std::shared_ptr<std::atomic<int64_t>>;
+    auto gone = [](void* p) {  // when the last of the graph's owners is destroyed; makes no CUDA call
+        Count* count = static_cast<Count*>(p);
+        --**count;
+        delete count;
+    };
+    Count* count = new Count(B->graphs);
+    ++**count;
+    cudaUserObject_t object = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&object, count, gone, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) {
+        gone(count);
+        return fail(PK_ERR_CUDA, "cudaUserObjectCreate: %s", cudaGetErrorString(e));
+    }
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) {
+        cudaUserObjectRelease(object, 1);
+        return fail(PK_ERR_CUDA, "cudaGraphRetainUserObject: %s", cudaGetErrorString(e));
+    }
+    B->capture_id = id;
+    return PK_OK;
+}
+
+int check_no_graphs(const pk_batch* B) {
+    if (B->graphs->load() > 0)
+        return fail(PK_ERR_UNSUPPORTED, "a CUDA graph captured from this batch still exists and reads its plan: use another batch");
+    return PK_OK;
+}
+
 int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     pk_pool* P = B->pool;
     const int g = H / P->kvh;
+    if (int rc = check_no_graphs(B)) return rc;
     B->plan_H = -1;
     if (B->bounded() || B->used) {
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
@@ -1716,7 +1759,9 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     PK_CUDA(cudaStreamIsCapturing(st, &capturing));
     const bool captured = capturing != cudaStreamCaptureStatusNone;
-    if (!captured) {
+    if (captured) {
+        if (int rc = keep_for_graph(B, st)) return rc;
+    } else {
         // The last call, and uploads of the tables and the plan, on other streams. A capture cannot wait
         // for them: it follows a call that did (build_attention_plan).
         PK_CUDA(wait_last(B, st));
@@ -2409,6 +2454,7 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
     if (nseq < 0) return fail(PK_ERR_INVALID_ARG, "nseq < 0");
     if (nseq > 0 && (!table_indptr || !starts || !n_new))
         return fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    if (int rc = check_no_graphs(B)) return rc;
     pk_pool* P = B->pool;
     const int bs = P->block_size;
     B->plan_H = -1;
@@ -2837,6 +2883,12 @@ int pk_batch_stats(const pk_batch* B, int64_t* s) {
 
 int pk_test_inject_launch_failure(void) {
     g_inject_launch_failure.store(1);
+    return PK_OK;
+}
+
+int pk_batch_graphs(const pk_batch* B, int64_t* graphs) {
+    if (!B || !graphs) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    *graphs = B->graphs->load();
     return PK_OK;
 }
 

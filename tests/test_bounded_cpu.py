@@ -115,6 +115,11 @@ def test_null_arguments():
     assert lib.pk_bm_compact(None, 0, 0, None, 0, None) == _lib.PK_ERR_INVALID_ARG
 
 
+def test_graph_count_needs_a_batch():
+    n = C.c_int64(7)
+    assert _lib.load().pk_batch_graphs(None, C.byref(n)) == _lib.PK_ERR_INVALID_ARG and n.value == 7
+
+
 # ------------------------------------------------------------------ block manager
 def test_compact_keeps_own_blocks_and_releases_the_rest():
     bm = BlockManager(16, 4, enable_prefix_caching=False)

@@ -138,3 +138,71 @@ def test_refused_evictions_leave_the_tables_alone(what):
     if what == "capture":
         bm.free(2)
         assert evict_sequences(pool, bm, [1], [100], 10).tolist() == [10]
+
+
+def _until(condition):
+    """A destroyed graph's end is counted by a thread of the driver's."""
+    import time
+
+    for _ in range(200):
+        if condition():
+            return True
+        time.sleep(0.01)
+    return False
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=_shape)
+def test_a_live_graph_keeps_the_plan_it_reads(shape):
+    """A graph holds addresses of its batch's tables, plan and scratch: they stay until it is gone, whether
+    the batch lives on, is asked for other heads, or is dropped and others are made."""
+    torch = torch_cuda()
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case(*shape, [4000, 40, 300], [1, 60, 5], window=500, sinks=4, weights="replace")
+    b = c.batch()
+    want = c.run(b).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b.write_and_attend(0, c.q, c.k, c.v)
+        got = b.write_and_attend(0, c.q, c.k, c.v)
+    handle = b._b
+    assert c.pool._graphs_of(handle) == 1
+    q2 = torch.cat([c.q, c.q], 1)
+    with pytest.raises(_lib.PagedKVError, match="graph"):
+        b.attend(0, q2)
+    assert torch.equal(c.run(b), want)  # the plan is as it was
+    del b
+    others = []
+    for _ in range(3):  # none of them gets the graph's handle
+        others.append(PagedBatch(c.pool, [c.tables[0]], [1000], [3], window=50))
+        others[-1].attend(0, q2[:3])
+    assert handle not in [o._b for o in others] and handle in c.pool._held_batches
+    for _ in range(2):
+        got.zero_()
+        c.pool.weights.copy_(c.before)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        c.check(got)
+    del graph
+    assert _until(lambda: c.pool._graphs_of(handle) == 0)
+    again = c.batch()
+    assert not c.pool._held_batches
+    c.check(again.write_and_attend(0, c.q, c.k, c.v))
+
+
+def test_a_failed_capture_keeps_nothing():
+    torch = torch_cuda()
+    c = Case("bf16", 8, 2, 128, 16, [100], [1], window=40)
+    b = c.batch()
+    c.run(b)
+    with pytest.raises(RuntimeError, match="on purpose"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            b.write_and_attend(0, c.q, c.k, c.v)
+            raise RuntimeError("on purpose")
+    torch.cuda.synchronize()
+    assert _until(lambda: c.pool._graphs_of(b._b) == 0)
+    q2 = torch.cat([c.q, c.q], 1)
+    b.attend(0, q2)
+    c.check(c.run(b))
