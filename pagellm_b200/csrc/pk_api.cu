@@ -2171,7 +2171,7 @@ const char* pk_last_error(void) { return g_err.c_str(); }
 int pk_abi_version(void) { return 1; }
 
 int pk_pool_create(int n_layers, int64_t num_blocks, int block_size, int n_kv_heads, int head_dim,
-                   int dtype, int device, pk_pool** out) {
+                   int dtype, int device, pk_pool** out) try {
     if (!out) return fail(PK_ERR_INVALID_ARG, "out is NULL");
     *out = nullptr;
     if (n_layers <= 0 || num_blocks <= 0 || block_size <= 0 || n_kv_heads <= 0 || head_dim <= 0)
@@ -2205,6 +2205,8 @@ int pk_pool_create(int n_layers, int64_t num_blocks, int block_size, int n_kv_he
     setup_tc(P);
     *out = P;
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_pool_destroy(pk_pool* pool) {
@@ -2254,7 +2256,7 @@ int pk_pool_copy_blocks_dev(pk_pool* pool, const int64_t* pairs_dev, int64_t npa
     return PK_OK;
 }
 
-int pk_pool_copy_blocks(pk_pool* pool, const int64_t* pairs_host, int64_t npairs, void* stream) {
+int pk_pool_copy_blocks(pk_pool* pool, const int64_t* pairs_host, int64_t npairs, void* stream) try {
     if (!pool) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
     if (npairs < 0) return fail(PK_ERR_INVALID_ARG, "npairs < 0");
     if (npairs == 0) return PK_OK;
@@ -2302,6 +2304,8 @@ int pk_pool_copy_blocks(pk_pool* pool, const int64_t* pairs_host, int64_t npairs
                                             pool->kvh * pool->block_size, st));
     }
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_pool_track_weights(pk_pool* pool, float** weights_dev) {
@@ -2418,7 +2422,7 @@ int pk_slot_mapping(const int32_t* table_dev, int64_t table_len, const int64_t* 
     return PK_OK;
 }
 
-int pk_batch_create(pk_pool* pool, pk_batch** out) {
+int pk_batch_create(pk_pool* pool, pk_batch** out) try {
     if (!pool || !out) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
     DeviceScope ds(pool->device);
     auto* B = new pk_batch();
@@ -2431,6 +2435,8 @@ int pk_batch_create(pk_pool* pool, pk_batch** out) {
     }
     *out = B;
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_batch_destroy(pk_batch* B) {
@@ -2741,7 +2747,7 @@ int pk_batch_write_and_attend(pk_batch* B, int layer, int n_heads, const float* 
 
 int pk_peer_gather_write_and_attend(pk_peer_gather* g, pk_batch* B, int layer, int n_heads,
                                     const float* q_dev, const float* k_dev, const float* v_dev,
-                                    float** result_dev, void* stream) {
+                                    float** result_dev, void* stream) try {
     if (!g || !B || !result_dev) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
     int rc = check_heads(B, n_heads);
     if (rc != PK_OK) return rc;
@@ -2781,11 +2787,13 @@ int pk_peer_gather_write_and_attend(pk_peer_gather* g, pk_batch* B, int layer, i
         slice = static_cast<const float*>(B->peer_slice.ptr);
     }
     return pk_peer_gather_heads(g, slice, B->nrows, row_floats, result_dev, stream);
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_batch_write_and_attend_host(pk_batch* B, int layer, int n_heads, const float* q_host,
                                    const float* k_host, const float* v_host, float* out_host,
-                                   void* stream) {
+                                   void* stream) try {
     if (!B) return fail(PK_ERR_INVALID_ARG, "batch is NULL");
     int rc = check_heads(B, n_heads);
     if (rc != PK_OK) return rc;
@@ -2842,6 +2850,8 @@ int pk_batch_write_and_attend_host(pk_batch* B, int layer, int n_heads, const fl
     }
     PK_CUDA(cudaStreamSynchronize(st));
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_batch_io_stats(const pk_batch* B, int64_t* s) {
@@ -2919,7 +2929,7 @@ int pk_batch_profile(pk_batch* B, int enable) {
     return PK_OK;
 }
 
-int pk_batch_profile_read(pk_batch* B, double* ms5, int64_t* count5) {
+int pk_batch_profile_read(pk_batch* B, double* ms5, int64_t* count5) try {
     double* ms4 = ms5;
     int64_t* count4 = count5;
     if (!B || !ms4 || !count4) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
@@ -2938,6 +2948,8 @@ int pk_batch_profile_read(pk_batch* B, double* ms5, int64_t* count5) {
     B->ev_used = 0;
     B->ev_kind.clear();
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 int pk_selftest_bounded_wait(int device, int64_t limit_ns, int* timed_out) {
@@ -2996,7 +3008,7 @@ int pk_plan_visible_blocks(int64_t first_position, int64_t context, int64_t wind
 }
 
 int pk_plan_partition(const int64_t* unit_blocks, int64_t n_units, int max_ctas, int unit_switch_blocks,
-                      int64_t* cta_first_block, int* ncta) {
+                      int64_t* cta_first_block, int* ncta) try {
     if (n_units < 0 || max_ctas <= 0 || unit_switch_blocks < 0 || !ncta || (n_units > 0 && !unit_blocks))
         return fail(PK_ERR_INVALID_ARG, "bad arguments");
     std::vector<int64_t> ub(static_cast<size_t>(n_units) + 1, 0);
@@ -3011,6 +3023,8 @@ int pk_plan_partition(const int64_t* unit_blocks, int64_t n_units, int max_ctas,
     if (cta_first_block)
         for (int c = 0; c <= *ncta; ++c) cta_first_block[c] = first[c];
     return PK_OK;
+} catch (const std::exception& e) {
+    return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
 }  // extern "C"

@@ -305,6 +305,28 @@ def test_evict_keep_orders_ties_and_nan():
     assert bo.evict_keep([1.0, 0.0, -0.0, 0.0], 2, 0, 0).tolist() == [0, 1]
 
 
+# ------------------------------------------------------------------ C entries
+def test_allocations_that_fail_are_errors():
+    """No exception leaves a C entry (which would end the process): a child asks for impossible sizes."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = '''
+import ctypes as C
+from pagellm_b200 import _lib
+lib = _lib.load()
+one, n, big = (C.c_int64 * 2)(0, 0), C.c_int(), C.c_int64()
+codes = [lib.pk_plan_partition(one, 1 << 61, 148, 1, None, C.byref(n)),
+         lib.pk_plan_evict(1 << 60, 16, 1, one, None, one, one, None, 4, 0, 0, C.byref(big))]
+print(codes, _lib.last_error())
+'''
+    root = Path(__file__).resolve().parents[1]
+    got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert got.returncode == 0, got.stderr
+    assert got.stdout.startswith(str([_lib.PK_ERR_CUDA] * 2)) and "host allocation" in got.stdout
+
+
 # ------------------------------------------------------------------ the sources
 def test_shared_memory_of_wide_words_is_declared_aligned():
     """Dynamic shared memory lies behind a kernel's static arrays: where it is read and written in 16-byte
