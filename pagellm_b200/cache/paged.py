@@ -344,18 +344,21 @@ def _csr(block_tables):
     if isinstance(block_tables, tuple) and len(block_tables) == 2 and isinstance(block_tables[0], np.ndarray) \
             and block_tables[0].ndim == 1 and len(block_tables[0]) and block_tables[0][0] == 0 \
             and block_tables[1].dtype == np.int32:
-        return np.ascontiguousarray(block_tables[0], np.int64), np.ascontiguousarray(block_tables[1])
+        indptr, ids = np.ascontiguousarray(block_tables[0], np.int64), np.ascontiguousarray(block_tables[1])
+        if int(indptr[-1]) > ids.size:
+            raise ValueError(f"CSR block tables: indptr ends at {int(indptr[-1])}, ids has {ids.size} entries")
+        return indptr, ids
     lens = np.fromiter(map(len, block_tables), dtype=np.int64, count=len(block_tables))
     indptr = np.zeros(len(lens) + 1, dtype=np.int64)
     np.cumsum(lens, out=indptr[1:])
     total = int(indptr[-1])
     if total and all(isinstance(t, np.ndarray) for t in block_tables):
-        ids = np.concatenate(block_tables).astype(np.int32, copy=False)
+        flat = np.concatenate(block_tables)
     else:
         flat = np.fromiter(itertools.chain.from_iterable(block_tables), dtype=np.int64, count=total)
-        if total and (flat.min() < -(2 ** 31) or flat.max() >= 2 ** 31):
-            raise IndexError("block id outside the int32 range")
-        ids = flat.astype(np.int32)
+    if total and flat.dtype != np.int32 and (flat.min() < -(2 ** 31) or flat.max() >= 2 ** 31):
+        raise IndexError("block id outside the int32 range")
+    ids = flat.astype(np.int32, copy=False)
     return indptr, np.ascontiguousarray(ids)
 
 

@@ -305,6 +305,23 @@ def test_evict_keep_orders_ties_and_nan():
     assert bo.evict_keep([1.0, 0.0, -0.0, 0.0], 2, 0, 0).tolist() == [0, 1]
 
 
+def test_block_ids_do_not_wrap_and_tables_do_not_run_out():
+    from pagellm_b200.cache.paged import _csr
+
+    for ids in ([2 ** 32], [-2 ** 31 - 1], [3, 2 ** 31]):
+        for tables in ([ids], [np.array(ids, np.int64)], [np.array([1], np.int32), np.array(ids, np.int64)]):
+            with pytest.raises(IndexError):
+                _csr(tables)
+    with pytest.raises(IndexError):
+        _csr([np.array([2 ** 31], np.uint32)])
+    with pytest.raises(ValueError):
+        _csr((np.array([0, 2, 4], np.int64), np.array([0, 1, 2], np.int32)))
+    for tables in ([[5, 0], [7]], [np.array([5, 0]), np.array([7])], [np.array([5, 0], np.int32), np.array([7], np.uint8)],
+                   (np.array([0, 2, 3], np.int64), np.array([5, 0, 7], np.int32))):
+        indptr, ids = _csr(tables)
+        assert indptr.tolist() == [0, 2, 3] and ids.tolist() == [5, 0, 7] and ids.dtype == np.int32
+
+
 # ------------------------------------------------------------------ C entries
 def test_allocations_that_fail_are_errors():
     """No exception leaves a C entry (which would end the process): a child asks for impossible sizes."""
