@@ -2577,14 +2577,14 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
                                      ? visible_blocks(B->starts[i], static_cast<int64_t>(B->starts[i]) + B->nnew[i], B->window,
                                                       B->sinks, bs)
                                      : VisibleBlocks{0, 0, n};
-        for (int32_t x = 0; x < vb.count; ++x) {
-            const int32_t j = x < vb.head ? x : x + vb.skip;
-            const int32_t b = t[j];
-            if (((wbits[b >> 6] >> (b & 63)) & 1) && (B->writer_seq[b] != i || B->writer_idx[b] != j)) {
-                B->fuse_append_ok = false;
-                break;
+        auto own = [&](int64_t j, int64_t end) {  // entries [j, end) name no block that another entry writes
+            for (; j < end; ++j) {
+                const int32_t b = t[j];
+                if (((wbits[b >> 6] >> (b & 63)) & 1) && (B->writer_seq[b] != i || B->writer_idx[b] != j)) return false;
             }
-        }
+            return true;
+        };
+        B->fuse_append_ok = own(0, vb.head) && own(vb.head + vb.skip, vb.count + vb.skip);
     }
     for (int32_t b : touched) {
         B->writer_seq[b] = B->writer_idx[b] = -1;
