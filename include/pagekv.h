@@ -112,6 +112,10 @@ PK_API int pk_pool_evict(pk_pool* pool, int nseq, const int64_t* table_indptr, c
                   const int64_t* lengths, const int64_t* new_indptr, const int32_t* new_ids, int64_t budget,
                   int64_t sinks, int64_t recent, int32_t* kept_dev, void* stream);
 
+/* Gives back the device memory that evictions without kept_dev keep between calls (*freed: its bytes,
+ * may be NULL). Waits for the device. */
+PK_API int pk_pool_trim(pk_pool* pool, int64_t* freed);
+
 /* slot_mapping (cache/paged.py:303-306): slots[i] = table[p / bs] * bs + p % bs for
  * p = positions[i]. Device arrays. A position outside [0, table_len * bs) yields slot
  * -1 and, if err_dev is not NULL, sets *err_dev to 1. */
@@ -146,6 +150,9 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
 PK_API int pk_batch_set_bounds(pk_batch* batch, int64_t window, int64_t sinks, int weights_mode);
 PK_API int pk_batch_graphs(const pk_batch* batch, int64_t* graphs);
 PK_API int pk_batch_destroy(pk_batch* batch);
+/* Device memory that the batch holds (no counterpart in pagellm): tables, plan and scratch, which only
+ * grow. The largest part can be the scores of steps with weights, up to 1.25 GB once a step needed them. */
+PK_API int pk_batch_scratch(const pk_batch* batch, int64_t* bytes);
 /* PagedBatch.__init__ (:397-439). Host arrays: block tables in CSR form
  * (table_indptr[nseq+1] int64, table_ids int32), starts[nseq], n_new[nseq] (int64).
  * Sequence i owns rows offsets[i] .. offsets[i]+n_new[i]-1 at positions starts[i]...

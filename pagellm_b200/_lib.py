@@ -56,6 +56,8 @@ SIGNATURES: dict[str, tuple] = {
     "pk_batch_write_and_attend_bf16": (_i32, [_p, _i32, _i32, _p, _p, _p, _p, _p]),
     "pk_batch_set_bounds": (_i32, [_p, _i64, _i64, _i32]),
     "pk_batch_graphs": (_i32, [_p, _pi64]),
+    "pk_batch_scratch": (_i32, [_p, _pi64]),
+    "pk_pool_trim": (_i32, [_p, _pi64]),
     "pk_batch_check": (_i32, [_p, _p]),
     "pk_batch_stats": (_i32, [_p, _pi64]),
     "pk_batch_io_stats": (_i32, [_p, _pi64]),

@@ -242,6 +242,23 @@ class PagedKVPool:
         return self._nbytes
 
     # ------------------------------------------------------------------ extras
+    def trim(self) -> int:
+        """Give back the device memory that earlier steps and evictions left behind for later ones:
+        idle batches' tables and scratch (most of it scores of steps with weights, up to 1.25 GB a
+        batch) and the scratch of evictions. Batches in use, or captured into a live CUDA graph,
+        keep theirs. Waits for the device; returns the bytes."""
+        lib = _lib.load()
+        n, total = C.c_int64(), 0
+        for h in self._idle_batches:
+            _lib.check(lib.pk_batch_scratch(h, C.byref(n)))
+            total += n.value
+            self._batch_prefix_mode.pop(h, None)  # (a later handle may have this address)
+            self._batch_bounds.pop(h, None)
+            _lib.check(lib.pk_batch_destroy(h))
+        self._idle_batches.clear()
+        _lib.check(lib.pk_pool_trim(self._h.ptr, C.byref(n)))
+        return total + n.value
+
     @property
     def tensor_core_path(self) -> tuple[bool, str]:
         """(enabled, reason) for the tensor-core attention kernel on this pool."""
@@ -484,6 +501,14 @@ class PagedBatch:
         keys = ("rows", "tc_units", "tc_ctas", "tc_blocks", "split_units", "generic_rows", "launches",
                 "wide_items")
         return dict(zip(keys, list(s)))
+
+    @property
+    def scratch_nbytes(self) -> int:
+        """Device memory that this batch's handle holds: tables, plan and scratch, which later batches
+        reuse and ``PagedKVPool.trim`` gives back."""
+        n = C.c_int64()
+        _lib.check(self._lib.pk_batch_scratch(self._b, C.byref(n)))
+        return n.value
 
     def io_stats(self) -> dict:
         """Bytes the last host-buffer ``write_and_attend`` moved: ``h2d``, ``d2h`` (a copy

@@ -2394,6 +2394,15 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     return fail(PK_ERR_CUDA, "host allocation failed: %s", e.what());
 }
 
+int pk_pool_trim(pk_pool* pool, int64_t* freed) {
+    if (!pool) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
+    DeviceScope ds(pool->device);
+    std::lock_guard<std::mutex> lock(pool->evict_mutex);
+    if (freed) *freed = static_cast<int64_t>(pool->evict_kept.cap);
+    pool->evict_kept.release();  // (cudaFree waits for the kernels that use it)
+    return PK_OK;
+}
+
 int pk_pool_append(pk_pool* pool, int layer, const float* k_dev, const float* v_dev,
                    const int64_t* slots_dev, int64_t n, void* stream) {
     if (!pool) return fail(PK_ERR_INVALID_ARG, "pool is NULL");
@@ -2893,6 +2902,17 @@ int pk_batch_stats(const pk_batch* B, int64_t* s) {
 
 int pk_test_inject_launch_failure(void) {
     g_inject_launch_failure.store(1);
+    return PK_OK;
+}
+
+int pk_batch_scratch(const pk_batch* B, int64_t* bytes) {
+    if (!B || !bytes) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
+    size_t sum = 0;
+    for (const DevBuf* b : {&B->meta.dev, &B->plan.dev, &B->rows, &B->err, &B->wpart, &B->qpk, &B->lse, &B->ws, &B->io,
+                            &B->peer_slice, &B->wpieces, &B->row_lse, &B->cc_part, &B->tile_part, &B->wtile_part,
+                            &B->score, &B->ml})
+        sum += b->cap;
+    *bytes = static_cast<int64_t>(sum);
     return PK_OK;
 }
 

@@ -115,6 +115,12 @@ def test_null_arguments():
     assert lib.pk_bm_compact(None, 0, 0, None, 0, None) == _lib.PK_ERR_INVALID_ARG
 
 
+def test_scratch_calls_need_their_objects():
+    n = C.c_int64(7)
+    assert _lib.load().pk_batch_scratch(None, C.byref(n)) == _lib.PK_ERR_INVALID_ARG
+    assert _lib.load().pk_pool_trim(None, C.byref(n)) == _lib.PK_ERR_INVALID_ARG and n.value == 7
+
+
 def test_graph_count_needs_a_batch():
     n = C.c_int64(7)
     assert _lib.load().pk_batch_graphs(None, C.byref(n)) == _lib.PK_ERR_INVALID_ARG and n.value == 7

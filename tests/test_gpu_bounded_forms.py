@@ -342,3 +342,36 @@ def test_batches_give_their_memory_back():
     torch.cuda.synchronize()
     # the device allocates 2 MB at a time; one split-key scratch alone is more than 8
     assert free - torch.cuda.mem_get_info()[0] <= 4 << 20
+
+
+def test_trim_gives_back_what_idle_batches_and_evictions_hold():
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case("bf16", 40, 8, 64, 16, [3000, 40], [300, 1], weights="replace", poison=False)
+    out = c.run()  # 300 rows x 5 heads in units: scores of some 240 MB
+    live = PagedBatch(c.pool, c.tables, c.starts, c.new, weights="replace")
+    live.write_and_attend(0, c.q, c.k, c.v)
+    other = PagedBatch(c.pool, c.tables, c.starts, c.new, window=70, sinks=1)
+    other.write_and_attend(0, c.q, c.k, c.v)
+    held = live.scratch_nbytes
+    assert held > 150 << 20
+    c.pool.evict(c.tables, c.starts + c.new, 900)
+    del other
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    first = c.pool.trim()
+    assert first > 0 and live.scratch_nbytes == held
+    del live
+    assert c.pool.trim() == held and c.pool.trim() == 0
+    assert torch.cuda.mem_get_info()[0] - free >= held - (8 << 20)
+    again = Case("bf16", 40, 8, 64, 16, [3000, 40], [300, 1], weights="replace", poison=False)
+    again.pool.trim()
+    assert torch.equal(again.run(), out)
+    # plain, windowed and evicting calls go on after it
+    b = PagedBatch(c.pool, [c.tables[1]], [10], [1], window=4)
+    b.write_and_attend(0, c.q[:1], c.k[:1], c.v[:1])
+    b.check()
+    c.pool.evict([c.tables[1]], [11], 5)
+    del b
+    assert c.pool.trim() > 0
