@@ -380,13 +380,13 @@ struct pk_batch {
     DevBuf score;                       // raw scores of a split-KV launch with weights
     bool use_scores = false;
     DevBuf ml;  // [rows][H] softmax statistics of a step with weights
-    // streams of the last uploads: the tables (pk_batch_plan) and the attention plan, which the first
-    // call makes on its own stream
-    cudaStream_t meta_stream = nullptr, plan_stream = nullptr;
+    // Streams of the last uploads: the tables (pk_batch_plan) and the attention plan, which the first
+    // call makes on its own stream. By id: a handle may be that of a stream destroyed since.
+    unsigned long long meta_stream = 0, plan_stream = 0;
     // End of the last bounded call, and its stream. Later calls and plans on another stream wait for it
     // (wait_last), so that one event stands for all calls before it.
     cudaEvent_t ev_bounded = nullptr;
-    cudaStream_t last_stream = nullptr;
+    unsigned long long last_stream = 0;
     bool used = false;
     // CUDA graphs that bounded calls of this batch were captured into and that still exist (keep_for_graph),
     // and the last such capture
@@ -1113,8 +1113,8 @@ int tc_parts(const pk_batch* B) {
 // Before uploads and kernels on `st`, which is not being captured: those of the last bounded call, where it
 // came on another stream, still read the tables and the plan and use the scratch (scores, statistics,
 // partials and their counters).
-cudaError_t wait_last(pk_batch* B, cudaStream_t st) {
-    return B->used && st != B->last_stream ? cudaStreamWaitEvent(st, B->ev_bounded, 0) : cudaSuccess;
+cudaError_t wait_last(pk_batch* B, cudaStream_t st, unsigned long long id) {
+    return B->used && id != B->last_stream ? cudaStreamWaitEvent(st, B->ev_bounded, 0) : cudaSuccess;
 }
 
 // A captured call's kernels hold the addresses and sizes of the batch's tables, plan and scratch: while the
@@ -1159,12 +1159,14 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     const int g = H / P->kvh;
     if (int rc = check_no_graphs(B)) return rc;
     B->plan_H = -1;
+    unsigned long long stream = 0;
     if (B->bounded() || B->used) {
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
         PK_CUDA(cudaStreamIsCapturing(st, &capturing));
-        if (capturing == cudaStreamCaptureStatusNone)
-            PK_CUDA(wait_last(B, st));
-        else if (B->bounded())
+        if (capturing == cudaStreamCaptureStatusNone) {
+            PK_CUDA(cudaStreamGetId(st, &stream));  // (fails on a capturing stream)
+            PK_CUDA(wait_last(B, st, stream));
+        } else if (B->bounded())
             return fail(PK_ERR_UNSUPPORTED, "plan the step before a stream capture (call once with the same n_heads)");
     }
     B->u_seq.clear(); B->u_t0.clear(); B->u_n.clear(); B->u_blk.assign(1, 0);
@@ -1448,7 +1450,7 @@ int build_attention_plan(pk_batch* B, int H, cudaStream_t st) {
     if (B->nprefix > 0) PK_CUDA(B->lse.reserve(static_cast<size_t>(B->nrows) * H * sizeof(float)));
     rc = B->plan.commit(st);
     if (rc != PK_OK) return rc;
-    B->plan_stream = st;
+    B->plan_stream = stream;
     B->plan_H = H;
     return PK_OK;
 }
@@ -1759,14 +1761,16 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     PK_CUDA(cudaStreamIsCapturing(st, &capturing));
     const bool captured = capturing != cudaStreamCaptureStatusNone;
+    unsigned long long stream = 0;
     if (captured) {
         if (int rc = keep_for_graph(B, st)) return rc;
     } else {
         // The last call, and uploads of the tables and the plan, on other streams. A capture cannot wait
         // for them: it follows a call that did (build_attention_plan).
-        PK_CUDA(wait_last(B, st));
-        if (st != B->meta_stream) PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
-        if (st != B->plan_stream) PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
+        PK_CUDA(cudaStreamGetId(st, &stream));
+        PK_CUDA(wait_last(B, st, stream));
+        if (stream != B->meta_stream) PK_CUDA(cudaStreamWaitEvent(st, B->meta.done, 0));
+        if (stream != B->plan_stream) PK_CUDA(cudaStreamWaitEvent(st, B->plan.done, 0));
     }
     // decode steps append inside the split-KV kernel and chunk rows with the packing of their
     // queries, as in plain steps
@@ -2032,7 +2036,7 @@ int attend_bounded(pk_batch* B, int layer, int H, const void* q, const void* k_n
     if (!captured) {
         if (!B->ev_bounded) PK_CUDA(cudaEventCreateWithFlags(&B->ev_bounded, cudaEventDisableTiming));
         PK_CUDA(cudaEventRecord(B->ev_bounded, st));
-        B->last_stream = st;
+        B->last_stream = stream;
         B->used = true;
     }
     return PK_OK;
@@ -2616,13 +2620,19 @@ int pk_batch_plan(pk_batch* B, int nseq, const int64_t* table_indptr, const int3
                 if (last[slot] == r) B->app_rows.push_back(r);
             }
     }
+    DeviceScope ds(P->device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (B->bounded() || B->used) {
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+        if (capturing != cudaStreamCaptureStatusNone)
+            return fail(PK_ERR_UNSUPPORTED, "a step's tables are uploaded before a stream capture");
+        PK_CUDA(cudaStreamGetId(st, &B->meta_stream));
+        PK_CUDA(wait_last(B, st, B->meta_stream));
+    }
     B->nseq = nseq;
     B->nrows = rows;
     if (n_rows) *n_rows = rows;
-    DeviceScope ds(P->device);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    PK_CUDA(wait_last(B, st));
-    B->meta_stream = st;
     B->meta.begin();
     B->meta.add(B->indptr.data(), B->indptr.size() * 4);
     B->meta.add(B->ids.data(), B->ids.size() * 4);

@@ -206,3 +206,54 @@ def test_a_failed_capture_keeps_nothing():
     q2 = torch.cat([c.q, c.q], 1)
     b.attend(0, q2)
     c.check(c.run(b))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=_shape)
+def test_a_new_stream_under_a_destroyed_ones_handle(shape):
+    """A destroyed stream's work goes on; the next stream may get its handle, not its place in the order."""
+    torch = torch_cuda()
+    import ctypes
+
+    c = Case(*shape, [9000, 40], [1, 60], window=5000, sinks=4, weights="replace")
+    b = c.batch()
+    qs = [c.q, torch.randn_like(c.q)]
+    want = [b.write_and_attend(0, q, c.k, c.v) for q in qs]
+    torch.cuda.synchronize()
+    rt = torch.cuda.cudart()
+
+    def create():
+        h = ctypes.c_void_p()
+        assert int(rt.cudaStreamCreate(ctypes.addressof(h))) == 0
+        return h.value
+
+    for _ in range(4):
+        first = create()
+        with torch.cuda.stream(torch.cuda.ExternalStream(first)):
+            torch.cuda._sleep(BUSY)
+            got = [b.write_and_attend(0, qs[0], c.k, c.v)]
+        assert int(rt.cudaStreamDestroy(first)) == 0
+        second = create()
+        with torch.cuda.stream(torch.cuda.ExternalStream(second)):
+            got.append(b.write_and_attend(0, qs[1], c.k, c.v))
+        torch.cuda.synchronize()
+        assert int(rt.cudaStreamDestroy(second)) == 0
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        if second == first:
+            break
+    b.check()
+
+
+def test_a_batch_is_made_before_a_capture():
+    """The refusal leaves the handle fit: its events belong to no capture."""
+    torch = torch_cuda()
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case("bf16", 8, 2, 128, 16, [100], [1], window=40)
+    c.run()
+    for kw in (dict(window=40), {}):  # the second: a plain step on a handle that ran a bounded one
+        with pytest.raises(_lib.PagedKVError, match="capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                PagedBatch(c.pool, c.tables, c.starts, c.new, **kw)
+        torch.cuda.synchronize()
+        c.check(c.run())
