@@ -281,6 +281,7 @@ struct pk_pool {
 
 struct pk_batch {
     pk_pool* pool = nullptr;
+    int device = 0;  // the pool's, which may be gone when the batch is destroyed
     int nseq = 0;
     int64_t nrows = 0;
     std::vector<int32_t> indptr, ids, starts, nnew, offsets, row_seq;
@@ -2440,6 +2441,7 @@ int pk_batch_create(pk_pool* pool, pk_batch** out) try {
     DeviceScope ds(pool->device);
     auto* B = new pk_batch();
     B->pool = pool;
+    B->device = pool->device;
     cudaError_t e = B->err.reserve(sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(B->err.ptr, 0, sizeof(int));
     if (e != cudaSuccess) {
@@ -2454,7 +2456,7 @@ int pk_batch_create(pk_pool* pool, pk_batch** out) try {
 
 int pk_batch_destroy(pk_batch* B) {
     if (!B) return PK_OK;
-    DeviceScope ds(B->pool->device);
+    DeviceScope ds(B->device);
     B->meta.release();
     B->plan.release();
     if (B->ev_bounded) cudaEventDestroy(B->ev_bounded);

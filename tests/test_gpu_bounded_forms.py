@@ -375,3 +375,23 @@ def test_trim_gives_back_what_idle_batches_and_evictions_hold():
     c.pool.evict([c.tables[1]], [11], 5)
     del b
     assert c.pool.trim() > 0
+
+
+def test_batches_may_outlive_their_pool():
+    """A pool closed before its last batch is dropped: the batch's memory goes without the pool's."""
+    torch = torch_cuda()
+    import gc
+
+    gc.collect()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(4):
+        c = Case("bf16", 40, 8, 64, 16, [3000], [100], weights="replace", poison=False)
+        b = c.batch()
+        b.write_and_attend(0, c.q, c.k, c.v)
+        b.check()
+        assert b.scratch_nbytes > 32 << 20
+        c.pool.close()
+        del b, c
+        gc.collect()
+    assert free - torch.cuda.mem_get_info()[0] <= 24 << 20  # (torch keeps some of the inputs' memory)
