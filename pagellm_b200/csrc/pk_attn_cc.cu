@@ -11,9 +11,11 @@
 // and serve all G heads from one read of K. Every lane group keeps its own running maximum, sum and
 // output; groups and warps are joined once at the end, in a fixed order. With few rows and long
 // contexts the keys are split over CTAs, whose partials the last one to finish joins, in order.
-// Bound by instructions when there are many rows (about 42 per key and warp of 4 keys at D=128, G=4: 32
-// decodes of 4 x 8 heads over 74k float32 tokens with their weights, 604 MB, 272 us, 2.2 TB/s), by the
-// chain row record -> block id -> key -> join when there are few (8 decodes over a small pool: 9 us).
+// Many rows are bound by the latency of the keys' loads: a group of 4 heads of 128 takes 244 registers, so two
+// CTAs share an SM and 8 warps have too few loads in flight (32 decodes of 4 x 8 heads over 74k float32
+// tokens with their weights, 604 MB: 270 us, 2.2 TB/s; issue slots 31 % busy, multiply-add pipe 17 %, the
+// first stall is the load). Few rows are bound by the chain row record -> block id -> key -> join (8 decodes
+// over a small pool: 9 us).
 //
 // Fused append: keys of the step itself are read from the inputs, rounded as the pool stores them,
 // and the CTA of (row, KV head, first group, first split) stores the row. Fused weights (one row per

@@ -8,7 +8,7 @@
 // neighbouring items of a sequence make a pair, so that a K/V tile of 64 keys serves 256 rows. A
 // pair lists the key tiles of the sinks in front of its first row's window, then those from the
 // window on: tiles that nobody sees are neither read nor computed. The (pair, KV head)s are dealt to
-// one CTA per SM, whole where that balances, else cut (build_chunk_schedule).
+// one CTA per SM, whole where that balances, else cut (build_wide_schedule).
 
 #include "pk_device.cuh"
 #include "pk_internal.h"
@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(kCThreads, 1)
                 const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
                                        fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * p.sscale;
                 // Lazy rescale: the base of earlier tiles stays unless this tile's maximum exceeds it by
-                // more than 8 (P stays <= 2^8 in bf16, l and O in fp32).
+                // more than 8 (P stays <= 2^8). P enters the second product in bf16, V's type (half a step,
+                // 2^-8 at most, of each probability); l and O are fp32.
                 const float mnew = (m == -INFINITY || mx > m + 8.f) ? mx : m;
                 const float base = mnew == -INFINITY ? 0.f : mnew;
                 const float corr = m == -INFINITY ? 0.f : ex2_approx(m - base);

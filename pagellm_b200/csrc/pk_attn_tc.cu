@@ -634,6 +634,9 @@ __global__ void __launch_bounds__((kTcMaxKvHeads + 1) * 32, 1)
                     // one vote decides whether anything is rescaled (rarely, once the maximum has been
                     // met), and 2^x is the special-function unit's (relative error 2^-22). Column by
                     // column this took 1350 of a 16-token block's 2800 clocks with two n8 tiles.
+                    // P enters the second product in bf16, as in plain steps (the matrix unit takes two
+                    // equal 16-bit types, and V is bf16): half a step, 2^-8 at most, of each probability;
+                    // the sum l and the weights keep its 32 bits.
                     float mx[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
