@@ -145,9 +145,11 @@ PK_API int pk_batch_create(pk_pool* pool, pk_batch** out);
  * order of the calls, behind the plan's uploads (what they read and write beyond the batch - rows,
  * the pool - is the caller's to order); graphs that were captured from one batch are the caller's to
  * replay one after another, and not while other calls of the batch run. While such a graph exists the
- * batch is not planned again, by pk_batch_plan or by a call with another n_heads (PK_ERR_UNSUPPORTED),
- * and must not be destroyed; pk_batch_graphs counts them (a graph's end may show a moment later). */
+ * batch is not planned again, by pk_batch_plan or by a call with another n_heads (PK_ERR_UNSUPPORTED). */
 PK_API int pk_batch_set_bounds(pk_batch* batch, int64_t window, int64_t sinks, int weights_mode);
+/* CUDA graphs that exist and that calls of the batch, bounded or plain, were captured into (a graph's end
+ * may show a moment later). They read the batch's tables, plan and scratch: a plain batch's graph is good
+ * until its next plan, and no batch may be destroyed before its graphs. */
 PK_API int pk_batch_graphs(const pk_batch* batch, int64_t* graphs);
 PK_API int pk_batch_destroy(pk_batch* batch);
 /* Device memory that the batch holds (no counterpart in pagellm): tables, plan and scratch, which only

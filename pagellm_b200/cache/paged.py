@@ -282,9 +282,8 @@ class PagedKVPool:
         _lib.check(_lib.load().pk_batch_create(self._h.ptr, C.byref(h)))
         return h.value
 
-    def _release_batch(self, h: int, bounded: bool) -> None:
-        # (only bounded calls count the graphs they are captured into)
-        (self._held_batches if bounded and self._graphs_of(h) else self._idle_batches).append(h)
+    def _release_batch(self, h: int) -> None:
+        (self._held_batches if self._graphs_of(h) else self._idle_batches).append(h)
 
     @staticmethod
     def _graphs_of(h: int) -> int:
@@ -455,7 +454,7 @@ class PagedBatch:
         b = getattr(self, "_b", None)
         if b is not None:
             try:
-                self.pool._release_batch(b, self._bounded)
+                self.pool._release_batch(b)
             except Exception:
                 pass
             self._b = None

@@ -389,9 +389,12 @@ struct pk_batch {
     cudaEvent_t ev_bounded = nullptr;
     unsigned long long last_stream = 0;
     bool used = false;
-    // CUDA graphs that bounded calls of this batch were captured into and that still exist (keep_for_graph),
-    // and the last such capture
-    std::shared_ptr<std::atomic<int64_t>> graphs = std::make_shared<std::atomic<int64_t>>(0);
+    // CUDA graphs that calls of this batch were captured into and that still exist (keep_for_graph), those of
+    // bounded calls among them, and the last such capture
+    struct Graphs {
+        std::atomic<int64_t> all{0}, bounded{0};
+    };
+    std::shared_ptr<Graphs> graphs = std::make_shared<Graphs>();
     unsigned long long capture_id = 0;
     bool bounded() const { return window > 0 || weights_mode != 0; }
     int launches = 0;
@@ -1119,25 +1122,31 @@ cudaError_t wait_last(pk_batch* B, cudaStream_t st, unsigned long long id) {
 }
 
 // A captured call's kernels hold the addresses and sizes of the batch's tables, plan and scratch: while the
-// graph (or one instantiated from it) exists, it counts in B->graphs, and the batch is not planned again.
+// graph (or one instantiated from it) exists, it counts in B->graphs. Then a bounded batch is not planned
+// again, and PagedKVPool does not hand its handle out.
 int keep_for_graph(pk_batch* B, cudaStream_t st) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
     cudaGraph_t graph = nullptr;
     PK_CUDA(cudaStreamGetCaptureInfo(st, &status, &id, &graph));
     if (status != cudaStreamCaptureStatusActive || id == B->capture_id) return PK_OK;  // once per capture
-    using Count = std::shared_ptr<std::atomic<int64_t>>;
-    auto gone = [](void* p) {  // when the last of the graph's owners is destroyed; makes no CUDA call
-        Count* count = static_cast<Count*>(p);
-        --**count;
-        delete count;
+    struct Entry {
+        std::shared_ptr<pk_batch::Graphs> graphs;
+        bool bounded;
     };
-    Count* count = new Count(B->graphs);
-    ++**count;
+    auto gone = [](void* p) {  // when the last of the graph's owners is destroyed; makes no CUDA call
+        Entry* entry = static_cast<Entry*>(p);
+        if (entry->bounded) --entry->graphs->bounded;
+        --entry->graphs->all;
+        delete entry;
+    };
+    Entry* entry = new Entry{B->graphs, B->bounded()};
+    ++entry->graphs->all;
+    if (entry->bounded) ++entry->graphs->bounded;
     cudaUserObject_t object = nullptr;
-    cudaError_t e = cudaUserObjectCreate(&object, count, gone, 1, cudaUserObjectNoDestructorSync);
+    cudaError_t e = cudaUserObjectCreate(&object, entry, gone, 1, cudaUserObjectNoDestructorSync);
     if (e != cudaSuccess) {
-        gone(count);
+        gone(entry);
         return fail(PK_ERR_CUDA, "cudaUserObjectCreate: %s", cudaGetErrorString(e));
     }
     e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
@@ -1150,7 +1159,7 @@ int keep_for_graph(pk_batch* B, cudaStream_t st) {
 }
 
 int check_no_graphs(const pk_batch* B) {
-    if (B->graphs->load() > 0)
+    if (B->graphs->bounded.load() > 0)
         return fail(PK_ERR_UNSUPPORTED, "a CUDA graph captured from this batch still exists and reads its plan: use another batch");
     return PK_OK;
 }
@@ -1597,6 +1606,10 @@ int attend_impl(pk_batch* B, int layer, int H, const float* q, float* out, cudaS
         if (rc != PK_OK) return rc;
     }
     if (B->nrows == 0) return PK_OK;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    PK_CUDA(cudaStreamIsCapturing(st, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone)
+        if (int rc = keep_for_graph(B, st)) return rc;
     const int g = H / P->kvh;
     // ---- wide-tile part (side stream when split-KV work runs beside it)
     cudaStream_t ws = st;
@@ -2930,7 +2943,7 @@ int pk_batch_scratch(const pk_batch* B, int64_t* bytes) {
 
 int pk_batch_graphs(const pk_batch* B, int64_t* graphs) {
     if (!B || !graphs) return fail(PK_ERR_INVALID_ARG, "NULL pointer");
-    *graphs = B->graphs->load();
+    *graphs = B->graphs->all.load();
     return PK_OK;
 }
 
@@ -2939,7 +2952,7 @@ int pk_batch_set_prefix_sharing(pk_batch* B, int mode) {
     if (mode < 0 || mode > 2) return fail(PK_ERR_INVALID_ARG, "prefix sharing mode %d not in 0..2", mode);
     if (B->prefix_sharing != mode) {
         B->prefix_sharing = mode;
-        B->plan_H = -1;
+        if (!B->bounded()) B->plan_H = -1;  // (bounded plans share no prefixes)
     }
     return PK_OK;
 }

@@ -257,3 +257,48 @@ def test_a_batch_is_made_before_a_capture():
                 PagedBatch(c.pool, c.tables, c.starts, c.new, **kw)
         torch.cuda.synchronize()
         c.check(c.run())
+
+
+def test_a_plain_graph_keeps_its_dropped_batch():
+    """Plain steps too: a graph goes on replaying after its batch was dropped, others made and the pool trimmed."""
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case("bf16", 8, 2, 128, 16, [700, 300, 90], [1, 1, 80], window=40, poison=False)
+    q, k, v = c.q.float(), c.k.float(), c.v.float()
+    b = PagedBatch(c.pool, c.tables, c.starts, c.new)
+    want = b.write_and_attend(0, q, k, v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b.write_and_attend(0, q, k, v)
+    handle = b._b
+    del b
+    for kw in ({}, dict(window=33)):
+        other = PagedBatch(c.pool, [c.tables[1], c.tables[0]], [200, 9], [1, 70], **kw)
+        assert other._b != handle
+        other.attend(0, q[:71])
+        del other
+    assert c.pool.trim() > 0 and c.pool._held_batches == [handle]
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del graph
+    assert _until(lambda: c.pool._graphs_of(handle) == 0)
+    again = PagedBatch(c.pool, c.tables, c.starts, c.new)
+    assert again._b == handle and torch.equal(again.write_and_attend(0, q, k, v), want)
+
+
+def test_prefix_sharing_does_not_unmake_a_bounded_plan():
+    torch = torch_cuda()
+    c = Case("bf16", 8, 2, 128, 16, [100, 40], [1, 5], window=40, sinks=2)
+    b = c.batch()
+    want = c.run(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = b.write_and_attend(0, c.q, c.k, c.v)
+    b.prefix_sharing = "off"
+    assert torch.equal(c.run(b), want)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
