@@ -249,13 +249,17 @@ class PagedKVPool:
         keep theirs. Waits for the device; returns the bytes."""
         lib = _lib.load()
         n, total = C.c_int64(), 0
-        for h in self._idle_batches:
+        self._recall_held()
+        while True:
+            try:
+                h = self._idle_batches.pop()
+            except IndexError:
+                break
             _lib.check(lib.pk_batch_scratch(h, C.byref(n)))
             total += n.value
             self._batch_prefix_mode.pop(h, None)  # (a later handle may have this address)
             self._batch_bounds.pop(h, None)
             _lib.check(lib.pk_batch_destroy(h))
-        self._idle_batches.clear()
         _lib.check(lib.pk_pool_trim(self._h.ptr, C.byref(n)))
         return total + n.value
 
@@ -272,15 +276,23 @@ class PagedKVPool:
         return self._h.ptr
 
     def _acquire_batch(self) -> int:
-        if self._held_batches:
-            held = self._held_batches
-            self._held_batches = [h for h in held if self._graphs_of(h)]
-            self._idle_batches += [h for h in held if h not in self._held_batches]
-        if self._idle_batches:
+        # (single list operations only: other threads take and give handles at the same time)
+        self._recall_held()
+        try:
             return self._idle_batches.pop()
+        except IndexError:
+            pass
         h = C.c_void_p()
         _lib.check(_lib.load().pk_batch_create(self._h.ptr, C.byref(h)))
         return h.value
+
+    def _recall_held(self) -> None:
+        """Handles whose graphs are gone become idle ones."""
+        for _ in range(len(self._held_batches)):
+            try:
+                self._release_batch(self._held_batches.pop(0))
+            except IndexError:
+                break
 
     def _release_batch(self, h: int) -> None:
         (self._held_batches if self._graphs_of(h) else self._idle_batches).append(h)

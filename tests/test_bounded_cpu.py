@@ -328,6 +328,42 @@ def test_block_ids_do_not_wrap_and_tables_do_not_run_out():
         assert indptr.tolist() == [0, 2, 3] and ids.tolist() == [5, 0, 7] and ids.dtype == np.int32
 
 
+def test_handles_survive_other_threads_between_two_operations(monkeypatch):
+    """What another thread gives or takes while a handle is looked at is neither lost nor handed out twice."""
+    from pagellm_b200.cache import PagedKVPool
+
+    pool = object.__new__(PagedKVPool)
+    pool._idle_batches, pool._held_batches = [], [1, 2, 3]
+    live = {1: 0, 2: 1, 3: 0, 9: 1}
+
+    def graphs_of(h):
+        if h == 1:
+            pool._held_batches.append(9)  # dropped by another thread just now
+        return live[h]
+
+    monkeypatch.setattr(PagedKVPool, "_graphs_of", staticmethod(graphs_of))
+    got = [pool._acquire_batch(), pool._acquire_batch()]
+    assert sorted(got) == [1, 3]
+    assert sorted(pool._held_batches) == [2, 9] and not pool._idle_batches
+
+    class Emptied(list):  # another thread takes the last one after this one has seen it
+        def pop(self, *a):
+            self.clear()
+            raise IndexError
+
+    pool._held_batches, pool._idle_batches = [], Emptied([5])
+
+    class Lib:
+        def pk_batch_create(self, pool, out):
+            out._obj.value = 77
+            return 0
+
+    monkeypatch.setattr(_lib, "load", Lib)
+    pool._h = type("H", (), {"ptr": 1})()
+    assert pool._acquire_batch() == 77
+    pool._idle_batches = []  # nothing for the pool's end to destroy
+
+
 # ------------------------------------------------------------------ C entries
 def test_allocations_that_fail_are_errors():
     """No exception leaves a C entry (which would end the process): a child asks for impossible sizes."""
