@@ -634,7 +634,9 @@ def evict_sequences(pool: PagedKVPool, manager: BlockManager, seq_ids, lengths, 
     block thins it out in place; sequences whose new blocks an earlier one still reads go into
     a later launch. What the pool's eviction refuses (a capturing stream, a head size beyond
     its kernels) is refused before any table changes; an error of the device leaves the
-    sequences of its call without valid caches."""
+    sequences of its call without valid caches. ``OutOfBlocks`` when a shared or published
+    block finds no fresh one: the sequences before that one are shortened all the same, and
+    the exception's ``lengths`` says how long every sequence is now."""
     seq_ids = [int(s) for s in seq_ids]
     lens = np.asarray(lengths, dtype=np.int64).reshape(-1)
     if len(seq_ids) != len(lens):
@@ -665,18 +667,23 @@ def evict_sequences(pool: PagedKVPool, manager: BlockManager, seq_ids, lengths, 
             pool.evict([g[0] for g in todo], [g[2] for g in todo], budget, sinks=sinks, recent=recent,
                        new_tables=[g[1] for g in todo])
 
+    now = lens.copy()
     try:
-        for s, n in zip(seq_ids, lens.tolist()):
+        for i, (s, n) in enumerate(zip(seq_ids, lens.tolist())):
             if n <= budget:
                 continue
             old, new = manager.compact(s, budget)
+            now[i] = budget
             if reads.intersection(new):
                 flush()
             group.append((old, new, n))
             reads.update(old)
+    except OutOfBlocks as e:
+        e.lengths = now
+        raise
     finally:  # sequences compacted before one that found no block are evicted all the same
         flush()
-    return np.minimum(lens, budget)
+    return now
 
 
 def slot_mapping(block_table, positions, block_size: int) -> np.ndarray:

@@ -253,6 +253,19 @@ def test_evict_sequences_runs_what_it_compacted_before_blocks_ran_out():
     assert [c[1] for c in pool.calls] == [[16]]
 
 
+def test_evict_sequences_tells_what_it_shortened_before_blocks_ran_out():
+    bm = BlockManager(8, 4, enable_prefix_caching=False)
+    bm.allocate(1, list(range(12)))  # keeps its three blocks: its table does not show that it was shortened
+    bm.allocate(4, list(range(4)))
+    bm.allocate(2, list(range(12)))
+    bm.fork(2, 3)
+    before = bm.block_table(1)
+    with pytest.raises(OutOfBlocks) as e:
+        evict_sequences(_FakePool(), bm, [1, 4, 2, 3], [12, 4, 12, 12], 9)
+    assert bm.block_table(1) == before
+    assert e.value.lengths.tolist() == [9, 4, 12, 12]
+
+
 @pytest.mark.parametrize("ids, lens, kw", [
     ([1], [4, 4], dict(budget=2)), ([1, 1], [4, 4], dict(budget=2)), ([1], [4], dict(budget=0)),
     ([1], [4], dict(budget=2, sinks=2, recent=1)), ([1], [4], dict(budget=2, sinks=-1)), ([1], [99], dict(budget=2)),
