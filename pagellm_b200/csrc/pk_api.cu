@@ -601,6 +601,7 @@ int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 constexpr int64_t kMinBlocksPerCta = 16;
 constexpr int64_t kUnitsPerCta = 3;
 constexpr int64_t kMaxScoreBytes = int64_t(1) << 30;
+constexpr size_t kMaxKeptBytes = size_t(128) << 20;  // kept positions of an eviction, beyond one layer's
 constexpr int kFuseMaxNew = 1;  // fuse the append only when split-KV sequences add <= 1 token
 
 int64_t split_kv_ctas(int64_t T, int64_t nu, int64_t max_ctas) {
@@ -2370,9 +2371,14 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     if (P->evict_done) PK_CUDA(cudaStreamWaitEvent(st, P->evict_done, 0));
     else PK_CUDA(cudaEventCreateWithFlags(&P->evict_done, cudaEventDisableTiming));
     pk::EvictParams p{};
+    int group = P->n_layers;  // layers of a launch
     if (kept_dev == nullptr) {
-        budget = std::min<int64_t>(budget, std::max(plan.max_len, 1));  // the scratch needs no more places
-        PK_CUDA(P->evict_kept.reserve(static_cast<size_t>(P->n_layers) * nseq * P->kvh * budget * sizeof(int32_t)));
+        // The scratch needs no more places than the longest sequence, and serves all layers at once while
+        // that takes no more than kMaxKeptBytes (an eviction is called when memory is short).
+        budget = std::min<int64_t>(budget, std::max(plan.max_len, 1));
+        const size_t layer_bytes = static_cast<size_t>(nseq) * P->kvh * budget * sizeof(int32_t);
+        group = static_cast<int>(std::min<size_t>(group, std::max<size_t>(1, kMaxKeptBytes / layer_bytes)));
+        PK_CUDA(P->evict_kept.reserve(layer_bytes * group));
         kept_dev = static_cast<int32_t*>(P->evict_kept.ptr);
     }
     Uploader& up = P->evict_up[P->evict_turn++ % 3];
@@ -2398,14 +2404,16 @@ int pk_pool_evict(pk_pool* P, int nseq, const int64_t* table_indptr, const int32
     p.num_blocks = P->num_blocks;
     p.nitems = static_cast<int>(plan.items.size() / 3);
     p.nseq = nseq;
-    p.layers = P->n_layers;
     p.kvh = P->kvh;
     p.bs = bs;
     p.row_bytes = P->d * P->esize;
     p.budget = static_cast<int>(budget);
     p.sinks = static_cast<int>(sinks);
     p.recent = static_cast<int>(recent);
-    PK_CUDA(pk::launch_evict(p, plan.max_len, st));
+    for (p.layer0 = 0; p.layer0 < P->n_layers; p.layer0 += group) {
+        p.layers = std::min(group, P->n_layers - p.layer0);
+        PK_CUDA(pk::launch_evict(p, plan.max_len, st));
+    }
     PK_CUDA(cudaEventRecord(P->evict_done, st));
     return PK_OK;
 } catch (const std::exception& e) {

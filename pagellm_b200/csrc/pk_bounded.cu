@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) evict_select_kernel(con
     const int m = min(n, p.budget);
     const int32_t* tbl = p.ids + p.indptr[i];
     const int32_t* ntbl = p.new_ids + p.new_indptr[i];
-    float* wl = p.weights + static_cast<size_t>(layer) * p.num_blocks * p.kvh * p.bs;
+    float* wl = p.weights + static_cast<size_t>(p.layer0 + layer) * p.num_blocks * p.kvh * p.bs;
     int32_t* kept = p.kept + ((static_cast<size_t>(layer) * p.nseq + i) * p.kvh + h) * p.budget;
     const bool cached = n <= p.cache_cap;
     auto at = [&](const int32_t* t, int j) {
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
     const int h = blockIdx.y % p.kvh, layer = blockIdx.y / p.kvh;
     const int words = p.row_words;
     W* base = static_cast<W*>(blockIdx.z == 0 ? p.pool_k : p.pool_v) +
-              (static_cast<size_t>(layer) * p.num_blocks * p.bs * p.kvh + h) * words;
+              (static_cast<size_t>(p.layer0 + layer) * p.num_blocks * p.bs * p.kvh + h) * words;
     const int32_t* tbl = p.ids + p.indptr[i];
     const int32_t* ntbl = p.new_ids + p.new_indptr[i];
     const int32_t* kept = p.kept + ((static_cast<size_t>(layer) * p.nseq + i) * p.kvh + h) * p.budget;

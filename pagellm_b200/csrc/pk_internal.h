@@ -335,6 +335,7 @@ struct EvictParams {
     int64_t num_blocks;
     int nitems;
     int nseq;
+    int layer0;  // the launch's layers: layer0 .. layer0 + layers - 1 (kept: the first is layer0's)
     int layers;
     int kvh;
     int bs;

@@ -395,3 +395,35 @@ def test_batches_may_outlive_their_pool():
         del b, c
         gc.collect()
     assert free - torch.cuda.mem_get_info()[0] <= 24 << 20  # (torch keeps some of the inputs' memory)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evictions_of_many_positions_take_the_layers_in_groups(in_place):
+    """The scratch of kept positions stays small (175 MB here in one piece): as with the caller's own."""
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedKVPool
+
+    layers, KVH, bs, n, budget = 37, 8, 16, 33000, 31000
+    nb = -(-n // bs)
+    lens = [n, 40, n - 100, n, 0]
+    tables = [np.arange(i * nb, (i + 1) * nb, dtype=np.int32) for i in range(4)] + [np.zeros(0, np.int32)]
+    new = None if in_place else [t + 4 * nb for t in tables]
+    pool = PagedKVPool(Shape(layers, KVH, 2), (4 if in_place else 8) * nb, bs, "bfloat16", track_weights=True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    state = (pool.k, pool.v, pool.weights)
+    for x in state:
+        x.normal_(generator=g)
+    before = [x.clone() for x in state]
+    kept = pool.evict(tables, lens, budget, sinks=4, recent=1000, new_tables=new, return_kept=True)[1]
+    assert kept.numel() * 4 > 128 << 20
+    del kept
+    want = [x.clone() for x in state]
+    assert not torch.equal(want[0], before[0])
+    for x, y in zip(state, before):
+        x.copy_(y)
+    del before
+    pool.trim()
+    assert pool.evict(tables, lens, budget, sinks=4, recent=1000, new_tables=new).tolist() == [budget, 40, budget, budget, 0]
+    for x, y in zip(state, want):
+        assert torch.equal(x, y)
+    assert 0 < pool.trim() <= (128 << 20) * 5 // 4  # (reserved with a quarter more)
