@@ -141,7 +141,7 @@ def test_refused_evictions_leave_the_tables_alone(what):
 
 
 def _until(condition):
-    """A destroyed graph's end is counted by a thread of the driver's."""
+    """A destroyed graph's end is counted a moment later, by a thread of CUDA's."""
     import time
 
     for _ in range(200):
