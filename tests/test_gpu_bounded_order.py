@@ -302,3 +302,55 @@ def test_prefix_sharing_does_not_unmake_a_bounded_plan():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+def test_host_rows_follow_the_tables_too():
+    torch = torch_cuda()
+    from pagellm_b200.cache import PagedBatch
+
+    c = Case("fp32", 8, 2, 64, 16, [100, 333, 40], [1, 1, 80], window=60, sinks=4, weights="replace")
+    PagedBatch(c.pool, [t[::-1].copy() for t in c.tables], c.starts, c.new, window=60)
+    planning, running = torch.cuda.Stream(), torch.cuda.Stream()
+    rows = [x.cpu().numpy() for x in (c.q, c.k, c.v)]
+    torch.cuda.synchronize()
+    _busy(planning)
+    with torch.cuda.stream(planning):
+        b = c.batch()
+    with torch.cuda.stream(running):
+        out = b.write_and_attend(0, *rows)
+    b.check()
+    c.check(torch.from_numpy(out))
+
+
+@pytest.mark.parametrize("bounds, weights", [((60, 4), None), ((60, 4), "replace"), ((None, 0), "replace")])
+@pytest.mark.parametrize("shape", SHAPES + [("bf16", 10, 2, 64, 16)], ids=_shape)
+def test_the_head_exchange_takes_bounded_steps(shape, bounds, weights):
+    """One rank, whose slice is the whole result: on the planning stream and on another."""
+    torch = torch_cuda()
+    import ctypes as C
+
+    from pagellm_b200 import _lib
+    from pagellm_b200.cache.paged import _CudaArray
+
+    lib = _lib.load()
+    c = Case(*shape, [100, 333, 40], [1, 1, 80], window=bounds[0], sinks=bounds[1], weights=weights, io="fp32")
+    b = c.batch()
+    want = c.run(b)
+    gather, own, res = C.c_void_p(), C.create_string_buffer(64), C.c_void_p()
+    _lib.check(lib.pk_peer_gather_create(0, 1, 0, 1 << 22, C.byref(gather)))
+    try:
+        _lib.check(lib.pk_peer_gather_handle(gather, own))
+        _lib.check(lib.pk_peer_gather_open(gather, own.raw))
+        for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+            torch.cuda.synchronize()
+            if weights:
+                c.pool.weights.copy_(c.before)
+                torch.cuda.synchronize()
+            _lib.check(lib.pk_peer_gather_write_and_attend(gather, b._b, 0, c.H, c.q.data_ptr(), c.k.data_ptr(),
+                                                           c.v.data_ptr(), C.byref(res), stream.cuda_stream))
+            _lib.check(lib.pk_peer_gather_check(gather, stream.cuda_stream))
+            got = torch.as_tensor(_CudaArray(res.value, c.q.shape, "<f4", None), device="cuda")
+            assert torch.equal(got, want)
+            c.check(got, q_step=2.0 ** -8 if shape[0] == "bf16" else 0.0)
+    finally:
+        _lib.check(lib.pk_peer_gather_destroy(gather))
